@@ -636,6 +636,73 @@ int sub1_test_slot_pool(int slots, int lost);
  */
 int sub1_unregister_dec(const int32_t *dec);
 
+/*
+ * Microscaled 4-bit matrices (OCP Microscaling Formats 1.0, MXFP4), beside the ternary ones, for layers
+ * that do not stand three values a row.  A row of W values is ceil(W / 32) blocks of 32:
+ *   codes   uint8 [rows, 16 * blocks]   value 2i of a block in the low half of its byte i; a code is a sign
+ *                                       (8) over the magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6.  16-byte aligned
+ *   scales  uint8 [rows, blocks]        the block's scale is 2^(byte - 127); 255: the block is no number
+ * Values behind W in the last block have code 0.  Codes and scales may hold anything: no value of theirs is
+ * followed as an address.  Any width and height from 1 to SUB1_MX4_MAX_WIDTH.
+ */
+#define SUB1_MX4_BF16 0
+#define SUB1_MX4_FP16 1
+#define SUB1_MX4_FP32 2
+#define SUB1_MX4_MAX_WIDTH 65536
+#define SUB1_MX4_MAX_TOKENS (1 << 20)
+
+/*
+ * x [rows, W] of `type`, row stride ldx (elements), to codes and scales.  With m the largest magnitude of a
+ * block the scale is 2^e, e = floor(log2 m) - 2 but not below -127 (m = 0: -127); a value becomes the
+ * nearest of the magnitudes times 2^e (of two the one with an even code; at most 6 * 2^e).  A block that
+ * holds an infinity or something that is no number gets scale 255 and codes 0.
+ * And back: what codes and scales stand for, rounded to `type` (exact in bf16 and fp32), to out [rows, W] of
+ * row stride ldo.
+ */
+int sub1_mx4_quantize(const void *x, int type, int64_t ldx, int64_t rows, int width, uint8_t *codes,
+                      uint8_t *scales, void *stream);
+int sub1_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int width, void *out, int type,
+                        int64_t ldo, void *stream);
+
+/*
+ * y[t, r] = bf16(sum_k W[r, k] x[t, k]) (not accumulated into y), fp32 sums: x bf16 [tokens, width] of row
+ * stride ldx, y bf16 [tokens, height] of row stride ldy.  The second with the activations in the format
+ * too, as sub1_mx4_quantize gives them: x_codes [tokens, 16 * blocks], x_scales [tokens, blocks].
+ */
+int sub1_mx4_product(const uint8_t *codes, const uint8_t *scales, int height, int width, const void *x, int64_t ldx,
+                     void *y, int64_t ldy, int tokens, void *stream);
+int sub1_mx4_product_quantized(const uint8_t *codes, const uint8_t *scales, int height, int width,
+                               const uint8_t *x_codes, const uint8_t *x_scales, void *y, int64_t ldy, int tokens,
+                               void *stream);
+
+/*
+ * A whole sparse MLP for a few tokens (what reference sub1.py:299-321 does around its experts): router,
+ * choice of experts, their two products with ReLU between, weighted sum.
+ *   router     [experts, d_model] of router_type (SUB1_MX4_BF16 or _FP32)
+ *   wi, wo     the experts' matrices in the format above, back to back: [experts * d_ff] rows of width d_model
+ *              and [experts * d_model] rows of width d_ff
+ *   top_k      experts a token, 1..SUB1_MX4_LAYER_TOP_K; normalize: their shares add up to 1
+ *   capacity   0, or with top_k 1: how many tokens of a sequence an expert takes, in their order
+ * x bf16 [tokens, d_model] is tokens / length sequences of `length` tokens.
+ *   logits [t, e] = sum_d x[t, d] router[e, d], summed in 64 bits;
+ *   index [t, :] the experts of the top_k largest, of equal ones the lower first (what is no number comes last);
+ *   p = softmax over all experts at those; h = bf16(relu(wi x)); y[t] = bf16(sum p (wo h)).
+ * A token beyond its expert's capacity keeps its input: y = bf16(p x); `index` names the expert all the same.
+ * `scratch`: sub1_mx4_layer_scratch_bytes(layer, tokens) bytes on 256, of any contents, the call's own until
+ * it has run; nothing is kept in it, so calls on several streams, or captured ones, need one each.
+ */
+#define SUB1_MX4_LAYER_TOKENS 256
+#define SUB1_MX4_LAYER_TOP_K 8
+#define SUB1_MX4_LAYER_EXPERTS 4096
+typedef struct sub1_mx4_layer {
+  const void *router;
+  const uint8_t *wi_codes, *wi_scales, *wo_codes, *wo_scales;
+  int32_t experts, d_model, d_ff, top_k, router_type, normalize, capacity;
+} sub1_mx4_layer;
+int64_t sub1_mx4_layer_scratch_bytes(const sub1_mx4_layer *layer, int tokens);
+int sub1_mx4_layer_forward(const sub1_mx4_layer *layer, const void *x, int tokens, int length, void *y, float *logits,
+                           int64_t *index, void *scratch, int64_t scratch_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,12 @@ PREPARED_MAX_WIDTH = 12288
 STATIC_SCRATCH_BYTES = 1 << 20   # SUB1_STATIC_SCRATCH_BYTES
 STATIC_MAX_TOKENS = 512           # SUB1_STATIC_MAX_TOKENS
 
+MX4_MAX_WIDTH = 65536             # SUB1_MX4_MAX_WIDTH
+MX4_MAX_TOKENS = 1 << 20          # SUB1_MX4_MAX_TOKENS
+MX4_LAYER_TOKENS = 256            # SUB1_MX4_LAYER_TOKENS
+MX4_LAYER_TOP_K = 8               # SUB1_MX4_LAYER_TOP_K
+MX4_LAYER_EXPERTS = 4096          # SUB1_MX4_LAYER_EXPERTS
+
 _vp = ctypes.c_void_p
 _int = ctypes.c_int
 _i64 = ctypes.c_int64
@@ -61,6 +67,14 @@ class Tiles(ctypes.Structure):
     _fields_ = [('meta', _vp), ('entries', _vp), ('meta_bytes', _i64), ('entry_bytes', _i64),
                 ('total_chunks', _i64), ('count', ctypes.c_int32), ('height', ctypes.c_int32),
                 ('width', ctypes.c_int32)]
+
+
+class Mx4Layer(ctypes.Structure):
+    """struct sub1_mx4_layer"""
+    _fields_ = [('router', _vp), ('wi_codes', _vp), ('wi_scales', _vp), ('wo_codes', _vp), ('wo_scales', _vp),
+                ('experts', ctypes.c_int32), ('d_model', ctypes.c_int32), ('d_ff', ctypes.c_int32),
+                ('top_k', ctypes.c_int32), ('router_type', ctypes.c_int32), ('normalize', ctypes.c_int32),
+                ('capacity', ctypes.c_int32)]
 
 
 # every symbol include/sub1_hip.h declares, with its prototype
@@ -118,6 +132,12 @@ PROTOTYPES = {
     'sub1_product_tiles': (_int, [ctypes.POINTER(Tiles), _int, _vp, _i64, _vp, _i64, _int, _vp]),
     'sub1_tiles_decode': (_int, [ctypes.POINTER(Tiles), _int, _vp, _vp]),
     'sub1_route_from_mask': (_int, [_vp, _int, _int, _int, _vp, _vp, _vp]),
+    'sub1_mx4_quantize': (_int, [_vp, _int, _i64, _i64, _int, _vp, _vp, _vp]),
+    'sub1_mx4_dequantize': (_int, [_vp, _vp, _i64, _int, _vp, _int, _i64, _vp]),
+    'sub1_mx4_product': (_int, [_vp, _vp, _int, _int, _vp, _i64, _vp, _i64, _int, _vp]),
+    'sub1_mx4_product_quantized': (_int, [_vp, _vp, _int, _int, _vp, _vp, _vp, _i64, _int, _vp]),
+    'sub1_mx4_layer_scratch_bytes': (_i64, [ctypes.POINTER(Mx4Layer), _int]),
+    'sub1_mx4_layer_forward': (_int, [ctypes.POINTER(Mx4Layer), _vp, _int, _int, _vp, _vp, _vp, _vp, _i64, _vp]),
     'sub1_timing_begin': (_int, [_vp]),
     'sub1_timing_end': (_int, [_vp, ctypes.POINTER(ctypes.c_double)]),
     'sub1_init': (_int, []),

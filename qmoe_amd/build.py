@@ -13,6 +13,8 @@ SOURCES = [os.path.join(HERE, 'csrc', 'sub1_kernels.hip'),
            os.path.join(HERE, 'csrc', 'sub1_pack.hip'),
            os.path.join(HERE, 'csrc', 'sub1_prepared.hip'),
            os.path.join(HERE, 'csrc', 'sub1_tiles.hip'),
+           os.path.join(HERE, 'csrc', 'mx4_matrix.hip'),
+           os.path.join(HERE, 'csrc', 'mx4_layer.hip'),
            os.path.join(HERE, 'csrc', 'sub1_tables.cpp')]
 
 HIPCC_FLAGS = [

@@ -1,0 +1,424 @@
+"""Microscaled 4-bit operators against the oracle in 64 bits: codes, scales and expanded values to the bit,
+products and the sparse MLP within the bounds that the oracle derives (half a step of bf16 where a
+value is rounded to it, half steps of fp32 along a sum)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import mx4_oracle as mo
+from qmoe_amd import _lib, mx4
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def gen(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+def host(t):
+    return t.detach().cpu().double().numpy()
+
+
+def matrix(height, width, seed, spread=0):
+    """(codes, scales) on the GPU and the values they stand for: any codes, scales around 1 / sqrt(width)."""
+    g = gen(seed)
+    nb = mo.blocks_of(width)
+    codes = torch.randint(0, 256, (height, 16 * nb), dtype=torch.uint8, generator=g)
+    behind = torch.arange(32 * nb) >= width                   # values behind the width are zero
+    keep = torch.where(behind[0::2], 0, 15) | torch.where(behind[1::2], 0, 240)
+    codes &= keep.to(torch.uint8)
+    middle = 127 - 2 - int(np.log2(width) / 2)
+    scales = torch.randint(middle - spread, middle + spread + 1, (height, nb), dtype=torch.int64, generator=g).to(torch.uint8)
+    return codes.cuda(), scales.cuda(), mo.dequantize(codes.numpy(), scales.numpy(), width)
+
+
+def activations(tokens, width, seed, strided=False):
+    """bf16; strided: a part of wider rows, NaN around it"""
+    x = torch.randn((tokens, width), generator=gen(seed)).bfloat16()
+    if not strided:
+        return x.cuda()
+    whole = torch.full((tokens, width + 7), float('nan'), dtype=torch.bfloat16)
+    whole[:, 3:3 + width] = x
+    return whole.cuda()[:, 3:3 + width]
+
+
+def within(got, exact, bound):
+    got = host(got)
+    assert got.shape == exact.shape
+    nan = np.isnan(exact)
+    assert np.array_equal(np.isnan(got), nan)
+    off = np.abs(np.where(nan, 0, got) - np.where(nan, 0, exact)) - np.where(nan, 0, bound)
+    assert (off <= 0).all(), 'off by %g beyond its bound at %s' % (off.max(), np.unravel_index(off.argmax(), off.shape))
+
+
+# ------------------------------------------------------- to the format and back ---
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows,width', [(1, 1), (3, 31), (1, 32), (5, 33), (2, 64), (7, 1023), (4, 2080), (300, 97)])
+@pytest.mark.parametrize('strided', [False, True])
+def test_quantize_to_the_bit(dtype, rows, width, strided):
+    g = gen(rows * 1000 + width)
+    x = torch.randn((rows, width), generator=g) * torch.exp2(4 * torch.randn((rows, width), generator=g))
+    x = torch.where(torch.rand((rows, width), generator=g) < 0.3, (x * 4).round() / 4, x).clamp(-6e4, 6e4).to(dtype)
+    if strided:
+        whole = torch.full((rows, width + 9), float('nan'), dtype=dtype, device='cuda')
+        whole[:, 2:2 + width] = x.cuda()
+        codes, scales = mx4.quantize(whole[:, 2:2 + width])
+    else:
+        codes, scales = mx4.quantize(x.cuda())
+    want_codes, want_scales = mo.quantize(host(x))
+    assert np.array_equal(scales.cpu().numpy(), want_scales)
+    assert np.array_equal(codes.cpu().numpy(), want_codes)
+    back = mx4.dequantize(codes, scales, width, dtype)
+    want = torch.from_numpy(mo.dequantize(want_codes, want_scales, width)).to(dtype)
+    assert torch.equal(back.cpu(), want)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_blocks_at_the_ends_of_the_range(dtype):
+    info = torch.finfo(dtype)
+    rows = [[0.0, -0.0], [info.smallest_normal, -info.smallest_normal / 4], [info.tiny * 3, 0.0], [info.max, -info.max / 2],
+            [info.max, 1.0], [float('inf'), 1.0], [-float('inf'), 1.0], [float('nan'), 1.0], [1.0, 0.25], [1.0, -0.125]]
+    for e in (-133, -130, -128, -127, -126, -125, -24, -14, 0, 1, 15, 125):
+        rows += [[s * 2.0 ** e, 2.0 ** e / 3] for s in (1, 1.25, 1.5, 1.75, 1.9, 5, 7, 7.9)]
+    x = torch.zeros((len(rows), 96), dtype=dtype)
+    for i, (a, b) in enumerate(rows):
+        x[i, 32], x[i, 63] = a, b
+        x[i, 1] = 1.5                                          # blocks beside it are as ever
+    codes, scales = mx4.quantize(x.cuda())
+    want_codes, want_scales = mo.quantize(host(x))
+    assert np.array_equal(scales.cpu().numpy(), want_scales) and np.array_equal(codes.cpu().numpy(), want_codes)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_every_code_under_every_scale(dtype):
+    codes = torch.arange(256, dtype=torch.uint8).repeat(256, 1)
+    scales = torch.arange(256, dtype=torch.uint8)[:, None].repeat(1, 16)
+    got = mx4.dequantize(codes.cuda(), scales.cuda(), 512, dtype).cpu()
+    with np.errstate(over='ignore', invalid='ignore'):
+        want = torch.from_numpy(mo.dequantize(codes.numpy(), scales.numpy(), 512)).to(dtype)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(nan=1), want.nan_to_num(nan=1))
+
+
+def test_shapes_and_rows_that_need_a_copy():
+    x = torch.randn((3, 4, 70), generator=gen(5)).cuda()
+    codes, scales = mx4.quantize(x)
+    assert codes.shape == (3, 4, 48) and scales.shape == (3, 4, 3)
+    back = mx4.dequantize(codes, scales, 70, torch.float32)
+    assert back.shape == x.shape
+    for other in (x.transpose(0, 1).contiguous().transpose(0, 1), torch.stack((x, x), -1)[..., 0]):
+        assert torch.equal(mx4.quantize(other)[0], codes) and torch.equal(mx4.quantize(other)[1], scales)
+    row = x[0, 0].expand(5, 70)                                # the same row five times
+    assert torch.equal(mx4.quantize(row)[0], codes[0, 0].expand(5, 48))
+    assert torch.equal(mx4.quantize(x[0, 0])[0], codes[0, 0])
+    for empty in (x[:0], x[:, :0]):
+        codes, scales = mx4.quantize(empty)
+        assert codes.shape == empty.shape[:2] + (48,)
+        assert mx4.dequantize(codes, scales, 70).shape == empty.shape
+    with pytest.raises(TypeError):
+        mx4.quantize(x.double())
+    with pytest.raises(ValueError):
+        mx4.quantize(x[..., :0])
+    with pytest.raises(ValueError):
+        mx4.dequantize(codes, scales, 97)
+
+
+# ------------------------------------------------------------------- products ---
+
+SHAPES = [(1, 1, 1), (16, 32, 1), (17, 33, 2), (3, 127, 16), (48, 129, 17), (100, 1000, 33), (65, 2080, 64), (130, 160, 65),
+          (257, 96, 200), (200, 3001, 13), (300, 515, 300)]
+
+
+@pytest.mark.parametrize('height,width,tokens', SHAPES)
+@pytest.mark.parametrize('strided', [False, True])
+def test_product(height, width, tokens, strided):
+    codes, scales, w = matrix(height, width, height + width, spread=3)
+    x = activations(tokens, width, tokens + width, strided)
+    within(mx4.product(x, codes, scales), *mo.product_bound(host(x), w))
+
+
+@pytest.mark.parametrize('height,width,tokens', SHAPES)
+def test_product_of_two_in_the_format(height, width, tokens):
+    codes, scales, w = matrix(height, width, height + width, spread=3)
+    x_codes, x_scales, x = matrix(tokens, width, tokens + width, spread=2)
+    got = mx4.product_quantized(x_codes, x_scales, codes, scales, width)
+    within(got, *mo.product_bound(x, w))
+
+
+@pytest.mark.parametrize('tokens', [1, 5, 16, 40, 130, 600])
+@pytest.mark.parametrize('quantized', [False, True])
+def test_what_is_no_number_stays_in_its_row(tokens, quantized):
+    height, width = 150, 333
+    codes, scales, w = matrix(height, width, 7)
+    x = activations(tokens, width, 8)
+    x[tokens // 2, 100] = float('inf')
+    x[tokens - 1, width - 1] = float('nan')
+    scales[5, 3] = 255
+    scales[height - 1, mo.blocks_of(width) - 1] = 255
+    layer = mx4.Mx4Linear(codes, scales, width, quantize_activations=quantized)
+    got = host(layer(x))
+    for t in range(tokens):
+        if t == tokens - 1 or (quantized and t == tokens // 2):
+            assert np.isnan(got[t]).all()
+            continue
+        assert np.isnan(got[t, [5, height - 1]]).all()
+        rest = np.delete(got[t], [5, height - 1])
+        assert (~np.isfinite(rest)).all() if t == tokens // 2 else np.isfinite(rest).all()
+
+
+@pytest.mark.parametrize('height,width,tokens', [(50, 100, 3), (50, 100, 40), (333, 200, 300), (16, 64, 129)])
+@pytest.mark.parametrize('quantized', [False, True])
+def test_nothing_is_written_beside_y(height, width, tokens, quantized):
+    """Through the C entry, which takes a row stride for y."""
+    lib = _lib.load()
+    codes, scales, w = matrix(height, width, 9)
+    ldy = height + 5
+    whole = torch.full((tokens + 2, ldy), 7.0, dtype=torch.bfloat16, device='cuda')
+    at = whole.data_ptr() + 2 * ldy
+    stream = torch.cuda.current_stream().cuda_stream
+    x = activations(tokens, width, 10)
+    if quantized:
+        c, s = mx4.quantize(x)
+        x = mx4.dequantize(c, s, width)
+        _lib.check(lib.sub1_mx4_product_quantized(codes.data_ptr(), scales.data_ptr(), height, width, c.data_ptr(), s.data_ptr(),
+                                                  at, ldy, tokens, stream))
+    else:
+        _lib.check(lib.sub1_mx4_product(codes.data_ptr(), scales.data_ptr(), height, width, x.data_ptr(), width, at, ldy, tokens,
+                                        stream))
+    within(whole[1:-1, :height], *mo.product_bound(host(x), w))
+    assert (whole[0] == 7).all() and (whole[-1] == 7).all() and (whole[1:-1, height:] == 7).all()
+
+
+def test_a_few_tokens_get_the_same_bits_whatever_tokens_they_come_with():
+    codes, scales, _ = matrix(200, 1000, 11)
+    x = activations(64, 1000, 12)
+    want = mx4.product(x, codes, scales)
+    for some in (slice(0, 1), slice(3, 8), slice(20, 53), slice(63, 64)):
+        assert torch.equal(mx4.product(x[some], codes, scales), want[some])
+
+
+def test_linear_layers():
+    w = torch.randn((70, 100), generator=gen(13)).cuda()
+    x = activations(12, 100, 14).view(3, 4, 100)
+    for quantized in (False, True):
+        layer = mx4.Mx4Linear.make(w, quantize_activations=quantized)
+        codes, scales = mo.quantize(host(w))
+        assert np.array_equal(layer.codes.cpu().numpy(), codes) and np.array_equal(layer.scales.cpu().numpy(), scales)
+        flat = host(x).reshape(12, 100)
+        if quantized:
+            flat = mo.dequantize(*mo.quantize(flat), 100)
+        exact, bound = mo.product_bound(flat, mo.dequantize(codes, scales, 100))
+        y = layer(x)
+        assert y.shape == (3, 4, 70)
+        within(y.reshape(12, 70), exact, bound)
+        assert layer(x[:0]).shape == (0, 4, 70)
+        again = mx4.Mx4Linear(torch.zeros_like(layer.codes), torch.zeros_like(layer.scales), 100, quantized)
+        again.load_state_dict(layer.state_dict())
+        assert torch.equal(again(x), y)
+        for wrong, error in ((x.float(), TypeError), (x[..., :99], ValueError), (x.cpu(), ValueError)):
+            with pytest.raises(error):
+                layer(wrong)
+
+
+# ----------------------------------------------------------------- the sparse MLP ---
+
+def experts(count, d_model, d_ff, seed):
+    """wi, wo as the layer takes them and as float64"""
+    wi, wo = matrix(count * d_ff, d_model, seed, 1), matrix(count * d_model, d_ff, seed + 1, 1)
+    shaped = [tuple(t.view(count, -1, t.shape[-1]) for t in m[:2]) for m in (wi, wo)]
+    return shaped[0], shaped[1], wi[2].reshape(count, d_ff, d_model), wo[2].reshape(count, d_model, d_ff)
+
+
+def against_the_oracle(layer, hidden, wi, wo):
+    y, (logits, index) = layer(hidden)
+    length = hidden.shape[-2]
+    x = host(hidden).reshape(-1, hidden.shape[-1])
+    exact, bound, want_logits, want_index = mo.sparse_mlp(x, host(layer.router), wi, wo, layer.top_k, layer.normalize,
+                                                          layer.capacity, length)
+    assert y.shape == hidden.shape and y.dtype == torch.bfloat16
+    assert index.shape == hidden.shape[:-1] + (layer.top_k,) and logits.shape == hidden.shape[:-1] + (layer.experts,)
+    assert np.array_equal(index.cpu().numpy().reshape(want_index.shape), want_index)
+    got = logits.cpu().numpy().reshape(want_logits.shape)
+    assert np.array_equal(np.isnan(got), np.isnan(want_logits))
+    # sums in 64 bits, rounded once: at most the neighbour where the sum lies between two
+    assert (np.abs(np.nan_to_num(got) - np.nan_to_num(want_logits)) <= 2.0 ** -23 * np.abs(np.nan_to_num(want_logits))).all()
+    within(y.reshape(-1, y.shape[-1]), exact, bound)
+    return y, logits, index
+
+
+CONFIGS = [
+    # experts, d_model, d_ff, sequences, length, top_k, normalize, capacity, router
+    (1, 1, 1, 1, 1, 1, False, None, torch.float32),
+    (4, 64, 96, 1, 1, 1, False, None, torch.float32),
+    (5, 33, 127, 2, 3, 2, True, None, torch.bfloat16),
+    (7, 130, 250, 3, 7, 1, False, 2, torch.float32),
+    (8, 100, 200, 1, 64, 8, True, None, torch.bfloat16),
+    (3, 128, 64, 16, 16, 2, False, None, torch.float32),
+    (2, 96, 160, 5, 40, 1, False, 11, torch.bfloat16),
+    (200, 40, 70, 9, 7, 3, False, None, torch.float32),
+    (4096, 24, 32, 1, 17, 1, False, None, torch.bfloat16),
+    (64, 2080, 65, 1, 2, 1, False, None, torch.float32),
+    (6, 70, 1300, 300, 1, 2, True, None, torch.float32),       # in two parts
+    (6, 70, 130, 6, 100, 1, False, 20, torch.float32),         # in three, of whole sequences
+]
+
+
+@pytest.mark.parametrize('config', CONFIGS)
+def test_sparse_mlp(config):
+    count, d_model, d_ff, sequences, length, top_k, normalize, capacity, dtype = config
+    wi, wo, dense_wi, dense_wo = experts(count, d_model, d_ff, 20)
+    router = (torch.randn((count, d_model), generator=gen(21)) / d_model ** 0.5).to(dtype).cuda()
+    layer = mx4.Mx4SparseMLP(router, wi, wo, top_k, normalize, capacity)
+    hidden = activations(sequences * length, d_model, 22).view(sequences, length, d_model)
+    y, _, _ = against_the_oracle(layer, hidden, dense_wi, dense_wo)
+    layer.router_outputs = False
+    assert torch.equal(layer(hidden), y)
+    assert torch.equal(layer(hidden.transpose(0, 1).contiguous().transpose(0, 1)), y)
+
+
+def test_equal_logits_and_tokens_that_are_no_numbers():
+    wi, wo, dense_wi, dense_wo = experts(6, 64, 96, 30)
+    router = torch.randn((6, 64), generator=gen(31))
+    router[4] = router[1]
+    router[5] = router[1]
+    router[0] = 0
+    hidden = activations(9, 64, 32).view(1, 9, 64)
+    hidden[0, 2] = 0                                           # all logits are equal
+    hidden[0, 5, 3] = float('nan')
+    hidden[0, 7, 9] = float('inf')
+    for top_k, capacity in ((1, 2), (3, None), (6, None)):
+        layer = mx4.Mx4SparseMLP(router.cuda(), wi, wo, top_k, False, capacity)
+        y, logits, index = layer(hidden)[0], *layer(hidden)[1]
+        want = mo.route(logits[0].cpu().numpy(), top_k)
+        assert np.array_equal(index[0].cpu().numpy(), want)
+        assert want[2].tolist() == list(range(top_k)) and want[5].tolist() == list(range(top_k))
+        assert y[0, 5].isnan().all() and y[0, 7].isnan().all()
+        fine = [0, 1, 2, 3, 4, 6, 8]
+        clean = hidden.clone()
+        clean[0, [5, 7]] = 0.0 if capacity is None else hidden[0, [0, 0]]
+        if capacity is None:
+            against_the_oracle(layer, clean, dense_wi, dense_wo)
+            assert torch.equal(layer(clean)[0][0, fine], y[0, fine])
+
+
+def test_all_tokens_to_one_expert():
+    wi, wo, dense_wi, dense_wo = experts(5, 100, 90, 40)
+    router = torch.zeros((5, 100))
+    router[3] = 1.0
+    hidden = activations(70, 100, 41).abs().view(2, 35, 100)
+    for capacity in (None, 1, 16, 17, 35):
+        layer = mx4.Mx4SparseMLP(router.cuda(), wi, wo, 1, False, capacity)
+        _, _, index = against_the_oracle(layer, hidden, dense_wi, dense_wo)
+        assert (index == 3).all()
+
+
+def test_a_token_gets_the_same_bits_in_every_batch():
+    wi, wo, _, _ = experts(16, 200, 300, 50)
+    router = torch.randn((16, 200), generator=gen(51)).cuda()
+    layer = mx4.Mx4SparseMLP(router, wi, wo, 2, True, router_outputs=False)
+    hidden = activations(256, 200, 52)
+    want = layer(hidden)
+    for some in (slice(0, 1), slice(7, 20), slice(100, 228)):
+        assert torch.equal(layer(hidden[some]), want[some])
+
+
+def test_on_two_streams_and_in_two_graphs():
+    """Two layers' calls on streams of their own at once, and two graphs captured on one stream and
+    replayed on two, between eager calls: every result that of the eager call."""
+    layers, inputs, wants = [], [], []
+    for i in range(2):
+        wi, wo, _, _ = experts(12, 150, 170, 60 + i)
+        router = torch.randn((12, 150), generator=gen(62 + i)).cuda()
+        layers.append(mx4.Mx4SparseMLP(router, wi, wo, 1 + i))
+        inputs.append(activations(40, 150, 64 + i))
+        wants.append(layers[i](inputs[i]))
+    linear = mx4.Mx4Linear(*matrix(90, 150, 66)[:2], 150, quantize_activations=True)
+    linear_want = [linear(x) for x in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+
+    def same(got, i):
+        return torch.equal(got[0], wants[i][0]) and torch.equal(got[1][0], wants[i][1][0]) and torch.equal(got[1][1], wants[i][1][1])
+
+    results = []
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                results.append((i, layers[i](inputs[i])))
+    torch.cuda.synchronize()
+    assert all(same(got, i) for i, got in results)
+    # one layer on both streams at once
+    results = []
+    for _ in range(20):
+        for s in streams:
+            with torch.cuda.stream(s):
+                results.append(layers[0](inputs[0]))
+    torch.cuda.synchronize()
+    assert all(same(got, 0) for got in results)
+    graphs, outputs = [], []
+    static = [x.clone() for x in inputs]
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outputs.append((layers[i](static[i]), linear(static[i])))
+        graphs.append(graph)
+    for turn in range(4):
+        for (y, (logits, index)), z in outputs:
+            for t in (y, logits, index, z):
+                t.zero_()
+        torch.cuda.synchronize()
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                graphs[i].replay()
+        if turn % 2:
+            assert same(layers[0](inputs[0]), 0)
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert same(outputs[i][0], i) and torch.equal(outputs[i][1], linear_want[i])
+
+
+def test_a_dense_switch_layer_brought_to_the_format():
+    """From the module of the installed transformers: its router, its capacity, its experts rounded to the
+    format, against that module with the rounded weights, in fp32."""
+    pytest.importorskip('transformers')
+    from transformers.models.switch_transformers import modeling_switch_transformers as hf
+    cfg = hf.SwitchTransformersConfig(d_model=64, d_ff=160, num_experts=6, expert_capacity=4, num_layers=2,
+                                      num_sparse_encoder_layers=1, num_heads=2, d_kv=16, vocab_size=64,
+                                      router_jitter_noise=0.0, dense_act_fn='relu', dropout_rate=0.0)
+    torch.manual_seed(5)
+    dense = hf.SwitchTransformersSparseMLP(cfg).eval().cuda()
+    for p in dense.parameters():
+        torch.nn.init.normal_(p, std=0.2)
+    layer = mx4.Mx4SparseMLP.from_mlp(dense, router_outputs=False)
+    assert layer.capacity == 4
+    hidden = activations(22, 64, 70).view(2, 11, 64)
+    wi, wo = [np.stack([mo.dequantize(*mo.quantize(host(getattr(e, n).weight)), getattr(e, n).weight.shape[1])
+                        for e in dense.experts.values()]) for n in ('wi', 'wo')]
+    exact, bound, _, index = mo.sparse_mlp(host(hidden).reshape(22, 64), host(dense.router.classifier.weight), wi, wo, 1, False, 4, 11)
+    assert max(np.bincount(index[:11, 0])) > 4                # some tokens keep their input
+    within(layer(hidden).view(22, 64), exact, bound)
+
+
+def test_quantised_layers_in_a_row_as_a_block_runs_them():
+    """A 4-bit projection, the sparse MLP on its result, a 4-bit projection with 4-bit activations."""
+    g = gen(80)
+    first = mx4.Mx4Linear.make(torch.randn((96, 72), generator=g).cuda() / 8)
+    wi, wo, dense_wi, dense_wo = experts(5, 96, 130, 81)
+    mlp = mx4.Mx4SparseMLP(torch.randn((5, 96), generator=g).cuda(), wi, wo, 2, True, router_outputs=False)
+    last = mx4.Mx4Linear.make(torch.randn((40, 96), generator=g).cuda() / 10, quantize_activations=True)
+    x = activations(9, 72, 82)
+    a = first(x)
+    b = mlp(a)
+    c = last(b)
+    values = [mo.dequantize(l.codes.cpu().numpy(), l.scales.cpu().numpy(), l.width) for l in (first, last)]
+    within(a, *mo.product_bound(host(x), values[0]))
+    exact, bound, _, _ = mo.sparse_mlp(host(a), host(mlp.router), dense_wi, dense_wo, 2, True, 0, 9)
+    within(b, exact, bound)
+    within(c, *mo.product_bound(mo.dequantize(*mo.quantize(host(b)), 96), values[1]))
