@@ -43,21 +43,28 @@ __device__ __forceinline__ bf16x8 expand8(uint32_t codes, float scale) {
 }
 
 // Eight 16-bit values from `first` on of a row of `width`; zeros behind its end, whatever
-// lies there.  Rows may begin anywhere.
+// lies there.  Rows may begin anywhere.  Where the end is inside, the row's last eight are read and
+// shifted: one load, as a load for each takes its time eight times over.
 __device__ __forceinline__ u32x4 load8(const uint16_t *row, int first, int width) {
   u32x4 v = {0, 0, 0, 0};
   if (first + 8 <= width) {
     __builtin_memcpy(&v, row + first, 16);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (first + i < width) v[i / 2] |= static_cast<uint32_t>(row[first + i]) << (16 * (i & 1));
+  } else if (first < width) {
+    unsigned __int128 last = 0;
+    if (width >= 8) {
+      __builtin_memcpy(&last, row + width - 8, 16);
+      last >>= 16 * (first + 8 - width);
+    } else {
+      for (int i = first; i < width; i++) last |= static_cast<unsigned __int128>(row[i]) << (16 * (i - first));
+    }
+    v = __builtin_bit_cast(u32x4, last);
   }
   return v;
 }
 
+// to nearest, ties to even (one instruction)
 __device__ __forceinline__ uint32_t two_bf16(float a, float b) {
-  return static_cast<uint32_t>(sub1::f32_to_bf16(a)) | static_cast<uint32_t>(sub1::f32_to_bf16(b)) << 16;
+  return __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(a), static_cast<__bf16>(b)});
 }
 
 // Few tokens: a workgroup of kFewWaves wavefronts multiplies 16 * kRows rows of a matrix with 16 *
@@ -75,7 +82,7 @@ struct FewSums {
 };
 
 // rows: `codes` and `scales` of the first row; `rows` that there are from there on.  x[n] is the row of
-// activations of this lane's token of tile n, null where there is none.
+// activations of this lane's token of tile n (any row where there is none: tokens do not meet).
 template <int kRows, int kTokens>
 __device__ __forceinline__ void few_products(FewSums<kRows, kTokens> &sums, const uint8_t *__restrict__ codes,
                                              const uint8_t *__restrict__ scales, int rows, int width,
@@ -122,10 +129,7 @@ __device__ __forceinline__ void few_products(FewSums<kRows, kTokens> &sums, cons
 #pragma unroll
     for (int n = 0; n < kTokens; n++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        v[n][k] = u32x4{0, 0, 0, 0};
-        if (x[n]) __builtin_memcpy(&v[n][k], x[n] + block * kBlock + 8 * k, 16);
-      }
+      for (int k = 0; k < 4; k++) __builtin_memcpy(&v[n][k], x[n] + block * kBlock + 8 * k, 16);
     multiply(w, s, v);
   }
   if (step < steps) {   // the last, with blocks that end inside it or are not there
@@ -144,10 +148,7 @@ __device__ __forceinline__ void few_products(FewSums<kRows, kTokens> &sums, cons
 #pragma unroll
     for (int n = 0; n < kTokens; n++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        v[n][k] = u32x4{0, 0, 0, 0};
-        if (x[n]) v[n][k] = load8(x[n], block * kBlock + 8 * k, width);
-      }
+      for (int k = 0; k < 4; k++) v[n][k] = load8(x[n], block * kBlock + 8 * k, width);
     multiply(w, s, v);
   }
 }

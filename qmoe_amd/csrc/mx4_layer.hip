@@ -216,7 +216,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_wi_kernel(const LayerArgs 
   uint16_t *h = a.h + pair * width + row0 + 4 * (lane >> 4);
   FewSums<1, 1> sums;
   if (row0 < a.d_ff) {
-    const uint16_t *x[1] = {pair >= 0 ? a.x + pair / a.top_k * a.d_model : nullptr};
+    const uint16_t *x[1] = {a.x + (pair >= 0 ? pair / a.top_k : 0) * a.d_model};
     const int64_t row = static_cast<int64_t>(t.expert) * a.d_ff + row0, blocks = blocks_of(a.d_model);
     few_products<1, 1>(sums, a.wi_codes + row * blocks * kBlockBytes, a.wi_scales + row * blocks, a.d_ff - row0,
                        a.d_model, x);
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_wo_kernel(const LayerArgs 
   if (!tile_of(a, blockIdx.y, t)) return;
   const int lane = threadIdx.x & 63, row0 = blockIdx.x * 16, width = h_width(a), mine = lane & 15;
   const int64_t pair = mine < t.pairs ? a.pairs[t.first + mine] : -1;
-  const uint16_t *x[1] = {pair >= 0 ? a.h + pair * width : nullptr};
+  const uint16_t *x[1] = {a.h + (pair >= 0 ? pair : a.pairs[t.first]) * width};
   const int64_t row = static_cast<int64_t>(t.expert) * a.d_model + row0, blocks = blocks_of(a.d_ff);
   FewSums<1, 1> sums;
   few_products<1, 1>(sums, a.wo_codes + row * blocks * kBlockBytes, a.wo_scales + row * blocks, a.d_model - row0, width,

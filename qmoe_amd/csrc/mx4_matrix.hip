@@ -1,6 +1,8 @@
 // Microscaled 4-bit matrices: values to the format and back, and products with them.
 #include "mx4.h"
 
+#include <type_traits>
+
 using namespace mx4;
 using sub1::fail;
 using sub1::misaligned;
@@ -167,7 +169,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(const ProductAr
 #pragma unroll
   for (int n = 0; n < kTokens; n++) {
     const int token = token0 + 16 * n + (lane & 15);
-    x[n] = token < p.tokens ? p.x + token * p.ldx : nullptr;
+    x[n] = p.x + min(token, p.tokens - 1) * p.ldx;
   }
   FewSums<kRows, kTokens> sums;
   few_products<kRows, kTokens>(sums, p.codes + row0 * blocks * kBlockBytes, p.scales + row0 * blocks, p.height - row0,
@@ -176,6 +178,446 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(const ProductAr
     const int token = token0 + 16 * n + (lane & 15);
     if (token < p.tokens) store_four(p.y + token * p.ldy, row0 + 16 * r + 4 * (lane >> 4), p.height, sum);
   });
+}
+
+// Many tokens: four wavefronts, two by two, each with 32 kRows rows of the matrix and 32 kTokens tokens, 64
+// values of a row a step.  Both sides go through LDS, where two wavefronts read each part.  (A wavefront that
+// fetched its 32 rows' 32 bytes of a step straight into its lanes would touch 32 lines for them, and the L1 takes
+// longer for that than the matrix cores for the products: 300 tokens through 6144 x 2080 19.0 us, so 18.7 and
+// with less in its way below 14.)
+// Lane l multiplies block l / 32 of row l % 32 with that of token l % 32: the k-th of a step's four
+// v_mfma_f32_32x32x16_bf16 takes the k-th eight values of every lane's block.
+template <int kRows, int kTokens>
+struct Many {
+  static constexpr int rows = 64 * kRows, tokens = 64 * kTokens;   // of a workgroup
+};
+
+// The sums of a workgroup's first 256 threads to y, past LDS, so that whole lines of y are written: the lanes
+// have four rows of a token each, 8 bytes of a line.
+template <int kRows, int kTokens>
+__device__ __forceinline__ void store_tile(const f32x16 (&sum)[kRows][kTokens], uint16_t *lds, uint16_t *y, int64_t ldy,
+                                           int row0, int token0, int height, int tokens) {
+  using M = Many<kRows, kTokens>;
+  constexpr int kPitch = M::rows + 8;   // 16 bytes further: neighbouring tokens in other banks
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, in_tile = lane & 31;
+  const bool has_sums = tid < 256;
+#pragma unroll
+  for (int n = 0; n < kTokens; n++)
+#pragma unroll
+    for (int r = 0; r < kRows; r++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if (!has_sums) break;
+        const uint32_t two[2] = {two_bf16(sum[r][n][4 * i], sum[r][n][4 * i + 1]),
+                                 two_bf16(sum[r][n][4 * i + 2], sum[r][n][4 * i + 3])};
+        __builtin_memcpy(__builtin_assume_aligned(
+                             lds + ((wave >> 1) * 32 * kTokens + 32 * n + in_tile) * kPitch +
+                                 ((wave & 1) * kRows + r) * 32 + 8 * i + 4 * half, 8),
+                         two, 8);
+      }
+  __syncthreads();
+  if (!has_sums) return;
+  constexpr int kParts = M::rows / 8, kAtOnce = 256 / kParts;   // parts of 16 bytes of a token, tokens a turn
+  const int row = tid % kParts * 8, rows_left = height - row0 - row;
+  const uint16_t *from = lds + tid / kParts * kPitch + row;
+  uint16_t *to = y + static_cast<int64_t>(token0 + tid / kParts) * ldy + row0 + row;
+  const int tokens_left = tokens - token0 - tid / kParts;
+  if (rows_left >= 8) {
+#pragma unroll 4
+    for (int i = 0; i < M::tokens / kAtOnce; i++) {
+      u32x4 v;
+      __builtin_memcpy(&v, __builtin_assume_aligned(from + i * kAtOnce * kPitch, 16), 16);
+      if (i * kAtOnce < tokens_left) __builtin_memcpy(to + i * kAtOnce * ldy, &v, 16);
+    }
+  } else if (rows_left > 0) {
+    for (int i = 0; i * kAtOnce < min(M::tokens, tokens_left); i++)
+      for (int k = 0; k < rows_left; k++) to[i * kAtOnce * ldy + k] = from[i * kAtOnce * kPitch + k];
+  }
+}
+
+// Through registers: the activations a step at a time, the codes 256 values of a row (128 bytes) at a time, in
+// four quarters of the rows, one a step.
+template <int kRows, int kTokens, int kWaves>
+__global__ __launch_bounds__(256, kWaves) void mx4_many_kernel(const ProductArgs p) {
+  using M = Many<kRows, kTokens>;
+  constexpr int kLoads = M::tokens / 32;                      // of 16 bytes of activations, a thread and step
+  constexpr int kQuarter = M::rows / 4;                       // rows
+  constexpr int kCodes = (kQuarter + 31) / 32;                // loads of 16 bytes of codes, a thread and step
+  // a row's or token's eight parts of 16 bytes, part i at i ^ (row % 8): eight lanes of neighbouring rows
+  // that read the same part find it in different banks
+  __shared__ u32x4 lds_x[2][M::tokens * 8], lds_w[2][M::rows * 8];
+  __shared__ uint8_t lds_s[2][M::rows * 8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, in_tile = lane & 31;
+  const int row0 = blockIdx.x * M::rows, token0 = blockIdx.y * M::tokens;
+  const int blocks = blocks_of(p.width), steps = (blocks + 1) / 2, whole = p.width / 64;
+  const int part = tid & 7, mine = tid >> 3;                  // what this thread fetches: a part of every 32nd row
+  const bool codes_too = kQuarter >= 32 || mine < kQuarter;   // (by whole wavefronts)
+
+  const uint16_t *x_row[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; i++) x_row[i] = p.x + min(token0 + mine + 32 * i, p.tokens - 1) * p.ldx + part * 8;
+
+  struct Step {
+    u32x4 x[kLoads], w[kCodes];
+    uint8_t s[kCodes];
+  };
+  auto load_x = [&](Step &t, int step) {
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) __builtin_memcpy(&t.x[i], x_row[i] + step * 64, 16);
+  };
+  // Quarter j % 4 of the rows' eight blocks from 8 (j / 4) on; blocks behind the last repeat it.
+  auto load_w = [&](Step &t, int j) {
+    if (codes_too) {
+      const int block = min(8 * (j >> 2) + part, blocks - 1);
+#pragma unroll
+      for (int i = 0; i < kCodes; i++) {
+        const int64_t row = min(row0 + (j & 3) * kQuarter + mine + 32 * i, p.height - 1);
+        t.w[i] = *reinterpret_cast<const u32x4 *>(p.codes + (row * blocks + block) * kBlockBytes);
+        t.s[i] = p.scales[row * blocks + block];
+      }
+    }
+  };
+  auto put_x = [&](const Step &t, int side) {
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) lds_x[side][(mine + 32 * i) * 8 + (part ^ (mine >> 1 & 7))] = t.x[i];
+  };
+  auto put_w = [&](const Step &t, int j) {
+    if (codes_too) {
+      const int side = (j >> 2) & 1;
+#pragma unroll
+      for (int i = 0; i < kCodes; i++) {
+        const int row = (j & 3) * kQuarter + mine + 32 * i;
+        lds_w[side][row * 8 + (part ^ (row >> 1 & 7))] = t.w[i];
+        // behind the last block nothing: zeros, with whatever scale its repeated codes had
+        lds_s[side][row * 8 + part] = 8 * (j >> 2) + part < blocks ? t.s[i] : static_cast<uint8_t>(0);
+      }
+    }
+  };
+  f32x16 sum[kRows][kTokens];
+#pragma unroll
+  for (int r = 0; r < kRows; r++)
+#pragma unroll
+    for (int n = 0; n < kTokens; n++) sum[r][n] = f32x16{0};
+
+  auto multiply = [&](int step) {
+    const int side = (step >> 2) & 1, block = 2 * (step & 3) + half;
+    const u32x4 *from = lds_x[step & 1] + ((wave >> 1) * 32 * kTokens + in_tile) * 8;
+    u32x4 w[kRows];
+    float scale[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; r++) {
+      const int row = ((wave & 1) * kRows + r) * 32 + in_tile;
+      w[r] = lds_w[side][row * 8 + (block ^ (row >> 1 & 7))];
+      scale[r] = scale_of(lds_s[side][row * 8 + block]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      bf16x8 a[kRows], b[kTokens];
+#pragma unroll
+      for (int n = 0; n < kTokens; n++)
+        b[n] = __builtin_bit_cast(bf16x8, from[n * 32 * 8 + ((4 * half + k) ^ (in_tile >> 1 & 7))]);
+#pragma unroll
+      for (int r = 0; r < kRows; r++) a[r] = expand8(w[r][k], scale[r]);
+#pragma unroll
+      for (int r = 0; r < kRows; r++)
+#pragma unroll
+        for (int n = 0; n < kTokens; n++)
+          sum[r][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[r], b[n], sum[r][n], 0, 0, 0);
+    }
+  };
+  // In turn `step` are asked for the activations of step + 2 and quarter step + 5 of the codes, and what was asked
+  // for in the turn before goes to LDS behind the products: the activations of step + 1, where nobody has read
+  // since the turn before, and quarter step + 4, whose side was last read in the turn before its first quarter.
+  // (Behind the last whole step that one is asked for again: a branch's end would wait for what is on its way.)
+  auto turn = [&](Step &now, Step &next, int step) {
+    load_x(now, min(step + 2, whole - 1));
+    load_w(now, step + 5);
+    __builtin_amdgcn_sched_barrier(0);   // (asked for here, not where the compiler has them needed)
+    multiply(step);
+    __builtin_amdgcn_sched_barrier(0);
+    put_x(next, (step + 1) & 1);
+    put_w(next, step + 4);
+    __syncthreads();
+  };
+  Step even, odd;
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) {
+    load_w(even, j);
+    load_w(odd, j + 1);
+    put_w(even, j);
+    put_w(odd, j + 1);
+  }
+  if (whole > 0) {
+    load_x(even, 0);
+    load_x(odd, min(1, whole - 1));
+    load_w(odd, 4);
+    put_x(even, 0);
+  }
+  __syncthreads();
+  if (whole > 0) {
+    int step = 0;
+    for (; step + 2 <= whole; step += 2) {
+      turn(even, odd, step);
+      turn(odd, even, step + 1);
+    }
+    if (step < whole) turn(even, odd, step);
+  }
+  if (whole < steps) {   // the last step, where the row ends inside it: its codes are there
+        for (int i = 0; i < kLoads; i++)
+      lds_x[whole & 1][(mine + 32 * i) * 8 + (part ^ (mine >> 1 & 7))] =
+          load8(p.x + min(token0 + mine + 32 * i, p.tokens - 1) * p.ldx, whole * 64 + part * 8, p.width);
+    __syncthreads();
+    multiply(whole);
+  }
+  __syncthreads();
+  store_tile<kRows, kTokens>(sum, reinterpret_cast<uint16_t *>(lds_x), p.y, p.ldy, row0, token0, p.height, p.tokens);
+}
+
+typedef __attribute__((address_space(3))) unsigned char *lds_bytes;
+__device__ __forceinline__ uint32_t lds_address(void *p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_bytes)p));
+}
+
+// 16 bytes a lane, or one byte (as 32 bits), from base + at into LDS, the lanes' back to back from `to` on.  The
+// compiler is not told what these are: it would let every read of LDS wait for all that is on its way
+// there, the steps after the next among it.  Their caller counts them, waits and meets the others (meet()).
+__device__ __forceinline__ void fetch(const void *base, uint32_t at, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(at), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void fetch_byte(const void *base, uint32_t at, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(to), "v"(at), "s"(base) : "memory", "m0");
+}
+// Waits until at most kLeft of this wavefront's loads are on their way, then for the other wavefronts.
+template <int kLeft>
+__device__ __forceinline__ void meet() {
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kLeft) : "memory");
+}
+
+// Straight into LDS, three steps of activations and three pairs of steps of codes and scales, each asked for two
+// steps or more ahead: no registers hold what is on its way, and a wavefront's turn is its reads of LDS and its
+// products (a 128 x 128 tile's turn 0.47 us, through registers 0.67; its MFMAs alone take 0.21).  What bounds it
+// with two workgroups a compute unit: LDS and L1 are each busy for more than half of the MFMAs' time, and their
+// wavefronts meet once a step (4096 x 4096 x 4096 124 us, 1.1 PFLOP/s; of 1.3 that a library product in bf16
+// reaches at twice that size).
+// kParts groups of four wavefronts share a tile's steps, where tiles alone would leave compute units idle.
+template <int kRows, int kTokens, int kParts, int kWaves>
+__global__ __launch_bounds__(256 * kParts, kWaves) void mx4_many_direct_kernel(const ProductArgs p) {
+  using M = Many<kRows, kTokens>;
+  constexpr int kLoads = M::tokens / 32;    // fetches of activations, a wavefront and step
+  constexpr int kStepBytes = M::tokens * 128, kPairBytes = M::rows * 64, kCodes = 3 * kStepBytes,
+                kScaleBytes = M::rows * 16, kScales = kCodes + 3 * kPairBytes,
+                kPartBytes = kScales + 3 * kScaleBytes;
+  // three steps of activations: a token's eight parts of 16 bytes, part i at i ^ (token / 2 % 8); three pairs of
+  // steps of codes: a row's four parts, part i at i ^ (row / 4 % 4); and of scales, 32 bits each
+  __shared__ u32x4 all_lds[kParts * kPartBytes / 16];
+  const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int which_part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  u32x4 *const lds = all_lds + which_part * (kPartBytes / 16);
+  const int half = lane >> 5, in_tile = lane & 31;
+  const int row0 = blockIdx.x * M::rows, token0 = blockIdx.y * M::tokens;
+  const int blocks = blocks_of(p.width), steps = (blocks + 1) / 2, whole = p.width / 64;
+
+  // the part's steps: as many turns for each part, those behind the last step without products
+  const int turns = kParts == 1 ? whole : (whole + 2 * kParts - 1) / (2 * kParts) * 2;
+  const int first_step = which_part * turns, my_steps = kParts == 1 ? whole : min(turns, whole - first_step);
+
+  // what this lane fetches, from the tile's first token and row on: a tile's activations span less than 4 GB
+  const uint16_t *x_tile = p.x + token0 * p.ldx;
+  const uint8_t *code_tile = p.codes + static_cast<int64_t>(row0) * blocks * kBlockBytes;
+  const uint8_t *scale_tile = p.scales + static_cast<int64_t>(row0) * blocks;
+  uint32_t x_at[kLoads], block_at[kRows];
+#pragma unroll
+  for (int i = 0; i < kLoads; i++)
+    x_at[i] = static_cast<uint32_t>(min((i * 4 + wave) * 8 + (lane >> 3), p.tokens - 1 - token0)) *
+                  static_cast<uint32_t>(p.ldx * 2) + ((lane & 7) ^ (4 * (wave & 1) + (lane >> 4))) * 16;
+  const int code_part = (lane & 3) ^ (lane >> 4);
+#pragma unroll
+  for (int q = 0; q < kRows; q++) block_at[q] = min((q * 4 + wave) * 16 + (lane >> 2), p.height - 1 - row0) * blocks;
+  const uint32_t lds_at = lds_address(lds);
+  auto fetch_x = [&](int side, int step) {
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) fetch(x_tile + step * 64, x_at[i], lds_at + side * kStepBytes + (i * 4 + wave) * 1024);
+  };
+  // 64 rows, those of `q`, of the four blocks from 4 pair on; blocks behind the last repeat it
+  auto fetch_w = [&](int side, int pair, int q) {
+    fetch(code_tile, (block_at[q] + min(4 * pair + code_part, blocks - 1)) * kBlockBytes,
+          lds_at + kCodes + side * kPairBytes + (q * 4 + wave) * 1024);
+    fetch_byte(scale_tile, block_at[q] + min(4 * pair + (lane & 3), blocks - 1),
+               lds_at + kScales + side * kScaleBytes + (q * 4 + wave) * 256);
+  };
+
+  f32x16 sum[kRows][kTokens];
+#pragma unroll
+  for (int r = 0; r < kRows; r++)
+#pragma unroll
+    for (int n = 0; n < kTokens; n++) sum[r][n] = f32x16{0};
+
+  auto multiply = [&](int x_side, int w_side, int q) {
+    const u32x4 *x = lds + (x_side * kStepBytes + (wave >> 1) * kTokens * 4096 + in_tile * 128) / 16;
+    const u32x4 *codes = lds + (kCodes + w_side * kPairBytes + (wave & 1) * kRows * 2048 + in_tile * 64) / 16;
+    const uint32_t *scales = reinterpret_cast<const uint32_t *>(lds) +
+                             (kScales + w_side * kScaleBytes + (wave & 1) * kRows * 512 + in_tile * 16) / 4;
+    u32x4 w[kRows];
+    float scale[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; r++) {
+      w[r] = codes[r * 128 + ((2 * q + half) ^ (in_tile >> 2 & 3))];
+      scale[r] = scale_of(scales[r * 128 + 2 * q + half]);
+    }
+    bf16x8 b[2][kTokens];
+    auto read = [&](int k) {
+#pragma unroll
+      for (int n = 0; n < kTokens; n++)
+        b[k & 1][n] = __builtin_bit_cast(bf16x8, x[n * 256 + ((4 * half + k) ^ (in_tile >> 1 & 7))]);
+    };
+    read(0);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      if (k < 3) read(k + 1);   // ahead of the products before it, where the compiler would not put it
+      __builtin_amdgcn_sched_barrier(0);
+      bf16x8 a[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; r++) a[r] = expand8(w[r][k], scale[r]);
+#pragma unroll
+      for (int r = 0; r < kRows; r++)
+#pragma unroll
+        for (int n = 0; n < kTokens; n++)
+          sum[r][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[r], b[k & 1][n], sum[r][n], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Turn `step` asks for the activations of step + 2, whose place was read in the turn before, and for 64 rows'
+  // codes of the pair after the next, whose place was read in the pair before; it waits for all that was
+  // asked for before the last turn, its own step among it.
+  auto turn = [&](auto number, int step) {
+    constexpr int kTurn = decltype(number)::value, q = kTurn & 1;
+    meet<kLoads + ((q ^ 1) < kRows ? 2 : 0)>();   // but for what the last turn asked for
+    if (q < kRows) fetch_w((kTurn / 2 + 2) % 3, ((first_step + step) >> 1) + 2, q);
+    fetch_x((kTurn + 2) % 3, min(first_step + step + 2, whole - 1));
+    if (kParts == 1 || step < my_steps) multiply(kTurn % 3, kTurn / 2 % 3, q);
+  };
+#pragma unroll
+  for (int q = 0; q < kRows; q++) {
+    fetch_w(0, first_step >> 1, q);
+    fetch_w(1, (first_step >> 1) + 1, q);
+  }
+  fetch_x(0, min(first_step, whole - 1));
+  fetch_x(1, min(first_step + 1, whole - 1));
+  meet<0>();
+  int step = 0;
+  for (;;) {
+    turn(std::integral_constant<int, 0>{}, step);
+    if (++step == turns) break;
+    turn(std::integral_constant<int, 1>{}, step);
+    if (++step == turns) break;
+    turn(std::integral_constant<int, 2>{}, step);
+    if (++step == turns) break;
+    turn(std::integral_constant<int, 3>{}, step);
+    if (++step == turns) break;
+    turn(std::integral_constant<int, 4>{}, step);
+    if (++step == turns) break;
+    turn(std::integral_constant<int, 5>{}, step);
+    if (++step == turns) break;
+  }
+  meet<0>();   // nothing is on its way into LDS any more
+  if (whole < steps) {   // the last step, where the row ends inside it: its activations go where step 0's were
+    const int part = tid & 7, mine = tid >> 3;
+    for (int i = 0; i < kLoads; i++)
+      lds[(mine + 32 * i) * 8 + (part ^ (mine >> 1 & 7))] =
+          load8(p.x + min(token0 + mine + 32 * i, p.tokens - 1) * p.ldx, whole * 64 + part * 8, p.width);
+    // and its codes and scales, both blocks, where the first pair's were
+    if (tid < M::rows) {
+      const int64_t row = min(row0 + tid, p.height - 1) * static_cast<int64_t>(blocks);
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const bool there = 2 * whole + i < blocks;
+        const int64_t block = row + min(2 * whole + i, blocks - 1);
+        lds[(kCodes + tid * 64) / 16 + (i ^ (tid >> 2 & 3))] = *reinterpret_cast<const u32x4 *>(p.codes + block * kBlockBytes);
+        reinterpret_cast<uint32_t *>(lds)[(kScales + tid * 16) / 4 + i] = there ? p.scales[block] : 0;
+      }
+    }
+    __syncthreads();
+    if (kParts == 1 || which_part == kParts - 1) multiply(0, 0, 0);
+  }
+  __syncthreads();
+  if constexpr (kParts > 1) {   // the parts' sums, added in their order
+    f32x4 *sums = reinterpret_cast<f32x4 *>(all_lds);
+    constexpr int kFours = 4 * kRows * kTokens;
+    if (which_part) {
+#pragma unroll
+      for (int i = 0; i < kFours; i++) {
+        const f32x16 &v = sum[i / 4 / kTokens][i / 4 % kTokens];
+        sums[((which_part - 1) * kFours + i) * 256 + tid] =
+            f32x4{v[i % 4 * 4], v[i % 4 * 4 + 1], v[i % 4 * 4 + 2], v[i % 4 * 4 + 3]};
+      }
+    }
+    __syncthreads();
+    if (which_part == 0) {
+#pragma unroll
+      for (int other = 0; other < kParts - 1; other++)
+#pragma unroll
+        for (int i = 0; i < kFours; i++) {
+          const f32x4 v = sums[(other * kFours + i) * 256 + tid];
+#pragma unroll
+          for (int k = 0; k < 4; k++) sum[i / 4 / kTokens][i / 4 % kTokens][i % 4 * 4 + k] += v[k];
+        }
+    }
+    __syncthreads();
+  }
+  store_tile<kRows, kTokens>(sum, reinterpret_cast<uint16_t *>(all_lds), p.y, p.ldy, row0, token0, p.height, p.tokens);
+}
+
+template <int kRows, int kTokens, int kParts, int kWaves>
+void launch_direct(const ProductArgs &p, hipStream_t s) {
+  using M = Many<kRows, kTokens>;
+  mx4_many_direct_kernel<kRows, kTokens, kParts, kWaves>
+      <<<dim3((p.height + M::rows - 1) / M::rows, (p.tokens + M::tokens - 1) / M::tokens), 256 * kParts, 0, s>>>(p);
+}
+
+template <int kRows, int kTokens, int kWaves>
+void launch_many(const ProductArgs &p, hipStream_t s) {
+  using M = Many<kRows, kTokens>;
+  mx4_many_kernel<kRows, kTokens, kWaves><<<dim3((p.height + M::rows - 1) / M::rows, (p.tokens + M::tokens - 1) / M::tokens),
+                                    256, 0, s>>>(p);
+}
+
+// Which kernel, by what was measured on matrices of 600 x 2500 to 6144 x 2080 (us, one after the other in a graph):
+// up to 32 tokens, where a wavefront takes rows and all their lines (24 tokens through 4096 x 1024 4.3, shared
+// activations 5.1), two row tiles a wavefront once one makes more than a workgroup a compute unit (32 through 6144
+// x 2080 6.5, one 8.7; through 2080 x 6144 18.0 and 15.3).  Then tiles of 64 x 64, as there are few of them
+// shared by four, two or one group of four wavefronts (70 through 2080 x 6144, 66 tiles: 13.7, 15.7, 20.5; 200
+// through 4096 x 1024, 256 tiles: 5.9, 5.5, 5.9; 568, 576 tiles: 14.3, 10.9, 8.9), and of 128 x 128 from four
+// of the small ones a compute unit on (2272 through 6144 x 2080, 3456 tiles: 72, small ones 94).
+// Activations whose rows do not lie on 16 bytes cannot be fetched into LDS and go through registers
+// (2272 through 6144 x 2080 86, 568 through 4096 x 1024 13.3).
+void launch_product(const ProductArgs &p, hipStream_t s) {
+  const int64_t small_tiles = static_cast<int64_t>((p.height + 63) / 64) * ((p.tokens + 63) / 64);
+  const unsigned rows = (p.height + 15) / 16;
+  if (p.tokens <= 32 || p.width < 64) {
+    sub1::note_kernel("mx4_few_kernel");
+    if (p.tokens <= 16)
+      mx4_few_kernel<1, 1><<<dim3(rows, 1), 64 * kFewWaves, 0, s>>>(p);
+    else if (rows <= 256)
+      mx4_few_kernel<1, 2><<<dim3(rows, (p.tokens + 31) / 32), 64 * kFewWaves, 0, s>>>(p);
+    else
+      mx4_few_kernel<2, 2><<<dim3((rows + 1) / 2, (p.tokens + 31) / 32), 64 * kFewWaves, 0, s>>>(p);
+  } else if (misaligned(p.x, 16) || p.ldx % 8 || p.ldx >= 1 << 23) {
+    sub1::note_kernel("mx4_many_kernel");
+    if (small_tiles < 1024)
+      launch_many<1, 1, 4>(p, s);
+    else
+      launch_many<2, 2, 2>(p, s);
+  } else {
+    sub1::note_kernel("mx4_many_direct_kernel");
+    if (small_tiles <= 96)
+      launch_direct<1, 1, 4, 4>(p, s);
+    else if (small_tiles <= 320)
+      launch_direct<1, 1, 2, 4>(p, s);
+    else if (small_tiles < 1024)
+      launch_direct<1, 1, 1, 4>(p, s);
+    else
+      launch_direct<2, 2, 1, 2>(p, s);
+  }
 }
 
 struct QuantizedArgs {
@@ -303,12 +745,7 @@ extern "C" int sub1_mx4_product(const uint8_t *codes, const uint8_t *scales, int
   hipStream_t s = static_cast<hipStream_t>(stream);
   const ProductArgs p{codes, scales, static_cast<const uint16_t *>(x), static_cast<uint16_t *>(y), ldx, ldy, height,
                       width, tokens};
-  const unsigned rows = (height + 15) / 16;
-  sub1::note_kernel("mx4_few_kernel");
-  if (tokens <= 16)
-    mx4_few_kernel<1, 1><<<dim3(rows, 1), 64 * kFewWaves, 0, s>>>(p);
-  else
-    mx4_few_kernel<1, 2><<<dim3(rows, (tokens + 31) / 32), 64 * kFewWaves, 0, s>>>(p);
+  launch_product(p, s);
   HIP_TRY(hipGetLastError());
   return SUB1_OK;
 }

@@ -133,7 +133,8 @@ def test_shapes_and_rows_that_need_a_copy():
 # ------------------------------------------------------------------- products ---
 
 SHAPES = [(1, 1, 1), (16, 32, 1), (17, 33, 2), (3, 127, 16), (48, 129, 17), (100, 1000, 33), (65, 2080, 64), (130, 160, 65),
-          (257, 96, 200), (200, 3001, 13), (300, 515, 300)]
+          (257, 96, 200), (200, 3001, 13), (300, 515, 300), (40, 64, 70), (40, 63, 70), (4100, 96, 30), (1000, 1056, 700),
+          (3000, 416, 1100), (2050, 2080, 2100)]
 
 
 @pytest.mark.parametrize('height,width,tokens', SHAPES)
@@ -196,11 +197,24 @@ def test_nothing_is_written_beside_y(height, width, tokens, quantized):
     assert (whole[0] == 7).all() and (whole[-1] == 7).all() and (whole[1:-1, height:] == 7).all()
 
 
+def test_the_forms_of_the_product():
+    """Which kernel a call takes, at the sizes where the choice turns."""
+    lib = _lib.load()
+    for tokens, height, width, strided, name in (
+            (32, 700, 128, False, b'mx4_few_kernel'), (33, 700, 128, False, b'mx4_many_direct_kernel'),
+            (33, 700, 63, False, b'mx4_few_kernel'), (33, 700, 128, True, b'mx4_many_kernel')):
+        codes, scales, w = matrix(height, width, tokens)
+        x = activations(tokens, width, tokens + 1, strided)
+        y = mx4.product(x, codes, scales)
+        assert lib.sub1_last_kernel() == name
+        within(y, *mo.product_bound(host(x), w))
+
+
 def test_a_few_tokens_get_the_same_bits_whatever_tokens_they_come_with():
     codes, scales, _ = matrix(200, 1000, 11)
-    x = activations(64, 1000, 12)
+    x = activations(32, 1000, 12)
     want = mx4.product(x, codes, scales)
-    for some in (slice(0, 1), slice(3, 8), slice(20, 53), slice(63, 64)):
+    for some in (slice(0, 1), slice(3, 8), slice(9, 30), slice(31, 32)):
         assert torch.equal(mx4.product(x[some], codes, scales), want[some])
 
 
