@@ -387,10 +387,11 @@ __device__ __forceinline__ void fetch(const void *base, uint32_t at, uint32_t to
 __device__ __forceinline__ void fetch_byte(const void *base, uint32_t at, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(to), "v"(at), "s"(base) : "memory", "m0");
 }
-// Waits until at most kLeft of this wavefront's loads are on their way, then for the other wavefronts.
+// Waits until at most kLeft of this wavefront's loads are on their way and it has done with LDS, then for the other
+// wavefronts.
 template <int kLeft>
 __device__ __forceinline__ void meet() {
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kLeft) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
 }
 
 // Straight into LDS, three steps of activations and three pairs of steps of codes and scales, each asked for two
@@ -581,6 +582,268 @@ void launch_many(const ProductArgs &p, hipStream_t s) {
                                     256, 0, s>>>(p);
 }
 
+struct QuantizedArgs {
+  const uint8_t *codes, *scales, *x_codes, *x_scales;
+  uint16_t *y;
+  int64_t ldy;
+  int height, width, tokens;
+};
+
+// sixteen bytes of codes as the scaled MFMAs take an operand of any of their types
+__device__ __forceinline__ i32x8 wide(u32x4 v) {
+  return i32x8{static_cast<int>(v[0]), static_cast<int>(v[1]), static_cast<int>(v[2]), static_cast<int>(v[3]), 0, 0, 0, 0};
+}
+
+// Both sides in the format, many tokens: kSides by four wavefronts, each with 128 rows of the matrix and 64 tokens,
+// 128 values of a row a step, as mx4_many_direct_kernel fetches them; v_mfma_scale_f32_32x32x64_f8f6f4 takes a lane's
+// block of 32 values as it is, and one byte of a register for its scale.  The scales come through registers, a
+// row's eight at a time: of one byte each they would be too many fetches, and of four they do not lie on four.
+// That load's wait is the compiler's, which waits for all fetches; it costs an eighth of the time (8192 x 8192 x 8192
+// 293 us, 3.8 PFLOP/s; without scales 256; the matrix cores are busy for 45 % of it, at 8.8 PFLOP/s).
+template <int kSides>
+__global__ __launch_bounds__(256 * kSides, 2) void mx4_both_kernel(const QuantizedArgs p) {
+  constexpr int kBothRows = 128 * kSides, kBothTokens = 256, kThreads = 256 * kSides, kWaves = 4 * kSides;
+  constexpr int kXFetches = 4 / kSides, kScaleRows = kBothRows + kBothTokens;
+  constexpr int kStepBytes = (kBothRows + kBothTokens) * 64, kScales = 3 * kStepBytes, kScaleBytes = (kBothRows + kBothTokens) * 8;
+  // three steps of codes, rows first, then tokens: four parts of 16 bytes, part i at i ^ (row / 4 % 4); two
+  // pairs of steps of scales, eight bytes a row
+  __shared__ u32x4 lds[(kScales + 2 * kScaleBytes) / 16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5, in_tile = lane & 31, row_side = wave % kSides, token_side = wave / kSides;
+  const int row0 = blockIdx.x * kBothRows, token0 = blockIdx.y * kBothTokens;
+  const int blocks = blocks_of(p.width), steps = (blocks + 3) / 4;
+  const uint8_t *code_tile = p.codes + static_cast<int64_t>(row0) * blocks * kBlockBytes;
+  const uint8_t *x_tile = p.x_codes + static_cast<int64_t>(token0) * blocks * kBlockBytes;
+  const uint32_t lds_at = lds_address(lds);
+
+  // what this lane fetches of a step: 16 rows' 64 bytes a fetch
+  const int part = (lane & 3) ^ (lane >> 4);
+  uint32_t w_at[2], x_at[kXFetches];
+#pragma unroll
+  for (int i = 0; i < 2; i++) w_at[i] = min((i * kWaves + wave) * 16 + (lane >> 2), p.height - 1 - row0) * blocks;
+#pragma unroll
+  for (int i = 0; i < kXFetches; i++)
+    x_at[i] = min((i * kWaves + wave) * 16 + (lane >> 2), p.tokens - 1 - token0) * blocks;
+  auto fetch_step = [&](int side, int step) {
+    const int block = min(4 * step + part, blocks - 1);
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+      fetch(code_tile, (w_at[i] + block) * kBlockBytes, lds_at + side * kStepBytes + (i * kWaves + wave) * 1024);
+#pragma unroll
+    for (int i = 0; i < kXFetches; i++)
+      fetch(x_tile, (x_at[i] + block) * kBlockBytes, lds_at + side * kStepBytes + kBothRows * 64 + (i * kWaves + wave) * 1024);
+  };
+  // a token's and a row's scales of eight blocks, or of its last eight (the caller's width has as many): each thread has a
+  // token or a row, or where there are more of them a token and the first half a row too
+  constexpr bool kTwo = kScaleRows > kThreads;
+  const bool is_token = kTwo || tid >= kBothRows, row_too = kTwo && tid < kBothRows;
+  const int my_row = kTwo ? tid : tid - kBothRows;
+  const uint8_t *row_scales = p.scales + static_cast<int64_t>(min(row0 + min(tid, kBothRows - 1), p.height - 1)) * blocks;
+  const uint8_t *first_scales =
+      is_token ? p.x_scales + static_cast<int64_t>(min(token0 + my_row, p.tokens - 1)) * blocks : row_scales;
+  struct Scales {
+    uint64_t first, second;
+  };
+  auto load_scales = [&](int pair) {
+    Scales v;
+    __builtin_memcpy(&v.first, first_scales + min(8 * pair, blocks - 8), 8);
+    if (kTwo) __builtin_memcpy(&v.second, row_scales + min(8 * pair, blocks - 8), 8);
+    return v;
+  };
+  auto put_scales = [&](int side, int pair, const Scales &v) {   // zeros behind the last
+    const int behind = min(8 * max(8 * pair + 8 - blocks, 0), 63);
+    uint64_t *to = reinterpret_cast<uint64_t *>(lds) + (kScales + side * kScaleBytes) / 8;
+    to[is_token ? kBothRows + my_row : tid] = v.first >> behind;
+    if (row_too) to[tid] = v.second >> behind;
+  };
+
+  f32x16 sum[4][2];
+#pragma unroll
+  for (int r = 0; r < 4; r++)
+#pragma unroll
+    for (int n = 0; n < 2; n++) sum[r][n] = f32x16{0};
+
+  auto multiply = [&](int side, int scale_side, auto which) {
+    constexpr int q = decltype(which)::value;   // the step's place in its pair
+    const u32x4 *w = lds + (side * kStepBytes + row_side * 128 * 64 + in_tile * 64) / 16;
+    const u32x4 *x = lds + (side * kStepBytes + kBothRows * 64 + token_side * 64 * 64 + in_tile * 64) / 16;
+    const uint64_t *scales = reinterpret_cast<const uint64_t *>(lds) + (kScales + scale_side * kScaleBytes) / 8 + in_tile;
+    uint32_t ws[4], xs[2];   // of this half's blocks: bytes 0 and 2
+#pragma unroll
+    for (int r = 0; r < 4; r++) ws[r] = static_cast<uint32_t>(scales[row_side * 128 + r * 32] >> (32 * q)) >> (8 * half);
+#pragma unroll
+    for (int n = 0; n < 2; n++)
+      xs[n] = static_cast<uint32_t>(scales[kBothRows + token_side * 64 + n * 32] >> (32 * q)) >> (8 * half);
+    u32x4 a[2][4], b[2][2];
+    auto read = [&](int k) {
+      const int at = (2 * k + half) ^ (in_tile >> 2 & 3);
+#pragma unroll
+      for (int r = 0; r < 4; r++) a[k][r] = w[r * 128 + at];
+#pragma unroll
+      for (int n = 0; n < 2; n++) b[k][n] = x[n * 128 + at];
+    };
+    read(0);
+    __builtin_amdgcn_sched_barrier(0);
+    read(1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+        sum[r][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a[0][r]), wide(b[0][n]), sum[r][n], 4, 4, 0, ws[r], 0, xs[n]);
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+        sum[r][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a[1][r]), wide(b[1][n]), sum[r][n], 4, 4, 2, ws[r], 2, xs[n]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  Scales scales = load_scales(0);
+  fetch_step(0, 0);
+  fetch_step(1, min(1, steps - 1));
+  put_scales(0, 0, scales);
+  __syncthreads();
+  // Turn `step` asks for step + 2's codes, whose place was read in the turn before, and the first of a pair for the
+  // next pair's scales, which the second puts where the pair before had its own.
+  auto turn = [&](auto number, int step) {
+    constexpr int kTurn = decltype(number)::value, q = kTurn & 1;
+    meet<2 + kXFetches>();   // but for the codes that the last turn asked for
+    if (q == 0) scales = load_scales((step >> 1) + 1);
+    fetch_step((kTurn + 2) % 3, min(step + 2, steps - 1));
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(kTurn % 3, step >> 1 & 1, std::integral_constant<int, q>{});
+    if (q == 1) put_scales(((step >> 1) + 1) & 1, (step >> 1) + 1, scales);
+  };
+  int step = 0;
+  for (;;) {
+    turn(std::integral_constant<int, 0>{}, step);
+    if (++step == steps) break;
+    turn(std::integral_constant<int, 1>{}, step);
+    if (++step == steps) break;
+    turn(std::integral_constant<int, 2>{}, step);
+    if (++step == steps) break;
+    turn(std::integral_constant<int, 3>{}, step);
+    if (++step == steps) break;
+    turn(std::integral_constant<int, 4>{}, step);
+    if (++step == steps) break;
+    turn(std::integral_constant<int, 5>{}, step);
+    if (++step == steps) break;
+  }
+  meet<0>();   // nothing is on its way into LDS any more
+  // to y past LDS, half of the tokens at a time
+  uint16_t *out = reinterpret_cast<uint16_t *>(lds);
+  constexpr int kPitch = kBothRows + 8, kParts = kBothRows / 8, kAtOnce = kThreads / kParts, kHalf = kBothTokens / 2;
+#pragma unroll
+  for (int side = 0; side < 2; side++) {
+    if (token_side / 2 == side) {
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t two[2] = {two_bf16(sum[r][n][4 * i], sum[r][n][4 * i + 1]),
+                                     two_bf16(sum[r][n][4 * i + 2], sum[r][n][4 * i + 3])};
+            __builtin_memcpy(__builtin_assume_aligned(out + ((token_side & 1) * 64 + 32 * n + in_tile) * kPitch + row_side * 128 +
+                                                          32 * r + 8 * i + 4 * half, 8),
+                             two, 8);
+          }
+    }
+    __syncthreads();
+    const int row = tid % kParts * 8, rows_left = p.height - row0 - row, token = tid / kParts;
+    const int tokens_left = p.tokens - token0 - kHalf * side - token;
+    const uint16_t *from = out + token * kPitch + row;
+    uint16_t *to = p.y + static_cast<int64_t>(token0 + kHalf * side + token) * p.ldy + row0 + row;
+    if (rows_left >= 8) {
+#pragma unroll 4
+      for (int i = 0; i < kHalf / kAtOnce; i++) {
+        u32x4 v;
+        __builtin_memcpy(&v, __builtin_assume_aligned(from + i * kAtOnce * kPitch, 16), 16);
+        if (i * kAtOnce < tokens_left) __builtin_memcpy(to + i * kAtOnce * p.ldy, &v, 16);
+      }
+    } else if (rows_left > 0) {
+      for (int i = 0; i * kAtOnce < min(kHalf, tokens_left); i++)
+        for (int k = 0; k < rows_left; k++) to[i * kAtOnce * p.ldy + k] = from[i * kAtOnce * kPitch + k];
+    }
+    __syncthreads();
+  }
+}
+
+// Few tokens of both sides: as mx4_few_kernel, a lane's block of a row and of a token to one instruction
+// (v_mfma_scale_f32_16x16x128_f8f6f4), as they are.
+template <int kRows, int kTokens>
+__global__ __launch_bounds__(64 * kFewWaves) void mx4_both_few_kernel(const QuantizedArgs p) {
+  __shared__ f32x4 lds[kFewLds<kRows, kTokens>];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4;
+  const int row0 = blockIdx.x * 16 * kRows, token0 = blockIdx.y * 16 * kTokens;
+  const int blocks = blocks_of(p.width), steps = (blocks + 3) / 4;
+  int64_t row[kRows], token[kTokens];
+#pragma unroll
+  for (int r = 0; r < kRows; r++) row[r] = static_cast<int64_t>(min(row0 + 16 * r + (lane & 15), p.height - 1)) * blocks;
+#pragma unroll
+  for (int n = 0; n < kTokens; n++) token[n] = static_cast<int64_t>(min(token0 + 16 * n + (lane & 15), p.tokens - 1)) * blocks;
+  FewSums<kRows, kTokens> sums;
+#pragma unroll
+  for (int r = 0; r < kRows; r++)
+#pragma unroll
+    for (int n = 0; n < kTokens; n++) sums.of[r][n] = f32x4{0, 0, 0, 0};
+#pragma unroll 2
+  for (int step = wave; step < steps; step += kFewWaves) {
+    const int block = min(4 * step + group, blocks - 1);
+    const bool there = 4 * step + group < blocks;   // behind the last block: its codes, under scales that make them nothing
+    u32x4 w[kRows], x[kTokens];
+    int ws[kRows], xs[kTokens];
+#pragma unroll
+    for (int r = 0; r < kRows; r++) {
+      w[r] = *reinterpret_cast<const u32x4 *>(p.codes + (row[r] + block) * kBlockBytes);
+      ws[r] = p.scales[row[r] + block];
+    }
+#pragma unroll
+    for (int n = 0; n < kTokens; n++) {
+      x[n] = *reinterpret_cast<const u32x4 *>(p.x_codes + (token[n] + block) * kBlockBytes);
+      xs[n] = p.x_scales[token[n] + block];
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; r++)
+#pragma unroll
+      for (int n = 0; n < kTokens; n++)
+        sums.of[r][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(w[r]), wide(x[n]), sums.of[r][n], 4, 4, 0,
+                                                                         there ? ws[r] : 0, 0, there ? xs[n] : 0);
+  }
+  few_join<kRows, kTokens>(sums, lds, [&](int r, int n, f32x4 sum) {
+    const int t = token0 + 16 * n + (lane & 15);
+    if (t < p.tokens) store_four(p.y + t * p.ldy, row0 + 16 * r + 4 * group, p.height, sum);
+  });
+}
+
+// Which kernel (us, measured as below): to 256 tokens wavefronts that take rows and all their lines, with two tiles each
+// way as soon as that leaves half a workgroup a compute unit (61 tokens through 2080 x 6144: 2 by 2 tiles 12.8, 2
+// by 4 17.9; 130 through 6144 x 2080 9.6 and 9.1, through LDS 13.6); then tiles through LDS, of 128 x 256 (300
+// through 2080 x 6144 29.9, few 34.6), and of 256 x 256 where they are enough (2272 through 6144 x 2080, 216 tiles:
+// 26.3, small ones 32.0; 1136, 120 tiles: 20.7 and 19.6).
+void launch_both(const QuantizedArgs &p, hipStream_t s) {
+  const unsigned rows = (p.height + 15) / 16;
+  const int64_t large_tiles = static_cast<int64_t>((p.height + 255) / 256) * ((p.tokens + 255) / 256);
+  if (p.tokens <= 256 || blocks_of(p.width) < 8) {
+    sub1::note_kernel("mx4_both_few_kernel");
+    const unsigned pairs = (rows + 1) / 2, fours = (p.tokens + 63) / 64;
+    if (p.tokens <= 16)
+      mx4_both_few_kernel<1, 1><<<dim3(rows, 1), 64 * kFewWaves, 0, s>>>(p);
+    else if (p.tokens <= 32 && rows <= 256)
+      mx4_both_few_kernel<1, 2><<<dim3(rows, 1), 64 * kFewWaves, 0, s>>>(p);
+    else if (p.tokens <= 32 || static_cast<int64_t>(pairs) * fours < 128)
+      mx4_both_few_kernel<2, 2><<<dim3(pairs, (p.tokens + 31) / 32), 64 * kFewWaves, 0, s>>>(p);
+    else
+      mx4_both_few_kernel<2, 4><<<dim3(pairs, fours), 64 * kFewWaves, 0, s>>>(p);
+  } else if (large_tiles < 180) {
+    sub1::note_kernel("mx4_both_kernel<1>");
+    mx4_both_kernel<1><<<dim3((p.height + 127) / 128, (p.tokens + 255) / 256), 256, 0, s>>>(p);
+  } else {
+    sub1::note_kernel("mx4_both_kernel<2>");
+    mx4_both_kernel<2><<<dim3((p.height + 255) / 256, (p.tokens + 255) / 256), 512, 0, s>>>(p);
+  }
+}
+
 // Which kernel, by what was measured on matrices of 600 x 2500 to 6144 x 2080 (us, one after the other in a graph):
 // up to 32 tokens, where a wavefront takes rows and all their lines (24 tokens through 4096 x 1024 4.3, shared
 // activations 5.1), two row tiles a wavefront once one makes more than a workgroup a compute unit (32 through 6144
@@ -618,39 +881,6 @@ void launch_product(const ProductArgs &p, hipStream_t s) {
     else
       launch_direct<2, 2, 1, 2>(p, s);
   }
-}
-
-struct QuantizedArgs {
-  const uint8_t *codes, *scales, *x_codes, *x_scales;
-  uint16_t *y;
-  int64_t ldy;
-  int height, width, tokens;
-};
-
-// Both sides in the format: a wavefront takes 16 rows and 16 tokens, 128 values of each a step, which the
-// matrix core multiplies from the codes as they are, each lane's block under its own scale.
-__global__ __launch_bounds__(256) void mx4_quantized_kernel(const QuantizedArgs p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4;
-  const int row0 = blockIdx.x * 16, token0 = blockIdx.y * 64 + 16 * wave;
-  if (token0 >= p.tokens) return;
-  const int blocks = blocks_of(p.width);
-  const int64_t row = min(row0 + (lane & 15), p.height - 1), token = min(token0 + (lane & 15), p.tokens - 1);
-  f32x4 sum = {0, 0, 0, 0};
-  for (int block = group; block < (blocks + 3) / 4 * 4; block += 4) {
-    i32x8 a = {0, 0, 0, 0, 0, 0, 0, 0}, b = {0, 0, 0, 0, 0, 0, 0, 0};
-    int sa = 0, sb = 0;
-    if (block < blocks) {
-      const u32x4 va = *reinterpret_cast<const u32x4 *>(p.codes + (row * blocks + block) * kBlockBytes);
-      const u32x4 vb = *reinterpret_cast<const u32x4 *>(p.x_codes + (token * blocks + block) * kBlockBytes);
-#pragma unroll
-      for (int i = 0; i < 4; i++) a[i] = va[i], b[i] = vb[i];
-      sa = p.scales[row * blocks + block];
-      sb = p.x_scales[token * blocks + block];
-    }
-    sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, sum, 4, 4, 0, sa, 0, sb);
-  }
-  const int t = token0 + (lane & 15);
-  if (t < p.tokens) store_four(p.y + t * p.ldy, row0 + 4 * group, p.height, sum);
 }
 
 // ------------------------------------------------------------------- launching ---
@@ -759,8 +989,7 @@ extern "C" int sub1_mx4_product_quantized(const uint8_t *codes, const uint8_t *s
   if (misaligned(x_codes, 16)) return fail(SUB1_ERR_ALIGN, "sub1_mx4_product_quantized: misaligned pointer");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const QuantizedArgs p{codes, scales, x_codes, x_scales, static_cast<uint16_t *>(y), ldy, height, width, tokens};
-  sub1::note_kernel("mx4_quantized_kernel");
-  mx4_quantized_kernel<<<dim3((height + 15) / 16, (tokens + 63) / 64), 256, 0, s>>>(p);
+  launch_both(p, s);
   HIP_TRY(hipGetLastError());
   return SUB1_OK;
 }

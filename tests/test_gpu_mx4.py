@@ -145,7 +145,8 @@ def test_product(height, width, tokens, strided):
     within(mx4.product(x, codes, scales), *mo.product_bound(host(x), w))
 
 
-@pytest.mark.parametrize('height,width,tokens', SHAPES)
+@pytest.mark.parametrize('height,width,tokens', SHAPES + [(300, 225, 257), (130, 224, 300), (1300, 1000, 1030), (3500, 2080, 3600),
+                                                          (2048, 4096, 20)])
 def test_product_of_two_in_the_format(height, width, tokens):
     codes, scales, w = matrix(height, width, height + width, spread=3)
     x_codes, x_scales, x = matrix(tokens, width, tokens + width, spread=2)
@@ -208,6 +209,14 @@ def test_the_forms_of_the_product():
         y = mx4.product(x, codes, scales)
         assert lib.sub1_last_kernel() == name
         within(y, *mo.product_bound(host(x), w))
+    for tokens, height, width, name in (
+            (256, 300, 256, b'mx4_both_few_kernel'), (257, 300, 256, b'mx4_both_kernel<1>'), (257, 300, 224, b'mx4_both_few_kernel'),
+            (2817, 3841, 256, b'mx4_both_kernel<2>')):
+        codes, scales, w = matrix(height, width, tokens)
+        x_codes, x_scales, x = matrix(tokens, width, tokens + 1)
+        y = mx4.product_quantized(x_codes, x_scales, codes, scales, width)
+        assert lib.sub1_last_kernel() == name
+        within(y, *mo.product_bound(x, w))
 
 
 def test_a_few_tokens_get_the_same_bits_whatever_tokens_they_come_with():
