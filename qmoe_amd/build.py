@@ -59,7 +59,7 @@ def build_tensor_args():
     cmd = [os.environ.get('CXX', 'g++'), '-O2', '-fPIC', '-shared', '-std=c++17', '-fvisibility=hidden',
            '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch._C._GLIBCXX_USE_CXX11_ABI,
            '-DSUB1_TORCH_VERSION="%s"' % torch.__version__,
-           os.path.join(HERE, 'csrc', 'tensor_args.cpp')]
+           '-I' + os.path.join(ROOT, 'include'), os.path.join(HERE, 'csrc', 'tensor_args.cpp')]
     cmd += ['-isystem' + path for path in cpp_extension.include_paths() + [sysconfig.get_paths()['include']]]
     cmd += ['-L' + path for path in cpp_extension.library_paths()]
     cmd += ['-ltorch_python', '-ltorch_cpu', '-lc10', '-o', TENSOR_ARGS_PATH]

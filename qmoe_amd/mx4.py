@@ -23,6 +23,34 @@ BLOCK = 32
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}      # SUB1_MX4_BF16 ..
 
 
+_entries = {}
+
+
+def _entry(name):
+    """The address of a library's function, for the calls that go all the way in C++."""
+    at = _entries.get(name)
+    if at is None:
+        at = _entries[name] = ctypes.cast(getattr(_lib.load(), name), ctypes.c_void_p).value
+    return at
+
+
+def _there():
+    """(the current device, torch's current stream on it)"""
+    device = torch._C._cuda_getDevice()
+    return device, torch._C._cuda_getCurrentRawStream(device)
+
+
+def _quick(name, *args):
+    """The result of a call whose tensors are plainly in order and on the current device, made in C++;
+    None for any other, which the caller then looks at itself, for its copies or its error."""
+    if not torch.cuda.is_initialized():      # (nothing is on a GPU yet)
+        return None
+    got = getattr(_lib.tensor_args(), name)(*args, *_there())
+    if type(got) is int:
+        _lib.check(got)
+    return got
+
+
 def _blocks(width):
     return (width + BLOCK - 1) // BLOCK
 
@@ -51,6 +79,9 @@ def quantize(x):
     fp32.  Per block of 32: the scale is 2^e, e = floor(log2 of the largest magnitude) - 2 and not
     below -127; a value becomes the nearest of the magnitudes times 2^e (of two the one with an even
     code; at most 6 * 2^e).  A block with an infinity or a NaN is NaN.  Rows may be strided."""
+    got = _quick('mx4_quantize', _entry('sub1_mx4_quantize'), x)
+    if got is not None:
+        return got
     rows, ld = _rows(x, 'x')
     kind = _TYPES.get(x.dtype)
     if kind is None:
@@ -82,6 +113,9 @@ def _matrix(codes, scales, width, name, device=None):
 
 def dequantize(codes, scales, width, dtype=torch.bfloat16):
     """[.., width]: what codes and scales stand for, rounded to dtype (exact in bf16 and fp32)."""
+    got = _quick('mx4_dequantize', _entry('sub1_mx4_dequantize'), codes, scales, width, dtype)
+    if got is not None:
+        return got
     kind = _TYPES.get(dtype)
     if kind is None:
         raise TypeError('dtype must be bf16, fp16 or fp32, got %s' % dtype)
@@ -100,6 +134,9 @@ def _fewer_tokens(x, what):
 
 def product(x, codes, scales):
     """bf16 [.., H] = x W^T for x bf16 [.., W] and W [H, W] in the format; fp32 sums."""
+    got = _quick('mx4_product', _entry('sub1_mx4_product'), None, x, codes, scales)
+    if got is not None:
+        return got
     rows, ld = _rows(x, 'x')
     if x.dtype != torch.bfloat16:
         raise TypeError('x must be torch.bfloat16, got %s' % x.dtype)
@@ -163,14 +200,22 @@ class Mx4Linear(nn.Module):
 
     def forward(self, x):
         """x bf16 [.., width] -> bf16 [.., height]"""
+        buffers = self._buffers
+        codes, scales = buffers['codes'], buffers['scales']
+        if self.quantize_activations:
+            got = _quick('mx4_product', _entry('sub1_mx4_product_quantized'), _entry('sub1_mx4_quantize'), x, codes, scales)
+        else:
+            got = _quick('mx4_product', _entry('sub1_mx4_product'), None, x, codes, scales)
+        if got is not None and x.shape[-1] == self.width:
+            return got
         if x.shape[-1:] != (self.width,):
             raise ValueError('x must be [.., %d], got %s' % (self.width, tuple(x.shape)))
         if not self.quantize_activations:
-            return product(x, self.codes, self.scales)
+            return product(x, codes, scales)
         if x.dtype != torch.bfloat16:
             raise TypeError('x must be torch.bfloat16, got %s' % x.dtype)
         x_codes, x_scales = quantize(x)
-        return product_quantized(x_codes, x_scales, self.codes, self.scales, self.width)
+        return product_quantized(x_codes, x_scales, codes, scales, self.width)
 
 
 class Mx4SparseMLP(nn.Module):
@@ -250,6 +295,12 @@ class Mx4SparseMLP(nn.Module):
     def forward(self, hidden):
         """hidden bf16 [.., S, d_model] -> hidden bf16 like it, with `router_outputs` also (logits
         fp32 [.., S, E], index int64 [.., S, top_k])."""
+        b = self._buffers
+        got = _quick('mx4_layer', _entry('sub1_mx4_layer_forward'), _entry('sub1_mx4_layer_scratch_bytes'), hidden, b['router'],
+                     b['wi_codes'], b['wi_scales'], b['wo_codes'], b['wo_scales'], self.top_k, int(self.normalize),
+                     self.capacity or 0)
+        if got is not None:
+            return (got[0], got[1:]) if self.router_outputs else got[0]
         if not isinstance(hidden, torch.Tensor):
             raise TypeError('hidden must be a torch.Tensor')
         if hidden.dim() < 2 or hidden.shape[-1] != self.d_model:
