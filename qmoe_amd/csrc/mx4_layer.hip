@@ -22,7 +22,8 @@ struct LayerArgs {
   // the scratch memory's parts
   int32_t *tiles;      // [0]: how many; from 4 on (expert, first pair, pairs, 0) of each
   int32_t *pairs;      // token * top_k + place, in the order of their experts, those that no expert takes left out
-  float *p;            // [tokens * top_k], negative where the token keeps its input
+  int32_t *chosen;     // the experts of the tokens' places
+  float *p;            // [tokens * top_k], their shares, negative where the token keeps its input
   uint16_t *h;         // bf16 [tokens * top_k, d_ff up to a whole block]
   float *out;          // [tokens * top_k, d_model]
 };
@@ -49,52 +50,144 @@ __device__ __forceinline__ void load4(const uint16_t *row, int first, int width,
   }
 }
 
-// A wavefront an expert, kTokens tokens at once.  Sums in 64 bits, in which the products are exact: which of
-// two close logits is the larger then follows from the values, not from the order of the sum.
-template <class R, int kTokens>
+__device__ __forceinline__ double wave_sum(double v) {   // in lane 63
+  auto add = [&](auto control, auto rows) {
+    constexpr int kControl = decltype(control)::value, kMask = decltype(rows)::value;
+    const unsigned long long u = __double_as_longlong(v);
+    const uint32_t low = sub1::dpp_or_zero<kControl, kMask>(static_cast<int>(u));
+    const uint32_t high = sub1::dpp_or_zero<kControl, kMask>(static_cast<int>(u >> 32));
+    v += __longlong_as_double(static_cast<unsigned long long>(high) << 32 | low);
+  };
+  add(std::integral_constant<int, sub1::kDppRowShr1>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, sub1::kDppRowShr2>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, sub1::kDppRowShr4>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, sub1::kDppRowShr8>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, sub1::kDppBcast15>{}, std::integral_constant<int, 0xa>{});
+  add(std::integral_constant<int, sub1::kDppBcast31>{}, std::integral_constant<int, 0xc>{});
+  return v;
+}
+
+// kExperts by kTokens a workgroup, whose four wavefronts share a row's length, 256 values at a time.  Sums in 64 bits,
+// in which the products are exact: which of two close logits is the larger then follows from the values,
+// not from the order of the sum.
+template <class R, int kExperts, int kTokens>
 __global__ __launch_bounds__(256) void mx4_logits_kernel(const LayerArgs a) {
-  const int lane = threadIdx.x & 63, expert = blockIdx.x * 4 + (threadIdx.x >> 6), token0 = blockIdx.y * kTokens;
-  if (expert >= a.experts) return;
-  const R *row = static_cast<const R *>(a.router) + static_cast<int64_t>(expert) * a.d_model;
-  double sum[kTokens];
+  __shared__ double parts[4][kExperts * kTokens];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int expert0 = blockIdx.x * kExperts, token0 = blockIdx.y * kTokens;
+  const R *row[kExperts];
+  const uint16_t *x[kTokens];
 #pragma unroll
-  for (int n = 0; n < kTokens; n++) sum[n] = 0;
-  for (int k = 4 * lane; k < a.d_model; k += 256) {
-    float r[4], v[4];
-    load4(row, k, a.d_model, r);
+  for (int e = 0; e < kExperts; e++)
+    row[e] = static_cast<const R *>(a.router) + static_cast<int64_t>(min(expert0 + e, a.experts - 1)) * a.d_model;
+#pragma unroll
+  for (int n = 0; n < kTokens; n++) x[n] = a.x + static_cast<int64_t>(min(token0 + n, a.tokens - 1)) * a.d_model;
+  double sum[kExperts][kTokens];
+#pragma unroll
+  for (int e = 0; e < kExperts; e++)
+#pragma unroll
+    for (int n = 0; n < kTokens; n++) sum[e][n] = 0;
+  auto add = [&](int first) {
+    float r[kExperts][4], v[kTokens][4];
+#pragma unroll
+    for (int e = 0; e < kExperts; e++) load4(row[e], first, a.d_model, r[e]);
+#pragma unroll
+    for (int n = 0; n < kTokens; n++) load4(x[n], first, a.d_model, v[n]);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int e = 0; e < kExperts; e++)
+#pragma unroll
+        for (int n = 0; n < kTokens; n++)
+          sum[e][n] = fma(static_cast<double>(r[e][i]), static_cast<double>(v[n][i]), sum[e][n]);
+  };
+  int k = wave * 256;
+#pragma unroll 2
+  for (; k + 256 <= a.d_model; k += 1024) {
+    __builtin_assume(k + 4 * lane + 4 <= a.d_model);
+    add(k + 4 * lane);
+  }
+  if (k < a.d_model) add(k + 4 * lane);
+#pragma unroll
+  for (int e = 0; e < kExperts; e++)
 #pragma unroll
     for (int n = 0; n < kTokens; n++) {
-      if (token0 + n >= a.tokens) break;
-      load4(a.x + static_cast<int64_t>(token0 + n) * a.d_model, k, a.d_model, v);
-#pragma unroll
-      for (int i = 0; i < 4; i++) sum[n] = fma(static_cast<double>(r[i]), static_cast<double>(v[i]), sum[n]);
+      const double all = wave_sum(sum[e][n]);
+      if (lane == 63) parts[wave][e * kTokens + n] = all;
     }
-  }
-#pragma unroll
-  for (int n = 0; n < kTokens; n++) {
-    for (int d = 32; d; d >>= 1) sum[n] += __shfl_xor(sum[n], d);
-    if (lane == 0 && token0 + n < a.tokens)
-      a.logits[static_cast<int64_t>(token0 + n) * a.experts + expert] = static_cast<float>(sum[n]);
+  __syncthreads();
+  if (threadIdx.x < kExperts * kTokens) {
+    const int i = threadIdx.x, expert = expert0 + i / kTokens, token = token0 + i % kTokens;
+    if (expert < a.experts && token < a.tokens)
+      a.logits[static_cast<int64_t>(token) * a.experts + expert] =
+          static_cast<float>(((parts[0][i] + parts[1][i]) + parts[2][i]) + parts[3][i]);
   }
 }
 
 // ------------------------------------------------------------ which experts ---
 
-// Logits in the order in which experts are taken: larger first, of equals the one of the lower index, those
-// that are no numbers last.
-__device__ __forceinline__ unsigned long long rank_of(float logit, int expert) {
-  uint32_t bits = __float_as_uint(logit + 0.0f);   // -0 is 0
-  bits = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
-  if (logit != logit) bits = 0;
-  return static_cast<unsigned long long>(bits) << 32 | (0xffffffffu - static_cast<uint32_t>(expert));
+// Logits in the order in which experts are taken, as whole numbers: larger first, those that are no numbers
+// last (0); of equal ones the expert of the lower index comes first.
+__device__ __forceinline__ uint32_t rank_of(float logit) {
+  const uint32_t bits = __float_as_uint(logit + 0.0f);   // -0 is 0
+  return logit != logit ? 0u : bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-__device__ __forceinline__ unsigned long long wave_max(unsigned long long v) {
-  for (int d = 32; d; d >>= 1) {
-    const unsigned long long u = __shfl_xor(v, d);
-    v = u > v ? u : v;
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {   // in all lanes
+  auto most = [&](auto control, auto rows) {
+    v = max(v, static_cast<uint32_t>(sub1::dpp_or_zero<decltype(control)::value, decltype(rows)::value>(static_cast<int>(v))));
+  };
+  most(std::integral_constant<int, sub1::kDppRowShr1>{}, std::integral_constant<int, 0xf>{});
+  most(std::integral_constant<int, sub1::kDppRowShr2>{}, std::integral_constant<int, 0xf>{});
+  most(std::integral_constant<int, sub1::kDppRowShr4>{}, std::integral_constant<int, 0xf>{});
+  most(std::integral_constant<int, sub1::kDppRowShr8>{}, std::integral_constant<int, 0xf>{});
+  most(std::integral_constant<int, sub1::kDppBcast15>{}, std::integral_constant<int, 0xa>{});
+  most(std::integral_constant<int, sub1::kDppBcast31>{}, std::integral_constant<int, 0xc>{});
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
+struct Choice {
+  uint32_t rank;
+  int expert;
+};
+constexpr Choice kNone = {0xffffffffu, -1};   // before the first (no logit has this rank)
+
+// A wavefront's token's next expert behind `last`.
+__device__ __forceinline__ Choice next_choice(const float *logits, int experts, Choice last) {
+  const int lane = threadIdx.x & 63;
+  Choice best = {0, -1};
+  for (int e = lane; e < experts; e += 64) {
+    const uint32_t rank = rank_of(logits[e]);
+    const bool left = rank < last.rank || (rank == last.rank && e > last.expert);
+    if (left && (best.expert < 0 || rank > best.rank)) best = {rank, e};
   }
-  return v;
+  const uint32_t rank = wave_max(best.expert < 0 ? 0 : best.rank);
+  return {rank, static_cast<int>(~wave_max(best.expert < 0 || best.rank != rank ? 0 : ~static_cast<uint32_t>(best.expert)))};
+}
+
+// A wavefront's token's experts and their shares: to index, and (expert, share) of place j to put(j, ..).
+template <class Put>
+__device__ __forceinline__ void choose(const LayerArgs &a, int token, Put put) {
+  const int lane = threadIdx.x & 63;
+  const float *logits = a.logits + static_cast<int64_t>(token) * a.experts;
+  Choice c = kNone;
+  float most = 0, sum = 0, taken = 0, mine = 0;
+  int expert = 0;
+  for (int j = 0; j < a.top_k; j++) {
+    c = next_choice(logits, a.experts, c);
+    if (j == 0) {
+      most = logits[c.expert];
+      for (int e = lane; e < a.experts; e += 64) sum += expf(logits[e] - most);
+      sum = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mx4::wave_sum(sum)), 63));
+    }
+    const float p = expf(logits[c.expert] - most) / sum;
+    taken += p;
+    if (lane == j) mine = p, expert = c.expert;
+  }
+  if (lane < a.top_k) {
+    a.index[static_cast<int64_t>(token) * a.top_k + lane] = expert;
+    put(lane, expert, a.normalize ? mine / taken : mine);
+  }
 }
 
 constexpr int kPlanThreads = 1024;
@@ -108,34 +201,11 @@ __global__ __launch_bounds__(kPlanThreads) void mx4_plan_kernel(const LayerArgs 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int pairs = a.tokens * a.top_k;
   for (int e = tid; e < a.experts; e += kPlanThreads) count[e] = 0;
-
-  for (int t = wave; t < a.tokens; t += kPlanThreads / 64) {
-    const float *logits = a.logits + static_cast<int64_t>(t) * a.experts;
-    float most = -__builtin_inff(), sum = 0;
-    for (int e = lane; e < a.experts; e += 64) most = fmaxf(most, logits[e]);
-    for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-    for (int e = lane; e < a.experts; e += 64) sum += expf(logits[e] - most);
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    unsigned long long last = ~0ull;
-    float taken = 0, mine = 0;
-    for (int j = 0; j < a.top_k; j++) {
-      unsigned long long best = 0;
-      for (int e = lane; e < a.experts; e += 64) {
-        const unsigned long long r = rank_of(logits[e], e);
-        if (r < last && r > best) best = r;
-      }
-      last = wave_max(best);
-      const int e = static_cast<int>(0xffffffffu - static_cast<uint32_t>(last));
-      const float p = expf(logits[e] - most) / sum;
-      taken += p;
-      if (lane == j) mine = p;
-      if (lane == 0) {
-        expert_of[t * a.top_k + j] = e;
-        a.index[t * a.top_k + j] = e;
-      }
-    }
-    if (lane < a.top_k) a.p[t * a.top_k + lane] = a.normalize ? mine / taken : mine;
-  }
+  for (int t = wave; t < a.tokens; t += kPlanThreads / 64)
+    choose(a, t, [&](int j, int expert, float p) {
+      expert_of[t * a.top_k + j] = expert;
+      a.p[t * a.top_k + j] = p;
+    });
   __syncthreads();
 
   // a token beyond its expert's capacity in its sequence (with one expert a token)
@@ -207,8 +277,24 @@ __device__ __forceinline__ bool tile_of(const LayerArgs &a, int i, Tile &t) {
 
 __device__ __forceinline__ int h_width(const LayerArgs &a) { return blocks_of(a.d_ff) * kBlock; }
 
+// The last row of workgroups, where a capacity may leave tokens with their input, writes those tokens' y.
+__device__ __forceinline__ void keep_inputs(const LayerArgs &a) {
+  for (int t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    const float p = a.p[t];
+    if (!(__float_as_uint(p) >> 31)) continue;
+    for (int d = threadIdx.x; d < a.d_model; d += 64 * kFewWaves) {
+      const int64_t at = static_cast<int64_t>(t) * a.d_model + d;
+      a.y[at] = static_cast<uint16_t>(two_bf16(-p * sub1::bf16_to_f32(a.x[at]), 0));
+    }
+  }
+}
+
 __global__ __launch_bounds__(64 * kFewWaves) void mx4_wi_kernel(const LayerArgs a) {
   __shared__ f32x4 lds[kFewLds<1, 1>];
+  if (a.capacity && blockIdx.y == gridDim.y - 1) {
+    keep_inputs(a);
+    return;
+  }
   Tile t;
   if (!tile_of(a, blockIdx.y, t)) return;
   const int lane = threadIdx.x & 63, row0 = blockIdx.x * 16, width = h_width(a), mine = lane & 15;
@@ -235,6 +321,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_wi_kernel(const LayerArgs 
   }
 }
 
+// With one expert a token the product, times the token's share, is its y; else it waits for the others.
+template <bool kOnly>
 __global__ __launch_bounds__(64 * kFewWaves) void mx4_wo_kernel(const LayerArgs a) {
   __shared__ f32x4 lds[kFewLds<1, 1>];
   Tile t;
@@ -249,9 +337,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_wo_kernel(const LayerArgs 
   few_join<1, 1>(sums, lds, [&](int, int, f32x4 sum) {
     if (pair < 0) return;
     const int row = row0 + 4 * (lane >> 4);
+    const float p = kOnly ? a.p[pair] : 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (row + i < a.d_model) a.out[pair * a.d_model + row + i] = sum[i];
+    for (int i = 0; i < 4; i++) {
+      if (row + i >= a.d_model) break;
+      if (kOnly)
+        a.y[pair * a.d_model + row + i] = static_cast<uint16_t>(two_bf16(p * sum[i], 0));
+      else
+        a.out[pair * a.d_model + row + i] = sum[i];
+    }
   });
 }
 
@@ -260,15 +354,103 @@ __global__ __launch_bounds__(256) void mx4_combine_kernel(const LayerArgs a) {
   const int64_t t = blockIdx.y;
   if (d >= a.d_model) return;
   float sum = 0;
-  for (int j = 0; j < a.top_k; j++) {
-    const int64_t pair = t * a.top_k + j;
-    const float p = a.p[pair];
-    sum += __float_as_uint(p) >> 31 ? -p * sub1::bf16_to_f32(a.x[t * a.d_model + d]) : p * a.out[pair * a.d_model + d];
+  for (int j = 0; j < a.top_k; j++) sum += a.p[t * a.top_k + j] * a.out[(t * a.top_k + j) * a.d_model + d];
+  a.y[t * a.d_model + d] = static_cast<uint16_t>(two_bf16(sum, 0));
+}
+
+// ---- a token at a time, each with its own experts' rows ----
+//
+// Where few tokens share an expert, grouping them costs more than it saves: a workgroup finds its token's expert by
+// itself and takes the token through kRows rows a wavefront, and the workgroups of wo add the token's experts up.
+// Three launches, with nothing between workgroups of one.
+
+template <int kRows>
+__global__ __launch_bounds__(64 * kOneWaves) void mx4_one_wi_kernel(const LayerArgs a) {
+  extern __shared__ u32x4 one_lds[];
+  const int pair = blockIdx.y, token = pair / a.top_k, place = pair - token * a.top_k, width = h_width(a);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  stage_one(one_lds, a.x + static_cast<int64_t>(token) * a.d_model, a.d_model);
+  const float *logits = a.logits + static_cast<int64_t>(token) * a.experts;
+  Choice c = kNone;
+  for (int j = 0; j <= place; j++) c = next_choice(logits, a.experts, c);
+  if (blockIdx.x == 0 && place == 0 && wave == 0)   // for wo, and for the caller
+    choose(a, token, [&](int j, int expert, float p) {
+      a.chosen[pair + j] = expert;
+      a.p[pair + j] = p;
+    });
+  __syncthreads();
+  const int blocks = blocks_of(a.d_model);
+#pragma unroll
+  for (int r = 0; r < kRows; r++) {
+    const int row = (blockIdx.x * kRows + r) * kOneWaves + wave;
+    if (row >= width) return;
+    float sum = 0;
+    if (row < a.d_ff) {
+      const int64_t first = (static_cast<int64_t>(c.expert) * a.d_ff + row) * blocks;
+      sum = one_product(a.wi_codes + first * kBlockBytes, a.wi_scales + first, blocks, one_lds, [] {});
+    }
+    // (bf16 between the layers, and zeros behind the last row, as above)
+    if ((threadIdx.x & 63) == 63)
+      a.h[static_cast<int64_t>(pair) * width + row] = static_cast<uint16_t>(two_bf16(sum < 0 ? 0.0f : sum, 0));
   }
-  a.y[t * a.d_model + d] = sub1::f32_to_bf16(sum);
+}
+
+template <int kRows>
+__global__ __launch_bounds__(64 * kOneWaves) void mx4_one_wo_kernel(const LayerArgs a) {
+  extern __shared__ u32x4 one_lds[];
+  const int token = blockIdx.y, width = h_width(a), blocks = blocks_of(a.d_ff);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  float all[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; r++) all[r] = 0;
+  for (int j = 0; j < a.top_k; j++) {
+    const int pair = token * a.top_k + j;
+    if (j) __syncthreads();
+    stage_one(one_lds, a.h + static_cast<int64_t>(pair) * width, width);
+    const int expert = a.chosen[pair];
+    const float p = a.p[pair];
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRows; r++) {
+      const int row = (blockIdx.x * kRows + r) * kOneWaves + wave;
+      const int64_t first = (static_cast<int64_t>(expert) * a.d_model + min(row, a.d_model - 1)) * blocks;
+      all[r] += p * one_product(a.wo_codes + first * kBlockBytes, a.wo_scales + first, blocks, one_lds, [] {});
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; r++) {
+    const int row = (blockIdx.x * kRows + r) * kOneWaves + wave;
+    if ((threadIdx.x & 63) == 63 && row < a.d_model)
+      a.y[static_cast<int64_t>(token) * a.d_model + row] = static_cast<uint16_t>(two_bf16(all[r], 0));
+  }
 }
 
 // ------------------------------------------------------------------- launching ---
+
+template <class R>
+int launch_logits(const LayerArgs &a, hipStream_t s) {
+  if (a.tokens == 1)
+    mx4_logits_kernel<R, 1, 1><<<dim3(a.experts, 1), 256, 0, s>>>(a);
+  else if (static_cast<int64_t>(a.experts) * a.tokens <= 8192)
+    mx4_logits_kernel<R, 1, 4><<<dim3(a.experts, (a.tokens + 3) / 4), 256, 0, s>>>(a);
+  else
+    mx4_logits_kernel<R, 4, 4><<<dim3((a.experts + 3) / 4, (a.tokens + 3) / 4), 256, 0, s>>>(a);
+  HIP_TRY(hipGetLastError());
+  return SUB1_OK;
+}
+
+template <int kRows>
+int launch_ones(const LayerArgs &a, hipStream_t s) {
+  constexpr int kAll = kRows * kOneWaves;
+  HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_wi_kernel<kRows>));
+  HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_wo_kernel<kRows>));
+  mx4_one_wi_kernel<kRows><<<dim3((blocks_of(a.d_ff) * kBlock + kAll - 1) / kAll, a.tokens * a.top_k), 64 * kOneWaves,
+                             one_lds_bytes(a.d_model), s>>>(a);
+  HIP_TRY(hipGetLastError());
+  mx4_one_wo_kernel<kRows><<<dim3((a.d_model + kAll - 1) / kAll, a.tokens), 64 * kOneWaves, one_lds_bytes(a.d_ff), s>>>(a);
+  HIP_TRY(hipGetLastError());
+  return SUB1_OK;
+}
 
 int most_tiles(const sub1_mx4_layer *l, int tokens) {
   const int pairs = tokens * l->top_k, taking = pairs < l->experts ? pairs : l->experts;
@@ -278,14 +460,15 @@ int most_tiles(const sub1_mx4_layer *l, int tokens) {
 int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 struct Parts {
-  int64_t tiles, pairs, p, h, out, bytes;
+  int64_t tiles, pairs, chosen, p, h, out, bytes;
 };
 Parts parts_of(const sub1_mx4_layer *l, int tokens) {
   const int64_t pairs = static_cast<int64_t>(tokens) * l->top_k;
   Parts at;
   at.tiles = 0;
   at.pairs = at.tiles + up(16 + 16 * static_cast<int64_t>(most_tiles(l, tokens)));
-  at.p = at.pairs + up(4 * pairs);
+  at.chosen = at.pairs + up(4 * pairs);
+  at.p = at.chosen + up(4 * pairs);
   at.h = at.p + up(4 * pairs);
   at.out = at.h + up(pairs * blocks_of(l->d_ff) * kBlock * 2);
   at.bytes = at.out + up(pairs * l->d_model * 4);
@@ -344,23 +527,33 @@ extern "C" int sub1_mx4_layer_forward(const sub1_mx4_layer *layer, const void *x
               static_cast<const uint16_t *>(x), static_cast<uint16_t *>(y), logits, index, tokens, length,
               layer->experts, layer->d_model, layer->d_ff, layer->top_k, layer->normalize, layer->capacity,
               reinterpret_cast<int32_t *>(base + at.tiles), reinterpret_cast<int32_t *>(base + at.pairs),
-              reinterpret_cast<float *>(base + at.p), reinterpret_cast<uint16_t *>(base + at.h),
+              reinterpret_cast<int32_t *>(base + at.chosen), reinterpret_cast<float *>(base + at.p), reinterpret_cast<uint16_t *>(base + at.h),
               reinterpret_cast<float *>(base + at.out)};
-  constexpr int kTokens = 4;
-  const dim3 routers((a.experts + 3) / 4, (tokens + kTokens - 1) / kTokens);
-  if (layer->router_type == SUB1_MX4_FP32)
-    mx4_logits_kernel<float, kTokens><<<routers, 256, 0, s>>>(a);
-  else
-    mx4_logits_kernel<uint16_t, kTokens><<<routers, 256, 0, s>>>(a);
-  HIP_TRY(hipGetLastError());
+  int rc2 = layer->router_type == SUB1_MX4_FP32 ? launch_logits<float>(a, s) : launch_logits<uint16_t>(a, s);
+  if (rc2) return rc2;
+  const char *f = getenv("MX4_FORM");
+  const int pairs = tokens * a.top_k;
+  if (!a.capacity && (f ? atoi(f) : 1)) {
+    const int form = f ? atoi(f) : 1;
+    sub1::note_kernel("mx4_one_wo_kernel");
+    if (form == 1) return launch_ones<1>(a, s);
+    if (form == 2) return launch_ones<2>(a, s);
+    return launch_ones<4>(a, s);
+  }
   mx4_plan_kernel<<<1, kPlanThreads, 0, s>>>(a);
   HIP_TRY(hipGetLastError());
   const unsigned tiles = static_cast<unsigned>(most_tiles(layer, tokens));
-  mx4_wi_kernel<<<dim3(blocks_of(a.d_ff) * 2, tiles), 64 * kFewWaves, 0, s>>>(a);
+  mx4_wi_kernel<<<dim3(blocks_of(a.d_ff) * 2, tiles + (a.capacity ? 1 : 0)), 64 * kFewWaves, 0, s>>>(a);
   HIP_TRY(hipGetLastError());
-  mx4_wo_kernel<<<dim3((a.d_model + 15) / 16, tiles), 64 * kFewWaves, 0, s>>>(a);
+  sub1::note_kernel("mx4_wo_kernel");
+  const dim3 wo((a.d_model + 15) / 16, tiles);
+  if (a.top_k == 1) {
+    mx4_wo_kernel<true><<<wo, 64 * kFewWaves, 0, s>>>(a);
+    HIP_TRY(hipGetLastError());
+    return SUB1_OK;
+  }
+  mx4_wo_kernel<false><<<wo, 64 * kFewWaves, 0, s>>>(a);
   HIP_TRY(hipGetLastError());
-  sub1::note_kernel("mx4_combine_kernel");
   mx4_combine_kernel<<<dim3((a.d_model + 255) / 256, tokens), 256, 0, s>>>(a);
   HIP_TRY(hipGetLastError());
   return SUB1_OK;

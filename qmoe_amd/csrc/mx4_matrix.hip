@@ -1,8 +1,6 @@
 // Microscaled 4-bit matrices: values to the format and back, and products with them.
 #include "mx4.h"
 
-#include <type_traits>
-
 using namespace mx4;
 using sub1::fail;
 using sub1::misaligned;
@@ -178,6 +176,17 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(const ProductAr
     const int token = token0 + 16 * n + (lane & 15);
     if (token < p.tokens) store_four(p.y + token * p.ldy, row0 + 16 * r + 4 * (lane >> 4), p.height, sum);
   });
+}
+
+__global__ __launch_bounds__(64 * kOneWaves) void mx4_one_kernel(const ProductArgs p) {
+  extern __shared__ u32x4 one_lds[];
+  const int row = blockIdx.x * kOneWaves + (threadIdx.x >> 6), blocks = blocks_of(p.width);
+  const int64_t first = static_cast<int64_t>(min(row, p.height - 1)) * blocks;   // (all wavefronts fill LDS)
+  const float sum = one_product(p.codes + first * kBlockBytes, p.scales + first, blocks, one_lds, [&] {
+    stage_one(one_lds, p.x, p.width);
+    __syncthreads();
+  });
+  if ((threadIdx.x & 63) == 63 && row < p.height) p.y[row] = static_cast<uint16_t>(two_bf16(sum, 0));
 }
 
 // Many tokens: four wavefronts, two by two, each with 32 kRows rows of the matrix and 32 kTokens tokens, 64
@@ -845,7 +854,7 @@ void launch_both(const QuantizedArgs &p, hipStream_t s) {
 }
 
 // Which kernel, by what was measured on matrices of 600 x 2500 to 6144 x 2080 (us, one after the other in a graph):
-// up to 32 tokens, where a wavefront takes rows and all their lines (24 tokens through 4096 x 1024 4.3, shared
+// a token alone by whole rows; up to 32 tokens, where a wavefront takes rows and all their lines (24 tokens through 4096 x 1024 4.3, shared
 // activations 5.1), two row tiles a wavefront once one makes more than a workgroup a compute unit (32 through 6144
 // x 2080 6.5, one 8.7; through 2080 x 6144 18.0 and 15.3).  Then tiles of 64 x 64, as there are few of them
 // shared by four, two or one group of four wavefronts (70 through 2080 x 6144, 66 tiles: 13.7, 15.7, 20.5; 200
@@ -853,10 +862,14 @@ void launch_both(const QuantizedArgs &p, hipStream_t s) {
 // of the small ones a compute unit on (2272 through 6144 x 2080, 3456 tiles: 72, small ones 94).
 // Activations whose rows do not lie on 16 bytes cannot be fetched into LDS and go through registers
 // (2272 through 6144 x 2080 86, 568 through 4096 x 1024 13.3).
-void launch_product(const ProductArgs &p, hipStream_t s) {
+int launch_product(const ProductArgs &p, hipStream_t s) {
   const int64_t small_tiles = static_cast<int64_t>((p.height + 63) / 64) * ((p.tokens + 63) / 64);
   const unsigned rows = (p.height + 15) / 16;
-  if (p.tokens <= 32 || p.width < 64) {
+  if (p.tokens == 1) {
+    sub1::note_kernel("mx4_one_kernel");
+    HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_kernel));
+    mx4_one_kernel<<<(p.height + kOneWaves - 1) / kOneWaves, 64 * kOneWaves, one_lds_bytes(p.width), s>>>(p);
+  } else if (p.tokens <= 32 || p.width < 64) {
     sub1::note_kernel("mx4_few_kernel");
     if (p.tokens <= 16)
       mx4_few_kernel<1, 1><<<dim3(rows, 1), 64 * kFewWaves, 0, s>>>(p);
@@ -881,6 +894,8 @@ void launch_product(const ProductArgs &p, hipStream_t s) {
     else
       launch_direct<2, 2, 1, 2>(p, s);
   }
+  HIP_TRY(hipGetLastError());
+  return SUB1_OK;
 }
 
 // ------------------------------------------------------------------- launching ---
@@ -975,9 +990,7 @@ extern "C" int sub1_mx4_product(const uint8_t *codes, const uint8_t *scales, int
   hipStream_t s = static_cast<hipStream_t>(stream);
   const ProductArgs p{codes, scales, static_cast<const uint16_t *>(x), static_cast<uint16_t *>(y), ldx, ldy, height,
                       width, tokens};
-  launch_product(p, s);
-  HIP_TRY(hipGetLastError());
-  return SUB1_OK;
+  return launch_product(p, s);
 }
 
 extern "C" int sub1_mx4_product_quantized(const uint8_t *codes, const uint8_t *scales, int height, int width,

@@ -133,7 +133,7 @@ def test_shapes_and_rows_that_need_a_copy():
 # ------------------------------------------------------------------- products ---
 
 SHAPES = [(1, 1, 1), (16, 32, 1), (17, 33, 2), (3, 127, 16), (48, 129, 17), (100, 1000, 33), (65, 2080, 64), (130, 160, 65),
-          (257, 96, 200), (200, 3001, 13), (300, 515, 300), (40, 64, 70), (40, 63, 70), (4100, 96, 30), (1000, 1056, 700),
+          (257, 96, 200), (200, 3001, 13), (300, 515, 300), (40, 64, 70), (40, 63, 70), (4100, 96, 30), (1000, 1056, 700), (77, 2049, 1), (9, 6144, 1), (2081, 100, 1),
           (3000, 416, 1100), (2050, 2080, 2100)]
 
 
@@ -202,6 +202,7 @@ def test_the_forms_of_the_product():
     """Which kernel a call takes, at the sizes where the choice turns."""
     lib = _lib.load()
     for tokens, height, width, strided, name in (
+            (1, 700, 128, False, b'mx4_one_kernel'), (1, 300, 65536, False, b'mx4_one_kernel'), (2, 700, 128, True, b'mx4_few_kernel'),
             (32, 700, 128, False, b'mx4_few_kernel'), (33, 700, 128, False, b'mx4_many_direct_kernel'),
             (33, 700, 63, False, b'mx4_few_kernel'), (33, 700, 128, True, b'mx4_many_kernel')):
         codes, scales, w = matrix(height, width, tokens)
@@ -223,7 +224,7 @@ def test_a_few_tokens_get_the_same_bits_whatever_tokens_they_come_with():
     codes, scales, _ = matrix(200, 1000, 11)
     x = activations(32, 1000, 12)
     want = mx4.product(x, codes, scales)
-    for some in (slice(0, 1), slice(3, 8), slice(9, 30), slice(31, 32)):
+    for some in (slice(0, 2), slice(3, 8), slice(9, 30), slice(30, 32)):
         assert torch.equal(mx4.product(x[some], codes, scales), want[some])
 
 
@@ -348,7 +349,7 @@ def test_a_token_gets_the_same_bits_in_every_batch():
     layer = mx4.Mx4SparseMLP(router, wi, wo, 2, True, router_outputs=False)
     hidden = activations(256, 200, 52)
     want = layer(hidden)
-    for some in (slice(0, 1), slice(7, 20), slice(100, 228)):
+    for some in (slice(0, 70), slice(7, 120), slice(100, 228)):
         assert torch.equal(layer(hidden[some]), want[some])
 
 
