@@ -176,26 +176,38 @@ __device__ __forceinline__ void few_join(const FewSums<kRows, kTokens> &sums, f3
 template <int kRows, int kTokens>
 constexpr int kFewLds = kRows *kTokens * 64 * kFewWaves;   // f32x4
 
-// One token: a wavefront takes a whole row, 64 blocks of it at a time, a block a lane: a row's codes are read as they
-// lie, 1 KB a load, and so are its scales.  (Few tokens' lanes above read 16 rows' 64 bytes a load, which the L1
-// takes several times as long for, but share them among 16 tokens.)  The token's values wait in LDS, the lanes' blocks
-// in four parts of 16 bytes, each part of 64 lanes back to back; v_dot2_f32_bf16 multiplies two at a time.  One
-// token through 2080 x 6144 3.6 us (by the kernel above 6.1), through 6144 x 2080 3.7 (4.3), of which some 2.3 are a
+// One token: kLanes lanes, a wavefront or half of one, take a whole row, a block a lane at a time: a row's codes are
+// read as they lie, 1 KB a load, and so are its scales.  (Few tokens' lanes above read 16 rows' 64 bytes a load, which
+// the L1 takes several times as long for, but share them among 16 tokens.)  The token's values wait in LDS, kLanes
+// blocks' four parts of 16 bytes each back to back; v_dot2_f32_bf16 multiplies two at a time.  One token
+// through 2080 x 6144 3.6 us (by the kernel above 6.1), through 6144 x 2080 3.5 (4.3), of which some 2.3 are a
 // launch's; two tokens so 4.4 and 4.6 (6.5, 4.4), four 6.3 and 6.5 (7.1, 4.7).
 constexpr int kOneWaves = 8;
 constexpr int kOneMostBytes = 128 * 1024;   // of LDS, for the widest row
 
 __host__ __device__ constexpr int one_lds_bytes(int width) { return (blocks_of(width) + 63) / 64 * 4096; }
-
 static_assert(one_lds_bytes(SUB1_MX4_MAX_WIDTH) <= kOneMostBytes, "every width has room");
+template <int kLanes>
+constexpr int kOneRows = kOneWaves * 64 / kLanes;   // of a workgroup, at once
 
-__device__ __forceinline__ void stage_one(u32x4 *lds, const uint16_t *x, int width) {
-  const int parts = (blocks_of(width) + 63) / 64 * 256;
-  for (int i = threadIdx.x; i < parts; i += 64 * kOneWaves)
-    lds[(i >> 8) * 256 + (i & 3) * 64 + (i >> 2 & 63)] = load8(x, 8 * i, width);
+// Half a wavefront a row where the last turn of a whole one would leave half of it or more idle and rows are many
+// enough for a workgroup every other compute unit (one token through 4096 x 1024 2.4 us, by whole ones 2.7; through
+// 3001 x 1023 2.5 and 2.8; 26 pairs of a sparse MLP of 1024 x 4096 31.7 and 40).
+inline bool halves_pay(int width, int64_t rows) {
+  const int over = blocks_of(width) % 64;
+  return over > 0 && over <= 32 && rows >= 128 * kOneRows<32>;
 }
 
-__device__ __forceinline__ float wave_sum(float v) {   // in lane 63
+template <int kLanes>
+__device__ __forceinline__ void stage_one(u32x4 *lds, const uint16_t *x, int width) {
+  const int parts = (blocks_of(width) + kLanes - 1) / kLanes * kLanes * 4;
+  for (int i = threadIdx.x; i < parts; i += 64 * kOneWaves)
+    lds[i / (4 * kLanes) * (4 * kLanes) + (i & 3) * kLanes + (i >> 2) % kLanes] = load8(x, 8 * i, width);
+}
+
+// Sums over kLanes lanes, in the last of them.
+template <int kLanes>
+__device__ __forceinline__ float lanes_sum(float v) {
   auto add = [&](auto control, auto rows) {
     v += __int_as_float(sub1::dpp_or_zero<decltype(control)::value, decltype(rows)::value>(__float_as_int(v)));
   };
@@ -204,16 +216,16 @@ __device__ __forceinline__ float wave_sum(float v) {   // in lane 63
   add(std::integral_constant<int, sub1::kDppRowShr4>{}, std::integral_constant<int, 0xf>{});
   add(std::integral_constant<int, sub1::kDppRowShr8>{}, std::integral_constant<int, 0xf>{});
   add(std::integral_constant<int, sub1::kDppBcast15>{}, std::integral_constant<int, 0xa>{});
-  add(std::integral_constant<int, sub1::kDppBcast31>{}, std::integral_constant<int, 0xc>{});
+  if (kLanes == 64) add(std::integral_constant<int, sub1::kDppBcast31>{}, std::integral_constant<int, 0xc>{});
   return v;
 }
 
-// The product of a row with the token in LDS, in lane 63.  ready() is called once the first loads are asked for,
-// and returns when the token is in LDS.
-template <class Ready>
+// The product of a row with the token in LDS, in the last of its lanes.  ready() is called once the first loads are
+// asked for, and returns when the token is in LDS.
+template <int kLanes, class Ready>
 __device__ __forceinline__ float one_product(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int blocks,
                                              const u32x4 *lds, Ready ready) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x % kLanes;
   u32x4 w;
   uint32_t s;
   auto load = [&](int block) {
@@ -223,11 +235,11 @@ __device__ __forceinline__ float one_product(const uint8_t *__restrict__ codes, 
   load(lane);
   float sum = 0;
   ready();
-  for (int first = 0; first < blocks; first += 64) {
+  for (int first = 0; first < blocks; first += kLanes) {
     // behind the last block: nothing (its codes were loaded again, and LDS holds zeros)
     const u32x4 now = first + lane < blocks ? w : u32x4{0, 0, 0, 0};
     const float scale = scale_of(first + lane < blocks ? s : 0);
-    if (first + 64 < blocks) load(first + 64 + lane);
+    if (first + kLanes < blocks) load(first + kLanes + lane);
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       union {
@@ -235,12 +247,12 @@ __device__ __forceinline__ float one_product(const uint8_t *__restrict__ codes, 
         bf16x2 pair[4];
       } a, x;
       a.all = expand8(now[k], scale);
-      x.all = __builtin_bit_cast(bf16x8, lds[first * 4 + k * 64 + lane]);
+      x.all = __builtin_bit_cast(bf16x8, lds[first * 4 + k * kLanes + lane]);
 #pragma unroll
       for (int i = 0; i < 4; i++) sum = __builtin_amdgcn_fdot2_f32_bf16(a.pair[i], x.pair[i], sum, false);
     }
   }
-  return wave_sum(sum);
+  return lanes_sum<kLanes>(sum);
 }
 
 }  // namespace mx4

@@ -67,14 +67,14 @@ __device__ __forceinline__ double wave_sum(double v) {   // in lane 63
   return v;
 }
 
-// kExperts by kTokens a workgroup, whose four wavefronts share a row's length, 256 values at a time.  Sums in 64 bits,
-// in which the products are exact: which of two close logits is the larger then follows from the values,
+// kExperts by kTokens a workgroup, whose four wavefronts share a row's length, 256 values at a time, or (kShare false) a
+// wavefront, where there are enough of them.  Sums in 64 bits, in which the products are exact: which of two close logits is the larger then follows from the values,
 // not from the order of the sum.
-template <class R, int kExperts, int kTokens>
+template <class R, int kExperts, int kTokens, bool kShare>
 __global__ __launch_bounds__(256) void mx4_logits_kernel(const LayerArgs a) {
   __shared__ double parts[4][kExperts * kTokens];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int expert0 = blockIdx.x * kExperts, token0 = blockIdx.y * kTokens;
+  const int expert0 = (kShare ? blockIdx.x : blockIdx.x * 4 + wave) * kExperts, token0 = blockIdx.y * kTokens;
   const R *row[kExperts];
   const uint16_t *x[kTokens];
 #pragma unroll
@@ -101,9 +101,9 @@ __global__ __launch_bounds__(256) void mx4_logits_kernel(const LayerArgs a) {
         for (int n = 0; n < kTokens; n++)
           sum[e][n] = fma(static_cast<double>(r[e][i]), static_cast<double>(v[n][i]), sum[e][n]);
   };
-  int k = wave * 256;
+  int k = kShare ? wave * 256 : 0;
 #pragma unroll 2
-  for (; k + 256 <= a.d_model; k += 1024) {
+  for (; k + 256 <= a.d_model; k += kShare ? 1024 : 256) {
     __builtin_assume(k + 4 * lane + 4 <= a.d_model);
     add(k + 4 * lane);
   }
@@ -113,8 +113,13 @@ __global__ __launch_bounds__(256) void mx4_logits_kernel(const LayerArgs a) {
 #pragma unroll
     for (int n = 0; n < kTokens; n++) {
       const double all = wave_sum(sum[e][n]);
-      if (lane == 63) parts[wave][e * kTokens + n] = all;
+      if (kShare) {
+        if (lane == 63) parts[wave][e * kTokens + n] = all;
+      } else if (lane == 63 && expert0 + e < a.experts && token0 + n < a.tokens) {
+        a.logits[static_cast<int64_t>(token0 + n) * a.experts + expert0 + e] = static_cast<float>(all);
+      }
     }
+  if (!kShare) return;
   __syncthreads();
   if (threadIdx.x < kExperts * kTokens) {
     const int i = threadIdx.x, expert = expert0 + i / kTokens, token = token0 + i % kTokens;
@@ -156,10 +161,17 @@ constexpr Choice kNone = {0xffffffffu, -1};   // before the first (no logit has 
 __device__ __forceinline__ Choice next_choice(const float *logits, int experts, Choice last) {
   const int lane = threadIdx.x & 63;
   Choice best = {0, -1};
-  for (int e = lane; e < experts; e += 64) {
-    const uint32_t rank = rank_of(logits[e]);
+  auto look = [&](float logit, int e) {
+    const uint32_t rank = rank_of(logit);
     const bool left = rank < last.rank || (rank == last.rank && e > last.expert);
-    if (left && (best.expert < 0 || rank > best.rank)) best = {rank, e};
+    if (e < experts && left && (best.expert < 0 || rank > best.rank)) best = {rank, e};
+  };
+  for (int first = lane; first < experts; first += 256) {   // four loads on their way at once
+    float logit[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) logit[i] = logits[min(first + 64 * i, experts - 1)];
+#pragma unroll
+    for (int i = 0; i < 4; i++) look(logit[i], first + 64 * i);
   }
   const uint32_t rank = wave_max(best.expert < 0 ? 0 : best.rank);
   return {rank, static_cast<int>(~wave_max(best.expert < 0 || best.rank != rank ? 0 : ~static_cast<uint32_t>(best.expert)))};
@@ -177,8 +189,14 @@ __device__ __forceinline__ void choose(const LayerArgs &a, int token, Put put) {
     c = next_choice(logits, a.experts, c);
     if (j == 0) {
       most = logits[c.expert];
-      for (int e = lane; e < a.experts; e += 64) sum += expf(logits[e] - most);
-      sum = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mx4::wave_sum(sum)), 63));
+      for (int first = lane; first < a.experts; first += 256) {
+        float logit[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) logit[i] = logits[min(first + 64 * i, a.experts - 1)];
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum += first + 64 * i < a.experts ? expf(logit[i] - most) : 0.0f;
+      }
+      sum = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(lanes_sum<64>(sum)), 63));
     }
     const float p = expf(logits[c.expert] - most) / sum;
     taken += p;
@@ -362,65 +380,100 @@ __global__ __launch_bounds__(256) void mx4_combine_kernel(const LayerArgs a) {
 //
 // Where few tokens share an expert, grouping them costs more than it saves: a workgroup finds its token's expert by
 // itself and takes the token through kRows rows a wavefront, and the workgroups of wo add the token's experts up.
-// Three launches, with nothing between workgroups of one.
+// Three launches, or four, with nothing between workgroups of one.
 
-template <int kRows>
+// A launch of its own for many experts, whose logits are looked through once a token, and where an expert's capacity
+// makes the choice one among a sequence's tokens: a workgroup a sequence.
+__global__ __launch_bounds__(256) void mx4_choose_kernel(const LayerArgs a) {
+  __shared__ int32_t expert_of[SUB1_MX4_LAYER_TOKENS];
+  __shared__ float p_of[SUB1_MX4_LAYER_TOKENS];
+  const int first = blockIdx.x * a.length, waves = blockDim.x >> 6;
+  for (int i = threadIdx.x >> 6; i < a.length; i += waves)
+    choose(a, first + i, [&](int j, int expert, float p) {
+      a.chosen[(first + i) * a.top_k + j] = expert;
+      a.p[(first + i) * a.top_k + j] = p;
+      if (a.capacity) expert_of[i] = expert, p_of[i] = p;
+    });
+  if (!a.capacity) return;
+  __syncthreads();
+  const int mine = threadIdx.x;   // (as many threads as a sequence has tokens at most)
+  if (mine >= a.length) return;
+  int before = 0;
+  for (int i = 0; i < mine; i++) before += expert_of[i] == expert_of[mine];
+  if (before >= a.capacity) a.p[first + mine] = -p_of[mine];
+}
+static_assert(SUB1_MX4_LAYER_TOKENS <= 256, "a thread a token");
+
+template <int kRows, int kLanes, bool kChosen>
 __global__ __launch_bounds__(64 * kOneWaves) void mx4_one_wi_kernel(const LayerArgs a) {
   extern __shared__ u32x4 one_lds[];
   const int pair = blockIdx.y, token = pair / a.top_k, place = pair - token * a.top_k, width = h_width(a);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  stage_one(one_lds, a.x + static_cast<int64_t>(token) * a.d_model, a.d_model);
-  const float *logits = a.logits + static_cast<int64_t>(token) * a.experts;
-  Choice c = kNone;
-  for (int j = 0; j <= place; j++) c = next_choice(logits, a.experts, c);
-  if (blockIdx.x == 0 && place == 0 && wave == 0)   // for wo, and for the caller
-    choose(a, token, [&](int j, int expert, float p) {
-      a.chosen[pair + j] = expert;
-      a.p[pair + j] = p;
-    });
+  stage_one<kLanes>(one_lds, a.x + static_cast<int64_t>(token) * a.d_model, a.d_model);
+  int expert;
+  if (kChosen) {
+    if (a.capacity && __float_as_uint(a.p[pair]) >> 31) return;   // (the whole workgroup: no expert takes it)
+    expert = a.chosen[pair];
+  } else {
+    const float *logits = a.logits + static_cast<int64_t>(token) * a.experts;
+    Choice c = kNone;
+    for (int j = 0; j <= place; j++) c = next_choice(logits, a.experts, c);
+    expert = c.expert;
+    if (blockIdx.x == 0 && place == 0 && threadIdx.x < 64)   // for wo, and for the caller
+      choose(a, token, [&](int j, int e, float p) {
+        a.chosen[pair + j] = e;
+        a.p[pair + j] = p;
+      });
+  }
   __syncthreads();
   const int blocks = blocks_of(a.d_model);
 #pragma unroll
   for (int r = 0; r < kRows; r++) {
-    const int row = (blockIdx.x * kRows + r) * kOneWaves + wave;
+    const int row = (blockIdx.x * kRows + r) * kOneRows<kLanes> + threadIdx.x / kLanes;
     if (row >= width) return;
     float sum = 0;
     if (row < a.d_ff) {
-      const int64_t first = (static_cast<int64_t>(c.expert) * a.d_ff + row) * blocks;
-      sum = one_product(a.wi_codes + first * kBlockBytes, a.wi_scales + first, blocks, one_lds, [] {});
+      const int64_t first = (static_cast<int64_t>(expert) * a.d_ff + row) * blocks;
+      sum = one_product<kLanes>(a.wi_codes + first * kBlockBytes, a.wi_scales + first, blocks, one_lds, [] {});
     }
     // (bf16 between the layers, and zeros behind the last row, as above)
-    if ((threadIdx.x & 63) == 63)
+    if (threadIdx.x % kLanes == kLanes - 1)
       a.h[static_cast<int64_t>(pair) * width + row] = static_cast<uint16_t>(two_bf16(sum < 0 ? 0.0f : sum, 0));
   }
 }
 
-template <int kRows>
+template <int kRows, int kLanes>
 __global__ __launch_bounds__(64 * kOneWaves) void mx4_one_wo_kernel(const LayerArgs a) {
   extern __shared__ u32x4 one_lds[];
   const int token = blockIdx.y, width = h_width(a), blocks = blocks_of(a.d_ff);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float all[kRows];
 #pragma unroll
   for (int r = 0; r < kRows; r++) all[r] = 0;
   for (int j = 0; j < a.top_k; j++) {
     const int pair = token * a.top_k + j;
-    if (j) __syncthreads();
-    stage_one(one_lds, a.h + static_cast<int64_t>(pair) * width, width);
-    const int expert = a.chosen[pair];
     const float p = a.p[pair];
+    if (a.capacity && __float_as_uint(p) >> 31) {   // no expert takes the token: its input, times its share
+#pragma unroll
+      for (int r = 0; r < kRows; r++) {
+        const int row = (blockIdx.x * kRows + r) * kOneRows<kLanes> + threadIdx.x / kLanes;
+        all[r] = -p * sub1::bf16_to_f32(a.x[static_cast<int64_t>(token) * a.d_model + min(row, a.d_model - 1)]);
+      }
+      break;   // (a capacity goes with one expert a token)
+    }
+    if (j) __syncthreads();
+    stage_one<kLanes>(one_lds, a.h + static_cast<int64_t>(pair) * width, width);
+    const int expert = a.chosen[pair];
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kRows; r++) {
-      const int row = (blockIdx.x * kRows + r) * kOneWaves + wave;
+      const int row = (blockIdx.x * kRows + r) * kOneRows<kLanes> + threadIdx.x / kLanes;
       const int64_t first = (static_cast<int64_t>(expert) * a.d_model + min(row, a.d_model - 1)) * blocks;
-      all[r] += p * one_product(a.wo_codes + first * kBlockBytes, a.wo_scales + first, blocks, one_lds, [] {});
+      all[r] += p * one_product<kLanes>(a.wo_codes + first * kBlockBytes, a.wo_scales + first, blocks, one_lds, [] {});
     }
   }
 #pragma unroll
   for (int r = 0; r < kRows; r++) {
-    const int row = (blockIdx.x * kRows + r) * kOneWaves + wave;
-    if ((threadIdx.x & 63) == 63 && row < a.d_model)
+    const int row = (blockIdx.x * kRows + r) * kOneRows<kLanes> + threadIdx.x / kLanes;
+    if (threadIdx.x % kLanes == kLanes - 1 && row < a.d_model)
       a.y[static_cast<int64_t>(token) * a.d_model + row] = static_cast<uint16_t>(two_bf16(all[r], 0));
   }
 }
@@ -429,27 +482,61 @@ __global__ __launch_bounds__(64 * kOneWaves) void mx4_one_wo_kernel(const LayerA
 
 template <class R>
 int launch_logits(const LayerArgs &a, hipStream_t s) {
+  const unsigned fours = (a.tokens + 3) / 4;
   if (a.tokens == 1)
-    mx4_logits_kernel<R, 1, 1><<<dim3(a.experts, 1), 256, 0, s>>>(a);
+    mx4_logits_kernel<R, 1, 1, true><<<a.experts, 256, 0, s>>>(a);
   else if (static_cast<int64_t>(a.experts) * a.tokens <= 8192)
-    mx4_logits_kernel<R, 1, 4><<<dim3(a.experts, (a.tokens + 3) / 4), 256, 0, s>>>(a);
+    mx4_logits_kernel<R, 1, 4, true><<<dim3(a.experts, fours), 256, 0, s>>>(a);
   else
-    mx4_logits_kernel<R, 4, 4><<<dim3((a.experts + 3) / 4, (a.tokens + 3) / 4), 256, 0, s>>>(a);
+    mx4_logits_kernel<R, 4, 4, false><<<dim3((a.experts + 15) / 16, fours), 256, 0, s>>>(a);
   HIP_TRY(hipGetLastError());
   return SUB1_OK;
 }
 
-template <int kRows>
-int launch_ones(const LayerArgs &a, hipStream_t s) {
-  constexpr int kAll = kRows * kOneWaves;
-  HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_wi_kernel<kRows>));
-  HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_wo_kernel<kRows>));
-  mx4_one_wi_kernel<kRows><<<dim3((blocks_of(a.d_ff) * kBlock + kAll - 1) / kAll, a.tokens * a.top_k), 64 * kOneWaves,
-                             one_lds_bytes(a.d_model), s>>>(a);
-  HIP_TRY(hipGetLastError());
-  mx4_one_wo_kernel<kRows><<<dim3((a.d_model + kAll - 1) / kAll, a.tokens), 64 * kOneWaves, one_lds_bytes(a.d_ff), s>>>(a);
+template <int kRows, int kLanes, bool kChosen>
+int launch_one_wi(const LayerArgs &a, hipStream_t s) {
+  constexpr int kAll = kRows * kOneRows<kLanes>;
+  HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_wi_kernel<kRows, kLanes, kChosen>));
+  mx4_one_wi_kernel<kRows, kLanes, kChosen>
+      <<<dim3((blocks_of(a.d_ff) * kBlock + kAll - 1) / kAll, a.tokens * a.top_k), 64 * kOneWaves, one_lds_bytes(a.d_model), s>>>(a);
   HIP_TRY(hipGetLastError());
   return SUB1_OK;
+}
+
+template <int kRows, int kLanes>
+int launch_one_wo(const LayerArgs &a, hipStream_t s) {
+  constexpr int kAll = kRows * kOneRows<kLanes>;
+  HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_wo_kernel<kRows, kLanes>));
+  mx4_one_wo_kernel<kRows, kLanes>
+      <<<dim3((a.d_model + kAll - 1) / kAll, a.tokens), 64 * kOneWaves, one_lds_bytes(a.d_ff), s>>>(a);
+  HIP_TRY(hipGetLastError());
+  return SUB1_OK;
+}
+
+// Rows a wavefront (or half one), by how many workgroups one each would make: more of them use a token that is in LDS
+// already, fewer leave compute units idle (us of a call with 1 / 2 / 4 / 8 rows of wi: one token through 2080 x 6144,
+// 384 workgroups, 12.0 / 12.5 / 14.3 / 17.7; three, 1152, 19.0 / 18.6 / 20.1 / 23.2; eight pairs through 1024 x 4096,
+// 2048, 20.7 / 18.4 / 17.8 / 19.0; 26, 6656, 41.7 / 34.8 / 31.7 / 31.7; with 1 / 2 / 4 of wo, 260 workgroups,
+// 12.3 / 12.6 / 14.5, 512, 21.6 / 21.6 / 24, 1664, 48 / 47 / 46).
+template <int kLanes, bool kChosen>
+int launch_wi(const LayerArgs &a, hipStream_t s) {
+  const int64_t n = static_cast<int64_t>(a.tokens) * a.top_k * ((a.d_ff + kOneRows<kLanes> - 1) / kOneRows<kLanes>);
+  return n < 1000   ? launch_one_wi<1, kLanes, kChosen>(a, s)
+         : n < 2000 ? launch_one_wi<2, kLanes, kChosen>(a, s)
+         : n < 8000 ? launch_one_wi<4, kLanes, kChosen>(a, s)
+                    : launch_one_wi<8, kLanes, kChosen>(a, s);
+}
+template <int kLanes>
+int launch_wo(const LayerArgs &a, hipStream_t s) {
+  const int64_t n = static_cast<int64_t>(a.tokens) * ((a.d_model + kOneRows<kLanes> - 1) / kOneRows<kLanes>);
+  return n < 400 ? launch_one_wo<1, kLanes>(a, s) : n < 1500 ? launch_one_wo<2, kLanes>(a, s) : launch_one_wo<4, kLanes>(a, s);
+}
+template <bool kChosen>
+int launch_ones(const LayerArgs &a, hipStream_t s) {
+  const int64_t wi_rows = static_cast<int64_t>(a.tokens) * a.top_k * a.d_ff, wo_rows = static_cast<int64_t>(a.tokens) * a.d_model;
+  const int rc = halves_pay(a.d_model, wi_rows) ? launch_wi<32, kChosen>(a, s) : launch_wi<64, kChosen>(a, s);
+  if (rc) return rc;
+  return halves_pay(a.d_ff, wo_rows) ? launch_wo<32>(a, s) : launch_wo<64>(a, s);
 }
 
 int most_tiles(const sub1_mx4_layer *l, int tokens) {
@@ -506,7 +593,7 @@ extern "C" int sub1_mx4_layer_forward(const sub1_mx4_layer *layer, const void *x
                                       float *logits, int64_t *index, void *scratch, int64_t scratch_bytes,
                                       void *stream) {
   const char *who = "sub1_mx4_layer_forward";
-  const int rc = check_layer(layer, tokens, who);
+  int rc = check_layer(layer, tokens, who);
   if (rc || tokens == 0) return rc;
   if (length < 1 || tokens % length)
     return fail(SUB1_ERR_SHAPE, "%s: %d tokens are no whole sequences of %d", who, tokens, length);
@@ -529,16 +616,17 @@ extern "C" int sub1_mx4_layer_forward(const sub1_mx4_layer *layer, const void *x
               reinterpret_cast<int32_t *>(base + at.tiles), reinterpret_cast<int32_t *>(base + at.pairs),
               reinterpret_cast<int32_t *>(base + at.chosen), reinterpret_cast<float *>(base + at.p), reinterpret_cast<uint16_t *>(base + at.h),
               reinterpret_cast<float *>(base + at.out)};
-  int rc2 = layer->router_type == SUB1_MX4_FP32 ? launch_logits<float>(a, s) : launch_logits<uint16_t>(a, s);
-  if (rc2) return rc2;
-  const char *f = getenv("MX4_FORM");
-  const int pairs = tokens * a.top_k;
-  if (!a.capacity && (f ? atoi(f) : 1)) {
-    const int form = f ? atoi(f) : 1;
+  rc = layer->router_type == SUB1_MX4_FP32 ? launch_logits<float>(a, s) : launch_logits<uint16_t>(a, s);
+  if (rc) return rc;
+  // A token at a time up to three pairs an expert (us, grouped by expert in brackets: one pair of 2080 x 6144 11.9 (18.4),
+  // 26 over 128 experts of 1024 x 4096 32 (58), 128 over 64 91 (125), 32 over 8 31 (34), 64 over 8 50 (40); 64 over 32 of
+  // 1000 x 2501 39 (52); 16 over 8 of 2080 x 6144 48 (47), 32 over 8 77 (58)).
+  if (tokens * a.top_k <= 3 * a.experts) {
     sub1::note_kernel("mx4_one_wo_kernel");
-    if (form == 1) return launch_ones<1>(a, s);
-    if (form == 2) return launch_ones<2>(a, s);
-    return launch_ones<4>(a, s);
+    if (a.experts <= 256 && !a.capacity) return launch_ones<false>(a, s);
+    mx4_choose_kernel<<<tokens / length, length == 1 ? 64 : 256, 0, s>>>(a);
+    HIP_TRY(hipGetLastError());
+    return launch_ones<true>(a, s);
   }
   mx4_plan_kernel<<<1, kPlanThreads, 0, s>>>(a);
   HIP_TRY(hipGetLastError());

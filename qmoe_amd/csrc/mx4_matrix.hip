@@ -178,15 +178,24 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(const ProductAr
   });
 }
 
+template <int kLanes>
 __global__ __launch_bounds__(64 * kOneWaves) void mx4_one_kernel(const ProductArgs p) {
   extern __shared__ u32x4 one_lds[];
-  const int row = blockIdx.x * kOneWaves + (threadIdx.x >> 6), blocks = blocks_of(p.width);
+  const int row = blockIdx.x * kOneRows<kLanes> + threadIdx.x / kLanes, blocks = blocks_of(p.width);
   const int64_t first = static_cast<int64_t>(min(row, p.height - 1)) * blocks;   // (all wavefronts fill LDS)
-  const float sum = one_product(p.codes + first * kBlockBytes, p.scales + first, blocks, one_lds, [&] {
-    stage_one(one_lds, p.x, p.width);
+  const float sum = one_product<kLanes>(p.codes + first * kBlockBytes, p.scales + first, blocks, one_lds, [&] {
+    stage_one<kLanes>(one_lds, p.x, p.width);
     __syncthreads();
   });
-  if ((threadIdx.x & 63) == 63 && row < p.height) p.y[row] = static_cast<uint16_t>(two_bf16(sum, 0));
+  if (threadIdx.x % kLanes == kLanes - 1 && row < p.height) p.y[row] = static_cast<uint16_t>(two_bf16(sum, 0));
+}
+
+template <int kLanes>
+int launch_one(const ProductArgs &p, hipStream_t s) {
+  HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_kernel<kLanes>));
+  mx4_one_kernel<kLanes><<<(p.height + kOneRows<kLanes> - 1) / kOneRows<kLanes>, 64 * kOneWaves, one_lds_bytes(p.width), s>>>(p);
+  HIP_TRY(hipGetLastError());
+  return SUB1_OK;
 }
 
 // Many tokens: four wavefronts, two by two, each with 32 kRows rows of the matrix and 32 kTokens tokens, 64
@@ -867,8 +876,7 @@ int launch_product(const ProductArgs &p, hipStream_t s) {
   const unsigned rows = (p.height + 15) / 16;
   if (p.tokens == 1) {
     sub1::note_kernel("mx4_one_kernel");
-    HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_kernel));
-    mx4_one_kernel<<<(p.height + kOneWaves - 1) / kOneWaves, 64 * kOneWaves, one_lds_bytes(p.width), s>>>(p);
+    return halves_pay(p.width, p.height) ? launch_one<32>(p, s) : launch_one<64>(p, s);
   } else if (p.tokens <= 32 || p.width < 64) {
     sub1::note_kernel("mx4_few_kernel");
     if (p.tokens <= 16)

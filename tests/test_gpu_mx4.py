@@ -290,6 +290,13 @@ CONFIGS = [
     (4096, 24, 32, 1, 17, 1, False, None, torch.bfloat16),
     (64, 2080, 65, 1, 2, 1, False, None, torch.float32),
     (6, 70, 1300, 300, 1, 2, True, None, torch.float32),       # in two parts
+    (2, 100, 90, 4, 8, 1, False, 3, torch.float32),            # grouped, with a capacity
+    (2, 100, 90, 1, 40, 1, False, None, torch.bfloat16),       # and without
+    (4, 97, 300, 8, 7, 4, True, None, torch.float32),
+    (300, 600, 520, 3, 9, 2, True, None, torch.float32),       # more experts than a workgroup looks through by itself
+    (300, 72, 2100, 2, 9, 1, False, 1, torch.bfloat16),
+    (16, 1030, 700, 1, 30, 1, False, None, torch.float32),     # rows of half a wavefront, eight of them
+    (40, 500, 4200, 1, 1, 1, False, None, torch.float32),
     (6, 70, 130, 6, 100, 1, False, 20, torch.float32),         # in three, of whole sequences
 ]
 
@@ -305,6 +312,16 @@ def test_sparse_mlp(config):
     layer.router_outputs = False
     assert torch.equal(layer(hidden), y)
     assert torch.equal(layer(hidden.transpose(0, 1).contiguous().transpose(0, 1)), y)
+
+
+def test_the_forms_of_the_sparse_mlp():
+    lib = _lib.load()
+    wi, wo, _, _ = experts(4, 64, 96, 30)
+    router = torch.randn((4, 64), generator=gen(31)).cuda()
+    for top_k, tokens, capacity, name in ((1, 12, None, b'mx4_one_wo_kernel'), (1, 13, None, b'mx4_wo_kernel'), (2, 6, None, b'mx4_one_wo_kernel'),
+                                          (2, 7, None, b'mx4_wo_kernel'), (1, 12, 2, b'mx4_one_wo_kernel'), (1, 13, 2, b'mx4_wo_kernel')):
+        mx4.Mx4SparseMLP(router, wi, wo, top_k, capacity=capacity)(activations(tokens, 64, 32))
+        assert lib.sub1_last_kernel() == name
 
 
 def test_equal_logits_and_tokens_that_are_no_numbers():
