@@ -184,6 +184,7 @@ constexpr int kFewLds = kRows *kTokens * 64 * kFewWaves;   // f32x4
 // launch's; two tokens so 4.4 and 4.6 (6.5, 4.4), four 6.3 and 6.5 (7.1, 4.7).
 constexpr int kOneWaves = 8;
 constexpr int kOneMostBytes = 128 * 1024;   // of LDS, for the widest row
+constexpr int kPlainLds = 64 * 1024;        // what a launch may have without asking (which takes the host 0.4 us)
 
 __host__ __device__ constexpr int one_lds_bytes(int width) { return (blocks_of(width) + 63) / 64 * 4096; }
 static_assert(one_lds_bytes(SUB1_MX4_MAX_WIDTH) <= kOneMostBytes, "every width has room");
@@ -220,26 +221,28 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// The product of a row with the token in LDS, in the last of its lanes.  ready() is called once the first loads are
-// asked for, and returns when the token is in LDS.
-template <int kLanes, class Ready>
-__device__ __forceinline__ float one_product(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int blocks,
-                                             const u32x4 *lds, Ready ready) {
-  const int lane = threadIdx.x % kLanes;
+// What a row's lanes load first: asked for before the token is in LDS, and for all rows that a wavefront takes.
+struct OneFirst {
   u32x4 w;
   uint32_t s;
-  auto load = [&](int block) {
-    w = *reinterpret_cast<const u32x4 *>(codes + static_cast<int64_t>(min(block, blocks - 1)) * kBlockBytes);
-    s = scales[min(block, blocks - 1)];
-  };
-  load(lane);
+};
+__device__ __forceinline__ OneFirst one_block(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
+                                              int64_t first, int block, int blocks) {
+  const int64_t at = first + min(block, blocks - 1);
+  return {*reinterpret_cast<const u32x4 *>(codes + at * kBlockBytes), scales[at]};
+}
+
+// The product of the row whose blocks begin at `first` with the token in LDS, in the last of its lanes.
+template <int kLanes>
+__device__ __forceinline__ float one_product(OneFirst v, const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
+                                             int64_t first, int blocks, const u32x4 *lds) {
+  const int lane = threadIdx.x % kLanes;
   float sum = 0;
-  ready();
-  for (int first = 0; first < blocks; first += kLanes) {
+  for (int begin = 0; begin < blocks; begin += kLanes) {
     // behind the last block: nothing (its codes were loaded again, and LDS holds zeros)
-    const u32x4 now = first + lane < blocks ? w : u32x4{0, 0, 0, 0};
-    const float scale = scale_of(first + lane < blocks ? s : 0);
-    if (first + kLanes < blocks) load(first + kLanes + lane);
+    const u32x4 now = begin + lane < blocks ? v.w : u32x4{0, 0, 0, 0};
+    const float scale = scale_of(begin + lane < blocks ? v.s : 0);
+    if (begin + kLanes < blocks) v = one_block(codes, scales, first, begin + kLanes + lane, blocks);
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       union {
@@ -247,7 +250,7 @@ __device__ __forceinline__ float one_product(const uint8_t *__restrict__ codes, 
         bf16x2 pair[4];
       } a, x;
       a.all = expand8(now[k], scale);
-      x.all = __builtin_bit_cast(bf16x8, lds[first * 4 + k * kLanes + lane]);
+      x.all = __builtin_bit_cast(bf16x8, lds[begin * 4 + k * kLanes + lane]);
 #pragma unroll
       for (int i = 0; i < 4; i++) sum = __builtin_amdgcn_fdot2_f32_bf16(a.pair[i], x.pair[i], sum, false);
     }

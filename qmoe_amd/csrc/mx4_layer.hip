@@ -424,20 +424,21 @@ __global__ __launch_bounds__(64 * kOneWaves) void mx4_one_wi_kernel(const LayerA
         a.p[pair + j] = p;
       });
   }
+  const int blocks = blocks_of(a.d_model), row0 = blockIdx.x * kRows * kOneRows<kLanes> + threadIdx.x / kLanes;
+  auto first_of = [&](int r) {   // rows that are not there: the last again
+    return (static_cast<int64_t>(expert) * a.d_ff + min(row0 + r * kOneRows<kLanes>, a.d_ff - 1)) * blocks;
+  };
+  OneFirst next = one_block(a.wi_codes, a.wi_scales, first_of(0), threadIdx.x % kLanes, blocks);
   __syncthreads();
-  const int blocks = blocks_of(a.d_model);
 #pragma unroll
   for (int r = 0; r < kRows; r++) {
-    const int row = (blockIdx.x * kRows + r) * kOneRows<kLanes> + threadIdx.x / kLanes;
-    if (row >= width) return;
-    float sum = 0;
-    if (row < a.d_ff) {
-      const int64_t first = (static_cast<int64_t>(expert) * a.d_ff + row) * blocks;
-      sum = one_product<kLanes>(a.wi_codes + first * kBlockBytes, a.wi_scales + first, blocks, one_lds, [] {});
-    }
+    const int row = row0 + r * kOneRows<kLanes>;
+    const OneFirst begin = next;   // the next row's first blocks are on their way meanwhile (all rows' at once: more registers, 10 % longer)
+    if (r + 1 < kRows) next = one_block(a.wi_codes, a.wi_scales, first_of(r + 1), threadIdx.x % kLanes, blocks);
+    const float sum = one_product<kLanes>(begin, a.wi_codes, a.wi_scales, first_of(r), blocks, one_lds);
     // (bf16 between the layers, and zeros behind the last row, as above)
-    if (threadIdx.x % kLanes == kLanes - 1)
-      a.h[static_cast<int64_t>(pair) * width + row] = static_cast<uint16_t>(two_bf16(sum < 0 ? 0.0f : sum, 0));
+    if (threadIdx.x % kLanes == kLanes - 1 && row < width)
+      a.h[static_cast<int64_t>(pair) * width + row] = static_cast<uint16_t>(two_bf16(row >= a.d_ff || sum < 0 ? 0.0f : sum, 0));
   }
 }
 
@@ -459,15 +460,20 @@ __global__ __launch_bounds__(64 * kOneWaves) void mx4_one_wo_kernel(const LayerA
       }
       break;   // (a capacity goes with one expert a token)
     }
+    const int expert = a.chosen[pair];
+    auto first_of = [&](int r) {
+      const int row = (blockIdx.x * kRows + r) * kOneRows<kLanes> + threadIdx.x / kLanes;
+      return (static_cast<int64_t>(expert) * a.d_model + min(row, a.d_model - 1)) * blocks;
+    };
+    OneFirst next = one_block(a.wo_codes, a.wo_scales, first_of(0), threadIdx.x % kLanes, blocks);
     if (j) __syncthreads();
     stage_one<kLanes>(one_lds, a.h + static_cast<int64_t>(pair) * width, width);
-    const int expert = a.chosen[pair];
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kRows; r++) {
-      const int row = (blockIdx.x * kRows + r) * kOneRows<kLanes> + threadIdx.x / kLanes;
-      const int64_t first = (static_cast<int64_t>(expert) * a.d_model + min(row, a.d_model - 1)) * blocks;
-      all[r] += p * one_product<kLanes>(a.wo_codes + first * kBlockBytes, a.wo_scales + first, blocks, one_lds, [] {});
+      const OneFirst begin = next;
+      if (r + 1 < kRows) next = one_block(a.wo_codes, a.wo_scales, first_of(r + 1), threadIdx.x % kLanes, blocks);
+      all[r] += p * one_product<kLanes>(begin, a.wo_codes, a.wo_scales, first_of(r), blocks, one_lds);
     }
   }
 #pragma unroll
@@ -496,7 +502,7 @@ int launch_logits(const LayerArgs &a, hipStream_t s) {
 template <int kRows, int kLanes, bool kChosen>
 int launch_one_wi(const LayerArgs &a, hipStream_t s) {
   constexpr int kAll = kRows * kOneRows<kLanes>;
-  HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_wi_kernel<kRows, kLanes, kChosen>));
+  if (one_lds_bytes(a.d_model) > kPlainLds) HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_wi_kernel<kRows, kLanes, kChosen>));
   mx4_one_wi_kernel<kRows, kLanes, kChosen>
       <<<dim3((blocks_of(a.d_ff) * kBlock + kAll - 1) / kAll, a.tokens * a.top_k), 64 * kOneWaves, one_lds_bytes(a.d_model), s>>>(a);
   HIP_TRY(hipGetLastError());
@@ -506,7 +512,7 @@ int launch_one_wi(const LayerArgs &a, hipStream_t s) {
 template <int kRows, int kLanes>
 int launch_one_wo(const LayerArgs &a, hipStream_t s) {
   constexpr int kAll = kRows * kOneRows<kLanes>;
-  HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_wo_kernel<kRows, kLanes>));
+  if (one_lds_bytes(a.d_ff) > kPlainLds) HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_wo_kernel<kRows, kLanes>));
   mx4_one_wo_kernel<kRows, kLanes>
       <<<dim3((a.d_model + kAll - 1) / kAll, a.tokens), 64 * kOneWaves, one_lds_bytes(a.d_ff), s>>>(a);
   HIP_TRY(hipGetLastError());

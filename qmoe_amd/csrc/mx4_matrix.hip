@@ -183,16 +183,16 @@ __global__ __launch_bounds__(64 * kOneWaves) void mx4_one_kernel(const ProductAr
   extern __shared__ u32x4 one_lds[];
   const int row = blockIdx.x * kOneRows<kLanes> + threadIdx.x / kLanes, blocks = blocks_of(p.width);
   const int64_t first = static_cast<int64_t>(min(row, p.height - 1)) * blocks;   // (all wavefronts fill LDS)
-  const float sum = one_product<kLanes>(p.codes + first * kBlockBytes, p.scales + first, blocks, one_lds, [&] {
-    stage_one<kLanes>(one_lds, p.x, p.width);
-    __syncthreads();
-  });
+  const OneFirst begin = one_block(p.codes, p.scales, first, threadIdx.x % kLanes, blocks);
+  stage_one<kLanes>(one_lds, p.x, p.width);
+  __syncthreads();
+  const float sum = one_product<kLanes>(begin, p.codes, p.scales, first, blocks, one_lds);
   if (threadIdx.x % kLanes == kLanes - 1 && row < p.height) p.y[row] = static_cast<uint16_t>(two_bf16(sum, 0));
 }
 
 template <int kLanes>
 int launch_one(const ProductArgs &p, hipStream_t s) {
-  HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_kernel<kLanes>));
+  if (one_lds_bytes(p.width) > kPlainLds) HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_kernel<kLanes>));
   mx4_one_kernel<kLanes><<<(p.height + kOneRows<kLanes> - 1) / kOneRows<kLanes>, 64 * kOneWaves, one_lds_bytes(p.width), s>>>(p);
   HIP_TRY(hipGetLastError());
   return SUB1_OK;

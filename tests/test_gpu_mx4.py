@@ -130,6 +130,22 @@ def test_shapes_and_rows_that_need_a_copy():
         mx4.dequantize(codes, scales, 97)
 
 
+def test_more_blocks_than_one_launch_counts():
+    """A row of one value is a block of four threads: 2^29 + 9 of them are more than one launch's 2^31, and
+    the codes pass 2^32 bytes."""
+    rows = (1 << 29) + 9
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip('needs 40 GB')
+    x = torch.zeros((rows, 1), dtype=torch.bfloat16, device='cuda')
+    at = torch.tensor([0, 1, 1 << 28, (1 << 29) - 1, 1 << 29, rows - 2, rows - 1], device='cuda')
+    x[at, 0] = torch.arange(1, 8, device='cuda').bfloat16()
+    codes, scales = mx4.quantize(x)
+    want_codes, want_scales = mo.quantize(host(x[at]))
+    assert np.array_equal(codes[at].cpu().numpy(), want_codes) and np.array_equal(scales[at].cpu().numpy(), want_scales)
+    back = mx4.dequantize(codes, scales, 1)
+    assert np.array_equal(host(back[at]), mo.dequantize(want_codes, want_scales, 1)) and int((back != 0).sum()) == 7
+
+
 # ------------------------------------------------------------------- products ---
 
 SHAPES = [(1, 1, 1), (16, 32, 1), (17, 33, 2), (3, 127, 16), (48, 129, 17), (100, 1000, 33), (65, 2080, 64), (130, 160, 65),
@@ -226,6 +242,19 @@ def test_a_few_tokens_get_the_same_bits_whatever_tokens_they_come_with():
     want = mx4.product(x, codes, scales)
     for some in (slice(0, 2), slice(3, 8), slice(9, 30), slice(30, 32)):
         assert torch.equal(mx4.product(x[some], codes, scales), want[some])
+
+
+@pytest.mark.parametrize('tokens', [1, 5, 40, 300])
+@pytest.mark.parametrize('scale', [1, 20, 120, 200, 240])
+def test_scales_far_from_one(tokens, scale):
+    """As large and as small as a bf16 result and its fp32 sum have room for."""
+    codes, scales, _ = matrix(70, 300, 15)
+    scales.fill_(scale)
+    w = mo.dequantize(codes.cpu().numpy(), scales.cpu().numpy(), 300)
+    x = activations(tokens, 300, 16) * (2.0 ** 12 if scale < 10 else 1)
+    within(mx4.product(x, codes, scales), *mo.product_bound(host(x), w))
+    c, s = mx4.quantize(x)
+    within(mx4.product_quantized(c, s, codes, scales, 300), *mo.product_bound(host(mx4.dequantize(c, s, 300)), w))
 
 
 def test_linear_layers():
@@ -381,6 +410,9 @@ def test_on_two_streams_and_in_two_graphs():
         inputs.append(activations(40, 150, 64 + i))
         wants.append(layers[i](inputs[i]))
     linear = mx4.Mx4Linear(*matrix(90, 150, 66)[:2], 150, quantize_activations=True)
+    wide = mx4.Mx4Linear(*matrix(20, 40000, 67)[:2], 40000)     # more LDS than a launch has without asking
+    wide_x = activations(1, 40000, 68)
+    wide_want = wide(wide_x)
     linear_want = [linear(x) for x in inputs]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
@@ -408,11 +440,11 @@ def test_on_two_streams_and_in_two_graphs():
     for i in range(2):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            outputs.append((layers[i](static[i]), linear(static[i])))
+            outputs.append((layers[i](static[i]), linear(static[i]), wide(wide_x)))
         graphs.append(graph)
     for turn in range(4):
-        for (y, (logits, index)), z in outputs:
-            for t in (y, logits, index, z):
+        for (y, (logits, index)), z, u in outputs:
+            for t in (y, logits, index, z, u):
                 t.zero_()
         torch.cuda.synchronize()
         for i, s in enumerate(streams):
@@ -423,6 +455,7 @@ def test_on_two_streams_and_in_two_graphs():
         torch.cuda.synchronize()
         for i in range(2):
             assert same(outputs[i][0], i) and torch.equal(outputs[i][1], linear_want[i])
+            assert torch.equal(outputs[i][2], wide_want)
 
 
 def test_a_dense_switch_layer_brought_to_the_format():
