@@ -612,22 +612,23 @@ __device__ __forceinline__ i32x8 wide(u32x4 v) {
   return i32x8{static_cast<int>(v[0]), static_cast<int>(v[1]), static_cast<int>(v[2]), static_cast<int>(v[3]), 0, 0, 0, 0};
 }
 
-// Both sides in the format, many tokens: kSides by four wavefronts, each with 128 rows of the matrix and 64 tokens,
-// 128 values of a row a step, as mx4_many_direct_kernel fetches them; v_mfma_scale_f32_32x32x64_f8f6f4 takes a lane's
+// Both sides in the format, many tokens: kRowSides by kTokenSides wavefronts, each with 32 kRows rows of the matrix and
+// 32 kTokens tokens, 128 values of a row a step, as mx4_many_direct_kernel fetches them; v_mfma_scale_f32_32x32x64_f8f6f4 takes a lane's
 // block of 32 values as it is, and one byte of a register for its scale.  The scales come through registers, a
 // row's eight at a time: of one byte each they would be too many fetches, and of four they do not lie on four.
 // That load's wait is the compiler's, which waits for all fetches; it costs an eighth of the time (8192 x 8192 x 8192
 // 293 us, 3.8 PFLOP/s; without scales 256; the matrix cores are busy for 45 % of it, at 8.8 PFLOP/s).
-template <int kSides>
-__global__ __launch_bounds__(256 * kSides, 2) void mx4_both_kernel(const QuantizedArgs p) {
-  constexpr int kBothRows = 128 * kSides, kBothTokens = 256, kThreads = 256 * kSides, kWaves = 4 * kSides;
-  constexpr int kXFetches = 4 / kSides, kScaleRows = kBothRows + kBothTokens;
+template <int kRows, int kTokens, int kRowSides, int kTokenSides>
+__global__ __launch_bounds__(64 * kRowSides * kTokenSides, 2) void mx4_both_kernel(const QuantizedArgs p) {
+  constexpr int kBothRows = 32 * kRows * kRowSides, kBothTokens = 32 * kTokens * kTokenSides;
+  constexpr int kWaves = kRowSides * kTokenSides, kThreads = 64 * kWaves;
+  constexpr int kWFetches = kBothRows / 16 / kWaves, kXFetches = kBothTokens / 16 / kWaves, kScaleRows = kBothRows + kBothTokens;
   constexpr int kStepBytes = (kBothRows + kBothTokens) * 64, kScales = 3 * kStepBytes, kScaleBytes = (kBothRows + kBothTokens) * 8;
   // three steps of codes, rows first, then tokens: four parts of 16 bytes, part i at i ^ (row / 4 % 4); two
   // pairs of steps of scales, eight bytes a row
   __shared__ u32x4 lds[(kScales + 2 * kScaleBytes) / 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int half = lane >> 5, in_tile = lane & 31, row_side = wave % kSides, token_side = wave / kSides;
+  const int half = lane >> 5, in_tile = lane & 31, row_side = wave % kRowSides, token_side = wave / kRowSides;
   const int row0 = blockIdx.x * kBothRows, token0 = blockIdx.y * kBothTokens;
   const int blocks = blocks_of(p.width), steps = (blocks + 3) / 4;
   const uint8_t *code_tile = p.codes + static_cast<int64_t>(row0) * blocks * kBlockBytes;
@@ -636,87 +637,80 @@ __global__ __launch_bounds__(256 * kSides, 2) void mx4_both_kernel(const Quantiz
 
   // what this lane fetches of a step: 16 rows' 64 bytes a fetch
   const int part = (lane & 3) ^ (lane >> 4);
-  uint32_t w_at[2], x_at[kXFetches];
+  uint32_t w_at[kWFetches], x_at[kXFetches];
 #pragma unroll
-  for (int i = 0; i < 2; i++) w_at[i] = min((i * kWaves + wave) * 16 + (lane >> 2), p.height - 1 - row0) * blocks;
+  for (int i = 0; i < kWFetches; i++) w_at[i] = min((i * kWaves + wave) * 16 + (lane >> 2), p.height - 1 - row0) * blocks;
 #pragma unroll
   for (int i = 0; i < kXFetches; i++)
     x_at[i] = min((i * kWaves + wave) * 16 + (lane >> 2), p.tokens - 1 - token0) * blocks;
   auto fetch_step = [&](int side, int step) {
     const int block = min(4 * step + part, blocks - 1);
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int i = 0; i < kWFetches; i++)
       fetch(code_tile, (w_at[i] + block) * kBlockBytes, lds_at + side * kStepBytes + (i * kWaves + wave) * 1024);
 #pragma unroll
     for (int i = 0; i < kXFetches; i++)
       fetch(x_tile, (x_at[i] + block) * kBlockBytes, lds_at + side * kStepBytes + kBothRows * 64 + (i * kWaves + wave) * 1024);
   };
-  // a token's and a row's scales of eight blocks, or of its last eight (the caller's width has as many): each thread has a
-  // token or a row, or where there are more of them a token and the first half a row too
-  constexpr bool kTwo = kScaleRows > kThreads;
-  const bool is_token = kTwo || tid >= kBothRows, row_too = kTwo && tid < kBothRows;
-  const int my_row = kTwo ? tid : tid - kBothRows;
-  const uint8_t *row_scales = p.scales + static_cast<int64_t>(min(row0 + min(tid, kBothRows - 1), p.height - 1)) * blocks;
-  const uint8_t *first_scales =
-      is_token ? p.x_scales + static_cast<int64_t>(min(token0 + my_row, p.tokens - 1)) * blocks : row_scales;
-  struct Scales {
-    uint64_t first, second;
-  };
+  // this thread's row's or token's scales of eight blocks, or of its last eight (the caller's width has as many);
+  // threads that are left over repeat the last token
+  static_assert(kScaleRows <= kThreads, "a row or token a thread");
+  const int scale_row = min(tid, kScaleRows - 1);
+  const uint8_t *my_scales =
+      scale_row < kBothRows ? p.scales + static_cast<int64_t>(min(row0 + scale_row, p.height - 1)) * blocks
+                            : p.x_scales + static_cast<int64_t>(min(token0 + scale_row - kBothRows, p.tokens - 1)) * blocks;
   auto load_scales = [&](int pair) {
-    Scales v;
-    __builtin_memcpy(&v.first, first_scales + min(8 * pair, blocks - 8), 8);
-    if (kTwo) __builtin_memcpy(&v.second, row_scales + min(8 * pair, blocks - 8), 8);
-    return v;
+    uint64_t eight;
+    __builtin_memcpy(&eight, my_scales + min(8 * pair, blocks - 8), 8);
+    return eight;
   };
-  auto put_scales = [&](int side, int pair, const Scales &v) {   // zeros behind the last
-    const int behind = min(8 * max(8 * pair + 8 - blocks, 0), 63);
-    uint64_t *to = reinterpret_cast<uint64_t *>(lds) + (kScales + side * kScaleBytes) / 8;
-    to[is_token ? kBothRows + my_row : tid] = v.first >> behind;
-    if (row_too) to[tid] = v.second >> behind;
+  auto put_scales = [&](int side, int pair, uint64_t eight) {   // zeros behind the last
+    reinterpret_cast<uint64_t *>(lds)[(kScales + side * kScaleBytes) / 8 + scale_row] =
+        eight >> min(8 * max(8 * pair + 8 - blocks, 0), 63);
   };
 
-  f32x16 sum[4][2];
+  f32x16 sum[kRows][kTokens];
 #pragma unroll
-  for (int r = 0; r < 4; r++)
+  for (int r = 0; r < kRows; r++)
 #pragma unroll
-    for (int n = 0; n < 2; n++) sum[r][n] = f32x16{0};
+    for (int n = 0; n < kTokens; n++) sum[r][n] = f32x16{0};
 
   auto multiply = [&](int side, int scale_side, auto which) {
     constexpr int q = decltype(which)::value;   // the step's place in its pair
-    const u32x4 *w = lds + (side * kStepBytes + row_side * 128 * 64 + in_tile * 64) / 16;
-    const u32x4 *x = lds + (side * kStepBytes + kBothRows * 64 + token_side * 64 * 64 + in_tile * 64) / 16;
+    const u32x4 *w = lds + (side * kStepBytes + row_side * kRows * 32 * 64 + in_tile * 64) / 16;
+    const u32x4 *x = lds + (side * kStepBytes + kBothRows * 64 + token_side * kTokens * 32 * 64 + in_tile * 64) / 16;
     const uint64_t *scales = reinterpret_cast<const uint64_t *>(lds) + (kScales + scale_side * kScaleBytes) / 8 + in_tile;
-    uint32_t ws[4], xs[2];   // of this half's blocks: bytes 0 and 2
+    uint32_t ws[kRows], xs[kTokens];   // of this half's blocks: bytes 0 and 2
 #pragma unroll
-    for (int r = 0; r < 4; r++) ws[r] = static_cast<uint32_t>(scales[row_side * 128 + r * 32] >> (32 * q)) >> (8 * half);
+    for (int r = 0; r < kRows; r++) ws[r] = static_cast<uint32_t>(scales[(row_side * kRows + r) * 32] >> (32 * q)) >> (8 * half);
 #pragma unroll
-    for (int n = 0; n < 2; n++)
-      xs[n] = static_cast<uint32_t>(scales[kBothRows + token_side * 64 + n * 32] >> (32 * q)) >> (8 * half);
-    u32x4 a[2][4], b[2][2];
+    for (int n = 0; n < kTokens; n++)
+      xs[n] = static_cast<uint32_t>(scales[kBothRows + (token_side * kTokens + n) * 32] >> (32 * q)) >> (8 * half);
+    u32x4 a[2][kRows], b[2][kTokens];
     auto read = [&](int k) {
       const int at = (2 * k + half) ^ (in_tile >> 2 & 3);
 #pragma unroll
-      for (int r = 0; r < 4; r++) a[k][r] = w[r * 128 + at];
+      for (int r = 0; r < kRows; r++) a[k][r] = w[r * 128 + at];
 #pragma unroll
-      for (int n = 0; n < 2; n++) b[k][n] = x[n * 128 + at];
+      for (int n = 0; n < kTokens; n++) b[k][n] = x[n * 128 + at];
     };
     read(0);
     __builtin_amdgcn_sched_barrier(0);
     read(1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int r = 0; r < 4; r++)
+    for (int r = 0; r < kRows; r++)
 #pragma unroll
-      for (int n = 0; n < 2; n++)
+      for (int n = 0; n < kTokens; n++)
         sum[r][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a[0][r]), wide(b[0][n]), sum[r][n], 4, 4, 0, ws[r], 0, xs[n]);
 #pragma unroll
-    for (int r = 0; r < 4; r++)
+    for (int r = 0; r < kRows; r++)
 #pragma unroll
-      for (int n = 0; n < 2; n++)
+      for (int n = 0; n < kTokens; n++)
         sum[r][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a[1][r]), wide(b[1][n]), sum[r][n], 4, 4, 2, ws[r], 2, xs[n]);
     __builtin_amdgcn_sched_barrier(0);
   };
-  Scales scales = load_scales(0);
+  uint64_t scales = load_scales(0);
   fetch_step(0, 0);
   fetch_step(1, min(1, steps - 1));
   put_scales(0, 0, scales);
@@ -725,7 +719,7 @@ __global__ __launch_bounds__(256 * kSides, 2) void mx4_both_kernel(const Quantiz
   // next pair's scales, which the second puts where the pair before had its own.
   auto turn = [&](auto number, int step) {
     constexpr int kTurn = decltype(number)::value, q = kTurn & 1;
-    meet<2 + kXFetches>();   // but for the codes that the last turn asked for
+    meet<kWFetches + kXFetches>();   // but for the codes that the last turn asked for
     if (q == 0) scales = load_scales((step >> 1) + 1);
     fetch_step((kTurn + 2) % 3, min(step + 2, steps - 1));
     __builtin_amdgcn_sched_barrier(0);
@@ -750,25 +744,25 @@ __global__ __launch_bounds__(256 * kSides, 2) void mx4_both_kernel(const Quantiz
   meet<0>();   // nothing is on its way into LDS any more
   // to y past LDS, half of the tokens at a time
   uint16_t *out = reinterpret_cast<uint16_t *>(lds);
-  constexpr int kPitch = kBothRows + 8, kParts = kBothRows / 8, kAtOnce = kThreads / kParts, kHalf = kBothTokens / 2;
+  constexpr int kPitch = kBothRows + 8, kPieces = kBothRows / 8, kAtOnce = kThreads / kPieces, kHalf = kBothTokens / 2;
 #pragma unroll
   for (int side = 0; side < 2; side++) {
-    if (token_side / 2 == side) {
+    if (token_side / (kTokenSides / 2) == side) {
 #pragma unroll
-      for (int n = 0; n < 2; n++)
+      for (int n = 0; n < kTokens; n++)
 #pragma unroll
-        for (int r = 0; r < 4; r++)
+        for (int r = 0; r < kRows; r++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
             const uint32_t two[2] = {two_bf16(sum[r][n][4 * i], sum[r][n][4 * i + 1]),
                                      two_bf16(sum[r][n][4 * i + 2], sum[r][n][4 * i + 3])};
-            __builtin_memcpy(__builtin_assume_aligned(out + ((token_side & 1) * 64 + 32 * n + in_tile) * kPitch + row_side * 128 +
-                                                          32 * r + 8 * i + 4 * half, 8),
+            __builtin_memcpy(__builtin_assume_aligned(out + ((token_side % (kTokenSides / 2) * kTokens + n) * 32 + in_tile) * kPitch +
+                                                          (row_side * kRows + r) * 32 + 8 * i + 4 * half, 8),
                              two, 8);
           }
     }
     __syncthreads();
-    const int row = tid % kParts * 8, rows_left = p.height - row0 - row, token = tid / kParts;
+    const int row = tid % kPieces * 8, rows_left = p.height - row0 - row, token = tid / kPieces;
     const int tokens_left = p.tokens - token0 - kHalf * side - token;
     const uint16_t *from = out + token * kPitch + row;
     uint16_t *to = p.y + static_cast<int64_t>(token0 + kHalf * side + token) * p.ldy + row0 + row;
@@ -785,6 +779,14 @@ __global__ __launch_bounds__(256 * kSides, 2) void mx4_both_kernel(const Quantiz
     }
     __syncthreads();
   }
+}
+
+template <int kRows, int kTokens, int kRowSides, int kTokenSides>
+void launch_both_tiles(const QuantizedArgs &p, hipStream_t s) {
+  constexpr int kBothRows = 32 * kRows * kRowSides, kBothTokens = 32 * kTokens * kTokenSides;
+  mx4_both_kernel<kRows, kTokens, kRowSides, kTokenSides>
+      <<<dim3((p.height + kBothRows - 1) / kBothRows, (p.tokens + kBothTokens - 1) / kBothTokens),
+         64 * kRowSides * kTokenSides, 0, s>>>(p);
 }
 
 // Few tokens of both sides: as mx4_few_kernel, a lane's block of a row and of a token to one instruction
@@ -834,15 +836,17 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_both_few_kernel(const Quan
   });
 }
 
-// Which kernel (us, measured as below): to 256 tokens wavefronts that take rows and all their lines, with two tiles each
+// Which kernel (us, measured as below): to 64 tokens wavefronts that take rows and all their lines, with two tiles each
 // way as soon as that leaves half a workgroup a compute unit (61 tokens through 2080 x 6144: 2 by 2 tiles 12.8, 2
-// by 4 17.9; 130 through 6144 x 2080 9.6 and 9.1, through LDS 13.6); then tiles through LDS, of 128 x 256 (300
-// through 2080 x 6144 29.9, few 34.6), and of 256 x 256 where they are enough (2272 through 6144 x 2080, 216 tiles:
-// 26.3, small ones 32.0; 1136, 120 tiles: 20.7 and 19.6).
+// by 4 17.9; through 6144 x 2080 5.6, through LDS 6.4; 130 tokens 9.5 and 7.0); then tiles of 128 x 64 through LDS, to one
+// a compute unit (568 through 2080 x 6144, 153 of them: 20.1, of 128 x 128 23.8), of 128 x 128 (1136 through 2080 x
+// 6144, 306 small ones: 25.6, small 30.9), and of 256 x 256 where they are enough (2272 through 6144 x 2080, 216
+// of them: 25.6, of 128 x 128 35.5; 1136, 120: 20.7 and 19.1).
 void launch_both(const QuantizedArgs &p, hipStream_t s) {
   const unsigned rows = (p.height + 15) / 16;
+  const int64_t small_tiles = static_cast<int64_t>((p.height + 127) / 128) * ((p.tokens + 63) / 64);
   const int64_t large_tiles = static_cast<int64_t>((p.height + 255) / 256) * ((p.tokens + 255) / 256);
-  if (p.tokens <= 256 || blocks_of(p.width) < 8) {
+  if (p.tokens <= 64 || blocks_of(p.width) < 8) {
     sub1::note_kernel("mx4_both_few_kernel");
     const unsigned pairs = (rows + 1) / 2, fours = (p.tokens + 63) / 64;
     if (p.tokens <= 16)
@@ -853,12 +857,15 @@ void launch_both(const QuantizedArgs &p, hipStream_t s) {
       mx4_both_few_kernel<2, 2><<<dim3(pairs, (p.tokens + 31) / 32), 64 * kFewWaves, 0, s>>>(p);
     else
       mx4_both_few_kernel<2, 4><<<dim3(pairs, fours), 64 * kFewWaves, 0, s>>>(p);
+  } else if (small_tiles <= 256) {
+    sub1::note_kernel("mx4_both_kernel<2, 1>");
+    launch_both_tiles<2, 1, 2, 2>(p, s);
   } else if (large_tiles < 180) {
-    sub1::note_kernel("mx4_both_kernel<1>");
-    mx4_both_kernel<1><<<dim3((p.height + 127) / 128, (p.tokens + 255) / 256), 256, 0, s>>>(p);
+    sub1::note_kernel("mx4_both_kernel<2, 2>");
+    launch_both_tiles<2, 2, 2, 2>(p, s);
   } else {
-    sub1::note_kernel("mx4_both_kernel<2>");
-    mx4_both_kernel<2><<<dim3((p.height + 255) / 256, (p.tokens + 255) / 256), 512, 0, s>>>(p);
+    sub1::note_kernel("mx4_both_kernel<4, 2>");
+    launch_both_tiles<4, 2, 2, 4>(p, s);
   }
 }
 

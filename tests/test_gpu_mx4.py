@@ -227,8 +227,8 @@ def test_the_forms_of_the_product():
         assert lib.sub1_last_kernel() == name
         within(y, *mo.product_bound(host(x), w))
     for tokens, height, width, name in (
-            (256, 300, 256, b'mx4_both_few_kernel'), (257, 300, 256, b'mx4_both_kernel<1>'), (257, 300, 224, b'mx4_both_few_kernel'),
-            (2817, 3841, 256, b'mx4_both_kernel<2>')):
+            (64, 300, 256, b'mx4_both_few_kernel'), (65, 300, 256, b'mx4_both_kernel<2, 1>'), (257, 300, 224, b'mx4_both_few_kernel'),
+            (1000, 2100, 256, b'mx4_both_kernel<2, 2>'), (2817, 3841, 256, b'mx4_both_kernel<4, 2>')):
         codes, scales, w = matrix(height, width, tokens)
         x_codes, x_scales, x = matrix(tokens, width, tokens + 1)
         y = mx4.product_quantized(x_codes, x_scales, codes, scales, width)
