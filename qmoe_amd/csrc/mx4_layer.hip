@@ -383,8 +383,9 @@ __global__ __launch_bounds__(256) void mx4_combine_kernel(const LayerArgs a) {
 // Three launches, or four, with nothing between workgroups of one.
 
 // A launch of its own for many experts, whose logits are looked through once a token, and where an expert's capacity
-// makes the choice one among a sequence's tokens: a workgroup a sequence.
-__global__ __launch_bounds__(256) void mx4_choose_kernel(const LayerArgs a) {
+// makes the choice one among a sequence's tokens: a workgroup a sequence, a wavefront a token.
+constexpr int kChooseWaves = 16;
+__global__ __launch_bounds__(64 * kChooseWaves) void mx4_choose_kernel(const LayerArgs a) {
   __shared__ int32_t expert_of[SUB1_MX4_LAYER_TOKENS];
   __shared__ float p_of[SUB1_MX4_LAYER_TOKENS];
   const int first = blockIdx.x * a.length, waves = blockDim.x >> 6;
@@ -396,13 +397,13 @@ __global__ __launch_bounds__(256) void mx4_choose_kernel(const LayerArgs a) {
     });
   if (!a.capacity) return;
   __syncthreads();
-  const int mine = threadIdx.x;   // (as many threads as a sequence has tokens at most)
+  const int mine = threadIdx.x;
   if (mine >= a.length) return;
   int before = 0;
   for (int i = 0; i < mine; i++) before += expert_of[i] == expert_of[mine];
   if (before >= a.capacity) a.p[first + mine] = -p_of[mine];
 }
-static_assert(SUB1_MX4_LAYER_TOKENS <= 256, "a thread a token");
+static_assert(SUB1_MX4_LAYER_TOKENS <= 64 * kChooseWaves, "a thread a token");
 
 template <int kRows, int kLanes, bool kChosen>
 __global__ __launch_bounds__(64 * kOneWaves) void mx4_one_wi_kernel(const LayerArgs a) {
@@ -630,7 +631,7 @@ extern "C" int sub1_mx4_layer_forward(const sub1_mx4_layer *layer, const void *x
   if (tokens * a.top_k <= 3 * a.experts) {
     sub1::note_kernel("mx4_one_wo_kernel");
     if (a.experts <= 256 && !a.capacity) return launch_ones<false>(a, s);
-    mx4_choose_kernel<<<tokens / length, length == 1 ? 64 : 256, 0, s>>>(a);
+    mx4_choose_kernel<<<tokens / length, 64 * (length < kChooseWaves ? length : kChooseWaves), 0, s>>>(a);
     HIP_TRY(hipGetLastError());
     return launch_ones<true>(a, s);
   }
