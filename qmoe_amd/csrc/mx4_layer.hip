@@ -202,9 +202,12 @@ __device__ __forceinline__ void choose(const LayerArgs &a, int token, Put put) {
     taken += p;
     if (lane == j) mine = p, expert = c.expert;
   }
+  if (a.normalize) mine /= taken;
+  // no share is negative, and one that is no number has no sign either: a sign marks a token that keeps its input
+  mine = __uint_as_float(__float_as_uint(mine) & 0x7fffffffu);
   if (lane < a.top_k) {
     a.index[static_cast<int64_t>(token) * a.top_k + lane] = expert;
-    put(lane, expert, a.normalize ? mine / taken : mine);
+    put(lane, expert, mine);
   }
 }
 

@@ -378,6 +378,24 @@ def test_equal_logits_and_tokens_that_are_no_numbers():
             assert torch.equal(layer(clean)[0][0, fine], y[0, fine])
 
 
+@pytest.mark.parametrize('count', [2, 16, 300])
+@pytest.mark.parametrize('sign', [0, -0x8000])
+def test_tokens_that_are_no_numbers_beyond_a_capacity(count, sign):
+    """all of them go to the expert of the lowest index; those that it takes and those that keep their input are NaN"""
+    hidden = torch.full((2, 12, 64), 0x7fc0 + sign, dtype=torch.int16, device='cuda').view(torch.bfloat16)
+    wi, wo, _, _ = experts(count, 64, 96, 33)
+    layer = mx4.Mx4SparseMLP(torch.randn((count, 64), generator=gen(34)).cuda(), wi, wo, capacity=3)
+    hidden[:, 4] = 0.5
+    for _ in range(2):
+        stale = torch.ones_like(hidden)
+        del stale
+        y, (logits, index) = layer(hidden)
+        nan = torch.ones(2, 12, dtype=torch.bool, device='cuda')
+        nan[:, 4] = False
+        assert torch.equal(y.isnan().all(-1), nan) and torch.equal(y.isnan().any(-1), nan)
+        assert (index[nan] == 0).all()
+
+
 def test_all_tokens_to_one_expert():
     wi, wo, dense_wi, dense_wo = experts(5, 100, 90, 40)
     router = torch.zeros((5, 100))
