@@ -228,7 +228,8 @@ class Mx4SparseMLP(nn.Module):
             of width d_ff
     top_k   experts a token (1 to 8); `normalize`: their shares add up to 1
     capacity  with one expert a token: how many tokens of a sequence (the last but one dimension of what
-            forward gets) an expert takes; the others keep their input, times their share
+            forward gets) an expert takes; the others keep their input, times their share.  Sequences that are
+            longer than it have at most 256 tokens
     router_outputs  whether forward returns (hidden, (logits, index)) or hidden alone
 
     Logits are summed in 64 bits and rounded to fp32; of equal ones the expert of the lower index comes
@@ -286,7 +287,7 @@ class Mx4SparseMLP(nn.Module):
     def _parts(self, tokens, length):
         """(first, tokens) of each launch: whole sequences where their order counts."""
         most = _lib.MX4_LAYER_TOKENS
-        if self.capacity is not None and tokens > most:
+        if self.capacity is not None and length > self.capacity and tokens > most:
             if length > most:
                 raise ValueError('a capacity is kept over sequences of at most %d tokens, got %d' % (most, length))
             most -= most % length
@@ -298,7 +299,7 @@ class Mx4SparseMLP(nn.Module):
         b = self._buffers
         got = _quick('mx4_layer', _entry('sub1_mx4_layer_forward'), _entry('sub1_mx4_layer_scratch_bytes'), hidden, b['router'],
                      b['wi_codes'], b['wi_scales'], b['wo_codes'], b['wo_scales'], self.top_k, int(self.normalize),
-                     self.capacity or 0)
+                     self.capacity or 0)      # (one past 2^30 goes the other way)
         if got is not None:
             return (got[0], got[1:]) if self.router_outputs else got[0]
         if not isinstance(hidden, torch.Tensor):
@@ -310,12 +311,13 @@ class Mx4SparseMLP(nn.Module):
         p_x = _need(x, torch.bfloat16, 'hidden', device)
         if self.router.dtype not in (torch.bfloat16, torch.float32):
             raise TypeError('router must be bf16 or fp32, got %s' % self.router.dtype)
+        length = shape[-2]
+        capacity = self.capacity if self.capacity is not None and length > self.capacity else 0   # 0: all are taken
         p_wi = _matrix(self.wi_codes, self.wi_scales, self.d_model, 'wi', device)
         p_wo = _matrix(self.wo_codes, self.wo_scales, self.d_ff, 'wo', device)
         layer = _lib.Mx4Layer(_need(self.router, self.router.dtype, 'router', device), p_wi[0], p_wi[1], p_wo[0], p_wo[1],
                               self.experts, self.d_model, self.d_ff, self.top_k, _TYPES[self.router.dtype],
-                              self.normalize, self.capacity or 0)
-        length = shape[-2]
+                              self.normalize, capacity)
         tokens = x.numel() // self.d_model
         y = torch.empty_like(x)
         logits = torch.empty(shape[:-1] + (self.experts,), dtype=torch.float32, device=device)
@@ -327,7 +329,7 @@ class Mx4SparseMLP(nn.Module):
             scratch = torch.empty(lib.sub1_mx4_layer_scratch_bytes(ctypes.byref(layer), count), dtype=torch.uint8,
                                   device=device)
             _launch(device, lib.sub1_mx4_layer_forward, ctypes.byref(layer), p_x + 2 * first * self.d_model, count,
-                    length if self.capacity is not None else 1, y.data_ptr() + 2 * first * self.d_model,
+                    length if capacity else 1, y.data_ptr() + 2 * first * self.d_model,
                     logits.data_ptr() + 4 * first * self.experts, index.data_ptr() + 8 * first * self.top_k,
                     scratch.data_ptr(), scratch.numel())
         if self.router_outputs:

@@ -396,6 +396,19 @@ def test_tokens_that_are_no_numbers_beyond_a_capacity(count, sign):
         assert (index[nan] == 0).all()
 
 
+@pytest.mark.parametrize('capacity', [300, 2 ** 32 + 1])
+def test_a_capacity_that_no_sequence_reaches(capacity):
+    wi, wo, _, _ = experts(3, 64, 96, 35)
+    router = torch.randn((3, 64), generator=gen(36)).cuda()
+    layer = mx4.Mx4SparseMLP(router, wi, wo, capacity=capacity)
+    free = mx4.Mx4SparseMLP(router, wi, wo)
+    for length in (8, 300):
+        hidden = activations(2 * length, 64, 37).view(2, length, 64)
+        assert torch.equal(layer(hidden)[0], free(hidden)[0])
+    with pytest.raises(ValueError):
+        mx4.Mx4SparseMLP(router, wi, wo, capacity=299)(hidden)
+
+
 def test_all_tokens_to_one_expert():
     wi, wo, dense_wi, dense_wo = experts(5, 100, 90, 40)
     router = torch.zeros((5, 100))
