@@ -789,74 +789,130 @@ void launch_both_tiles(const QuantizedArgs &p, hipStream_t s) {
          64 * kRowSides * kTokenSides, 0, s>>>(p);
 }
 
-// Few tokens of both sides: as mx4_few_kernel, a lane's block of a row and of a token to one instruction
-// (v_mfma_scale_f32_16x16x128_f8f6f4), as they are.
+// Few tokens of both sides: eight wavefronts a workgroup take eight blocks of its rows and tokens in turn, and
+// v_mfma_scale_f32_16x16x128_f8f6f4 a lane's block of a row and of a token as they are.  Eight lanes read a row's
+// whole line and hand the blocks round through LDS, a part of the wavefront's own: the lanes that multiply are 16 rows
+// apart, and their own loads would be pieces of 16 bytes, one by one in the L1 (61 tokens through 2080 x 6144 12.8 us
+// with blocks four at a time and a byte of scale each, 9.3 with eight and eight bytes, through LDS 6.0).
+// The next blocks are on their way meanwhile.  What bounds it: three turns' trips to memory, and a launch.
 template <int kRows, int kTokens>
 __global__ __launch_bounds__(64 * kFewWaves) void mx4_both_few_kernel(const QuantizedArgs p) {
-  __shared__ f32x4 lds[kFewLds<kRows, kTokens>];
+  constexpr int kSides = kRows + kTokens;   // 16 rows or tokens of eight blocks each: 2 KB
+  __shared__ u32x4 lds[kFewWaves * kSides * 128];
+  static_assert(kSides * 128 * kFewWaves >= kFewLds<kRows, kTokens>, "the sums take the place of the codes");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4;
   const int row0 = blockIdx.x * 16 * kRows, token0 = blockIdx.y * 16 * kTokens;
-  const int blocks = blocks_of(p.width), steps = (blocks + 3) / 4;
-  int64_t row[kRows], token[kTokens];
+  const int blocks = blocks_of(p.width), units = (blocks + 7) / 8;
+  u32x4 *const mine = lds + wave * kSides * 128;
+  const uint8_t *codes[2] = {p.codes + static_cast<int64_t>(row0) * blocks * kBlockBytes,
+                             p.x_codes + static_cast<int64_t>(token0) * blocks * kBlockBytes};
+  const uint8_t *scales[2] = {p.scales + static_cast<int64_t>(row0) * blocks, p.x_scales + static_cast<int64_t>(token0) * blocks};
+  const int last[2] = {p.height - 1 - row0, p.tokens - 1 - token0};
+  uint32_t first[kSides][2], scale_first[kSides];
 #pragma unroll
-  for (int r = 0; r < kRows; r++) row[r] = static_cast<int64_t>(min(row0 + 16 * r + (lane & 15), p.height - 1)) * blocks;
+  for (int i = 0; i < kSides; i++) {
+    const int side = i >= kRows, at = 16 * (side ? i - kRows : i);
 #pragma unroll
-  for (int n = 0; n < kTokens; n++) token[n] = static_cast<int64_t>(min(token0 + 16 * n + (lane & 15), p.tokens - 1)) * blocks;
+    for (int h = 0; h < 2; h++) first[i][h] = min(at + 8 * h + (lane >> 3), last[side]) * blocks;
+    scale_first[i] = min(at + (lane & 15), last[side]) * blocks;
+  }
   FewSums<kRows, kTokens> sums;
 #pragma unroll
   for (int r = 0; r < kRows; r++)
 #pragma unroll
     for (int n = 0; n < kTokens; n++) sums.of[r][n] = f32x4{0, 0, 0, 0};
-#pragma unroll 2
-  for (int step = wave; step < steps; step += kFewWaves) {
-    const int block = min(4 * step + group, blocks - 1);
-    const bool there = 4 * step + group < blocks;   // behind the last block: its codes, under scales that make them nothing
-    u32x4 w[kRows], x[kTokens];
-    int ws[kRows], xs[kTokens];
+
+  u32x4 next[kSides][2];
+  uint64_t next_scales[kSides];
+  auto scales_from = [&](int unit) { return max(min(8 * unit, blocks - 8), 0); };
+  auto fetch_unit = [&](int unit) {
+    const int block = min(8 * unit + (lane & 7), blocks - 1);
 #pragma unroll
-    for (int r = 0; r < kRows; r++) {
-      w[r] = *reinterpret_cast<const u32x4 *>(p.codes + (row[r] + block) * kBlockBytes);
-      ws[r] = p.scales[row[r] + block];
+    for (int i = 0; i < kSides; i++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) next[i][h] = *reinterpret_cast<const u32x4 *>(codes[i >= kRows] + (first[i][h] + block) * kBlockBytes);
+#pragma unroll
+    for (int i = 0; i < kSides; i++) {
+      const uint8_t *from = scales[i >= kRows] + scale_first[i];
+      if (blocks >= 8) {
+        __builtin_memcpy(&next_scales[i], from + scales_from(unit), 8);
+      } else {
+        const int one = min(group, blocks - 1), two = min(4 + group, blocks - 1);
+        next_scales[i] = static_cast<uint64_t>(from[one]) << (8 * one) | static_cast<uint64_t>(from[two]) << (8 * two);
+      }
     }
+  };
+  if (wave < units) fetch_unit(wave);
+  for (int unit = wave; unit < units; unit += kFewWaves) {
+    uint64_t now[kSides];
 #pragma unroll
-    for (int n = 0; n < kTokens; n++) {
-      x[n] = *reinterpret_cast<const u32x4 *>(p.x_codes + (token[n] + block) * kBlockBytes);
-      xs[n] = p.x_scales[token[n] + block];
+    for (int i = 0; i < kSides; i++) {
+      now[i] = next_scales[i];
+#pragma unroll
+      for (int h = 0; h < 2; h++) mine[i * 128 + h * 64 + (lane & 56) + ((lane & 7) ^ (lane >> 3))] = next[i][h];
     }
+    if (unit + kFewWaves < units) fetch_unit(unit + kFewWaves);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int from = scales_from(unit);
 #pragma unroll
-    for (int r = 0; r < kRows; r++)
+    for (int i = 0; i < 2; i++) {
+      const int block = 8 * unit + 4 * i + group;
+      const bool there = block < blocks;   // behind the last block: its codes, under scales that make them nothing
+      const int by = 8 * (min(block, blocks - 1) - from);
+      u32x4 v[kSides];
+      int s[kSides];
 #pragma unroll
-      for (int n = 0; n < kTokens; n++)
-        sums.of[r][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(w[r]), wide(x[n]), sums.of[r][n], 4, 4, 0,
-                                                                         there ? ws[r] : 0, 0, there ? xs[n] : 0);
+      for (int j = 0; j < kSides; j++) {
+        v[j] = mine[j * 128 + (lane & 15) * 8 + ((4 * i + group) ^ (lane & 7))];
+        s[j] = there ? static_cast<int>(now[j] >> by) & 255 : 0;
+      }
+#pragma unroll
+      for (int r = 0; r < kRows; r++)
+#pragma unroll
+        for (int n = 0; n < kTokens; n++)
+          sums.of[r][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(v[r]), wide(v[kRows + n]), sums.of[r][n], 4, 4, 0,
+                                                                           s[r], 0, s[kRows + n]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
-  few_join<kRows, kTokens>(sums, lds, [&](int r, int n, f32x4 sum) {
+  __syncthreads();
+  few_join<kRows, kTokens>(sums, reinterpret_cast<f32x4 *>(lds), [&](int r, int n, f32x4 sum) {
     const int t = token0 + 16 * n + (lane & 15);
     if (t < p.tokens) store_four(p.y + t * p.ldy, row0 + 16 * r + 4 * group, p.height, sum);
   });
 }
 
-// Which kernel (us, measured as below): to 64 tokens wavefronts that take rows and all their lines, with two tiles each
-// way as soon as that leaves half a workgroup a compute unit (61 tokens through 2080 x 6144: 2 by 2 tiles 12.8, 2
-// by 4 17.9; through 6144 x 2080 5.6, through LDS 6.4; 130 tokens 9.5 and 7.0); then tiles of 128 x 64 through LDS, to one
+template <int kRows, int kTokens>
+void launch_both_few(const QuantizedArgs &p, hipStream_t s) {
+  const dim3 grid((p.height + 16 * kRows - 1) / (16 * kRows), (p.tokens + 16 * kTokens - 1) / (16 * kTokens));
+  mx4_both_few_kernel<kRows, kTokens><<<grid, 64 * kFewWaves, 0, s>>>(p);
+}
+
+// Which kernel (us, measured as below): wavefronts that take rows and all their blocks, in the smallest tiles that are no
+// more than the compute units (2080 x 6144: 61 tokens by 16 x 16, 16 x 32, 32 x 32, 32 x 64 7.3, 6.9, 6.0, 7.9, and
+// through LDS 12; 32 tokens 5.2, 5.0, 5.8, 7.8; 192 tokens 14.0, 12.8, 12.3, 8.6 and 12.5; 6144 x 2080: 61 tokens
+// 7.7, 6.9, 7.0, 5.8; 128 tokens, 384 of the largest, 10.2 and 6.8; 64 tokens through 1024 x 4096 3.9, 4.7, 5.5, 7.3).
+// Beyond that tiles of 128 x 64 through LDS, to one
 // a compute unit (568 through 2080 x 6144, 153 of them: 20.1, of 128 x 128 23.8), of 128 x 128 (1136 through 2080 x
 // 6144, 306 small ones: 25.6, small 30.9), and of 256 x 256 where they are enough (2272 through 6144 x 2080, 216
-// of them: 25.6, of 128 x 128 35.5; 1136, 120: 20.7 and 19.1).
+// of them: 25.6, of 128 x 128 35.5; 1136, 120: 20.7 and 19.1); not for up to 64 tokens or rows of less than a step.
 void launch_both(const QuantizedArgs &p, hipStream_t s) {
-  const unsigned rows = (p.height + 15) / 16;
-  const int64_t small_tiles = static_cast<int64_t>((p.height + 127) / 128) * ((p.tokens + 63) / 64);
-  const int64_t large_tiles = static_cast<int64_t>((p.height + 255) / 256) * ((p.tokens + 255) / 256);
-  if (p.tokens <= 64 || blocks_of(p.width) < 8) {
+  auto tiles = [&](int rows, int tokens) {
+    return static_cast<int64_t>((p.height + rows - 1) / rows) * ((p.tokens + tokens - 1) / tokens);
+  };
+  const int64_t small_tiles = tiles(128, 64), large_tiles = tiles(256, 256);
+  if (p.tokens <= 64 || tiles(32, 64) <= 256 || blocks_of(p.width) < 8) {
     sub1::note_kernel("mx4_both_few_kernel");
-    const unsigned pairs = (rows + 1) / 2, fours = (p.tokens + 63) / 64;
-    if (p.tokens <= 16)
-      mx4_both_few_kernel<1, 1><<<dim3(rows, 1), 64 * kFewWaves, 0, s>>>(p);
-    else if (p.tokens <= 32 && rows <= 256)
-      mx4_both_few_kernel<1, 2><<<dim3(rows, 1), 64 * kFewWaves, 0, s>>>(p);
-    else if (p.tokens <= 32 || static_cast<int64_t>(pairs) * fours < 128)
-      mx4_both_few_kernel<2, 2><<<dim3(pairs, (p.tokens + 31) / 32), 64 * kFewWaves, 0, s>>>(p);
+    if (p.tokens <= 16 || tiles(16, 16) <= 256)
+      launch_both_few<1, 1>(p, s);
+    else if (tiles(16, 32) <= 256)
+      launch_both_few<1, 2>(p, s);
+    else if (tiles(32, 32) <= 256)
+      launch_both_few<2, 2>(p, s);
     else
-      mx4_both_few_kernel<2, 4><<<dim3(pairs, fours), 64 * kFewWaves, 0, s>>>(p);
+      launch_both_few<2, 4>(p, s);
   } else if (small_tiles <= 256) {
     sub1::note_kernel("mx4_both_kernel<2, 1>");
     launch_both_tiles<2, 1, 2, 2>(p, s);

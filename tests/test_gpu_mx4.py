@@ -162,7 +162,9 @@ def test_product(height, width, tokens, strided):
 
 
 @pytest.mark.parametrize('height,width,tokens', SHAPES + [(300, 225, 257), (130, 224, 300), (1300, 1000, 1030), (3500, 2080, 3600),
-                                                          (2048, 4096, 20)])
+                                                          (2048, 4096, 20), (4101, 515, 70), (4099, 300, 129), (1100, 999, 500),
+                                                          (37, 2081, 31), (1000, 225, 62), (513, 257, 90), (1025, 480, 130), (7, 250, 3),
+                                                          (8200, 97, 64), (33000, 256, 18)])
 def test_product_of_two_in_the_format(height, width, tokens):
     codes, scales, w = matrix(height, width, height + width, spread=3)
     x_codes, x_scales, x = matrix(tokens, width, tokens + width, spread=2)
@@ -227,7 +229,7 @@ def test_the_forms_of_the_product():
         assert lib.sub1_last_kernel() == name
         within(y, *mo.product_bound(host(x), w))
     for tokens, height, width, name in (
-            (64, 300, 256, b'mx4_both_few_kernel'), (65, 300, 256, b'mx4_both_kernel<2, 1>'), (257, 300, 224, b'mx4_both_few_kernel'),
+            (64, 300, 256, b'mx4_both_few_kernel'), (256, 1024, 256, b'mx4_both_few_kernel'), (65, 4128, 256, b'mx4_both_kernel<2, 1>'), (257, 300, 224, b'mx4_both_few_kernel'),
             (1000, 2100, 256, b'mx4_both_kernel<2, 2>'), (2817, 3841, 256, b'mx4_both_kernel<4, 2>')):
         codes, scales, w = matrix(height, width, tokens)
         x_codes, x_scales, x = matrix(tokens, width, tokens + 1)
