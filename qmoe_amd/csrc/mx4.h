@@ -181,7 +181,7 @@ constexpr int kFewLds = kRows *kTokens * 64 * kFewWaves;   // f32x4
 // the L1 takes several times as long for, but share them among 16 tokens.)  The token's values wait in LDS, kLanes
 // blocks' four parts of 16 bytes each back to back; v_dot2_f32_bf16 multiplies two at a time.  One token
 // through 2080 x 6144 3.6 us (by the kernel above 6.1), through 6144 x 2080 3.5 (4.3), of which some 2.3 are a
-// launch's; two tokens so 4.4 and 4.6 (6.5, 4.4), four 6.3 and 6.5 (7.1, 4.7).
+// launch's; two tokens so 4.4 and 4.6 (by the kernels of a few 5.3, 4.1), four 6.3 and 6.5 (5.4, 4.3).
 constexpr int kOneWaves = 8;
 constexpr int kOneMostBytes = 128 * 1024;   // of LDS, for the widest row
 constexpr int kPlainLds = 64 * 1024;        // what a launch may have without asking (which takes the host 0.4 us)

@@ -178,6 +178,108 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(const ProductAr
   });
 }
 
+// The same for rows of a step a wavefront or more: neighbouring lanes read a row's pieces as they lie and hand them round through LDS, a part of
+// the wavefront's own, while the next step's are on their way; the lanes that multiply are rows apart, and their own
+// loads are pieces of 16 bytes, one by one in the L1.  Sums are added up in the same order.  What bounds it: the
+// activations, of which a workgroup reads four times the bytes of its 16 rows, on their way one step ahead (two and
+// three steps ahead measured alike: 13 tokens through 2080 x 6144 8.0 us each, 2 tokens 5.4).
+template <int kRows, int kTokens>
+__global__ __launch_bounds__(64 * kFewWaves) void mx4_few_lines_kernel(const ProductArgs p) {
+  constexpr int kStage = kRows * 64 + kTokens * 256;   // a wavefront's rows of 64 bytes, tokens of 256
+  __shared__ u32x4 lds[kFewWaves * kStage];
+  static_assert(kStage >= kRows * kTokens * 64, "the sums take the place of the values");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane >> 4;
+  const int row0 = blockIdx.x * 16 * kRows, token0 = blockIdx.y * 16 * kTokens;
+  const int blocks = blocks_of(p.width), steps = (blocks + 3) / 4, whole = p.width / 128;
+  const uint8_t *codes = p.codes + static_cast<int64_t>(row0) * blocks * kBlockBytes;
+  const uint8_t *scales = p.scales + static_cast<int64_t>(row0) * blocks;
+  FewSums<kRows, kTokens> sums;
+  u32x4 *const codes_lds = lds + wave * kStage, *const x_lds = codes_lds + kRows * 64;
+  int code_row[kRows], scale_row[kRows];   // rows that are not there repeat the last
+  const uint16_t *token[kTokens][4];
+#pragma unroll
+  for (int r = 0; r < kRows; r++) {
+    code_row[r] = min(16 * r + (lane >> 2), p.height - 1 - row0) * blocks;
+    scale_row[r] = min(16 * r + (lane & 15), p.height - 1 - row0) * blocks;
+  }
+#pragma unroll
+  for (int n = 0; n < kTokens; n++)
+#pragma unroll
+    for (int h = 0; h < 4; h++) token[n][h] = p.x + min(token0 + 16 * n + 4 * h + group, p.tokens - 1) * p.ldx;
+#pragma unroll
+  for (int r = 0; r < kRows; r++)
+#pragma unroll
+    for (int n = 0; n < kTokens; n++) sums.of[r][n] = f32x4{0, 0, 0, 0};
+
+  u32x4 next[kRows], next_x[kTokens][4];
+  uint32_t next_scales[kRows];
+  auto fetch = [&](int step) {
+    const int block = min(4 * step + (lane & 3), blocks - 1);
+#pragma unroll
+    for (int r = 0; r < kRows; r++) {
+      next[r] = *reinterpret_cast<const u32x4 *>(codes + (code_row[r] + block) * kBlockBytes);
+      if (blocks >= 4)
+        __builtin_memcpy(&next_scales[r], scales + scale_row[r] + min(4 * step, blocks - 4), 4);
+      else
+        next_scales[r] = static_cast<uint32_t>(scales[scale_row[r] + min(group, blocks - 1)]) << 8 * min(group, blocks - 1);
+    }
+#pragma unroll
+    for (int n = 0; n < kTokens; n++)
+#pragma unroll
+      for (int h = 0; h < 4; h++) {
+        if (token0 + 16 * n + 4 * h >= p.tokens) break;   // (what LDS holds there goes nowhere)
+        if (step < whole)
+          __builtin_memcpy(&next_x[n][h], token[n][h] + 128 * step + 8 * (lane & 15), 16);
+        else
+          next_x[n][h] = load8(token[n][h], 128 * step + 8 * (lane & 15), p.width);
+      }
+  };
+  if (wave < steps) fetch(wave);
+  for (int step = wave; step < steps; step += kFewWaves) {
+    const int block = 4 * step + group, from = blocks >= 4 ? min(4 * step, blocks - 4) : 0;
+    float scale[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; r++) {
+      // behind the last block: its codes, under a scale and with activations that make them nothing
+      scale[r] = scale_of(block < blocks ? next_scales[r] >> 8 * (block - from) & 255 : 0);
+      codes_lds[r * 64 + (lane & 60) + ((lane & 3) ^ (lane >> 3 & 3))] = next[r];
+    }
+#pragma unroll
+    for (int n = 0; n < kTokens; n++)
+#pragma unroll
+      for (int h = 0; h < 4; h++) {
+        const int i = 4 * h + group;
+        if (token0 + 16 * n + 4 * h < p.tokens) x_lds[n * 256 + 16 * i + ((lane & 15) ^ (i & 7))] = next_x[n][h];
+      }
+    if (step + kFewWaves < steps) fetch(step + kFewWaves);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    u32x4 w[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; r++) w[r] = codes_lds[r * 64 + 4 * (lane & 15) + (group ^ (lane >> 1 & 3))];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      bf16x8 v[kTokens];
+#pragma unroll
+      for (int n = 0; n < kTokens; n++)
+        v[n] = __builtin_bit_cast(bf16x8, x_lds[n * 256 + 16 * (lane & 15) + ((4 * group + k) ^ (lane & 7))]);
+#pragma unroll
+      for (int r = 0; r < kRows; r++) {
+        const bf16x8 a = expand8(w[r][k], scale[r]);
+#pragma unroll
+        for (int n = 0; n < kTokens; n++) sums.of[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, v[n], sums.of[r][n], 0, 0, 0);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  few_join<kRows, kTokens>(sums, reinterpret_cast<f32x4 *>(lds), [&](int r, int n, f32x4 sum) {
+    const int t = token0 + 16 * n + (lane & 15);
+    if (t < p.tokens) store_four(p.y + t * p.ldy, row0 + 16 * r + 4 * group, p.height, sum);
+  });
+}
+
 template <int kLanes>
 __global__ __launch_bounds__(64 * kOneWaves) void mx4_one_kernel(const ProductArgs p) {
   extern __shared__ u32x4 one_lds[];
@@ -800,7 +902,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_both_few_kernel(const Quan
   constexpr int kSides = kRows + kTokens;   // 16 rows or tokens of eight blocks each: 2 KB
   __shared__ u32x4 lds[kFewWaves * kSides * 128];
   static_assert(kSides * 128 * kFewWaves >= kFewLds<kRows, kTokens>, "the sums take the place of the codes");
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane >> 4;
   const int row0 = blockIdx.x * 16 * kRows, token0 = blockIdx.y * 16 * kTokens;
   const int blocks = blocks_of(p.width), units = (blocks + 7) / 8;
   u32x4 *const mine = lds + wave * kSides * 128;
@@ -925,29 +1027,51 @@ void launch_both(const QuantizedArgs &p, hipStream_t s) {
   }
 }
 
-// Which kernel, by what was measured on matrices of 600 x 2500 to 6144 x 2080 (us, one after the other in a graph):
-// a token alone by whole rows; up to 32 tokens, where a wavefront takes rows and all their lines (24 tokens through 4096 x 1024 4.3, shared
-// activations 5.1), two row tiles a wavefront once one makes more than a workgroup a compute unit (32 through 6144
-// x 2080 6.5, one 8.7; through 2080 x 6144 18.0 and 15.3).  Then tiles of 64 x 64, as there are few of them
-// shared by four, two or one group of four wavefronts (70 through 2080 x 6144, 66 tiles: 13.7, 15.7, 20.5; 200
+template <int kRows, int kTokens>
+dim3 few_grid(const ProductArgs &p) {
+  return dim3((p.height + 16 * kRows - 1) / (16 * kRows), (p.tokens + 16 * kTokens - 1) / (16 * kTokens));
+}
+template <int kRows, int kTokens>
+void launch_few(const ProductArgs &p, hipStream_t s) {
+  sub1::note_kernel("mx4_few_kernel");
+  mx4_few_kernel<kRows, kTokens><<<few_grid<kRows, kTokens>(p), 64 * kFewWaves, 0, s>>>(p);
+}
+template <int kRows, int kTokens>
+void launch_few_lines(const ProductArgs &p, hipStream_t s) {
+  sub1::note_kernel("mx4_few_lines_kernel");
+  mx4_few_lines_kernel<kRows, kTokens><<<few_grid<kRows, kTokens>(p), 64 * kFewWaves, 0, s>>>(p);
+}
+
+// Which kernel, by what was measured on matrices of 500 x 500 to 6144 x 2080 (us, one after the other in a graph):
+// a token alone by whole rows.  Up to 32 tokens, and more where tiles of 32 x 16 are no more than the compute units,
+// wavefronts that take rows and all their values: with pieces handed round through LDS (13 tokens through 2080 x 6144
+// 7.7 us, without 8.9; 32 through 1024 x 4096 6.0 and 10.8; 13 through 3001 x 1023 4.3 and 5.2; 16 rows a workgroup to
+// one a compute unit, then 32: 48 tokens through 2080 x 6144 11.7 and 10.5, through tiles shared as below 13.3), but
+// not in rows of less than a step a wavefront (5 through 768 x 768 3.1, without 2.7) nor for 17 to 32 tokens and
+// rows enough for two tiles each way (32 through 6144 x 2080 7.4 and 6.6).  Then tiles of 64 x 64, as there are few of
+// them shared by four, two or one group of four wavefronts (70 through 2080 x 6144, 66 tiles: 13.7, 15.7, 20.5; 200
 // through 4096 x 1024, 256 tiles: 5.9, 5.5, 5.9; 568, 576 tiles: 14.3, 10.9, 8.9), and of 128 x 128 from four
 // of the small ones a compute unit on (2272 through 6144 x 2080, 3456 tiles: 72, small ones 94).
-// Activations whose rows do not lie on 16 bytes cannot be fetched into LDS and go through registers
+// Activations whose rows do not lie on 16 bytes cannot be fetched into LDS without registers
 // (2272 through 6144 x 2080 86, 568 through 4096 x 1024 13.3).
 int launch_product(const ProductArgs &p, hipStream_t s) {
-  const int64_t small_tiles = static_cast<int64_t>((p.height + 63) / 64) * ((p.tokens + 63) / 64);
-  const unsigned rows = (p.height + 15) / 16;
+  auto tiles = [&](int rows, int tokens) {
+    return static_cast<int64_t>((p.height + rows - 1) / rows) * ((p.tokens + tokens - 1) / tokens);
+  };
+  const int64_t small_tiles = tiles(64, 64);
   if (p.tokens == 1) {
     sub1::note_kernel("mx4_one_kernel");
     return halves_pay(p.width, p.height) ? launch_one<32>(p, s) : launch_one<64>(p, s);
-  } else if (p.tokens <= 32 || p.width < 64) {
-    sub1::note_kernel("mx4_few_kernel");
-    if (p.tokens <= 16)
-      mx4_few_kernel<1, 1><<<dim3(rows, 1), 64 * kFewWaves, 0, s>>>(p);
-    else if (rows <= 256)
-      mx4_few_kernel<1, 2><<<dim3(rows, (p.tokens + 31) / 32), 64 * kFewWaves, 0, s>>>(p);
+  } else if (p.tokens <= 32 || p.width < 64 || tiles(32, 16) <= 256) {
+    const int64_t rows = tiles(16, 1 << 20);
+    if (p.width < 64 || (p.tokens > 16 && p.tokens <= 32 && rows > 256))
+      launch_few<2, 2>(p, s);
+    else if (p.tokens <= 16 && blocks_of(p.width) < 32)
+      launch_few<1, 1>(p, s);
+    else if (p.tokens <= 16 || tiles(16, 16) <= 256)
+      launch_few_lines<1, 1>(p, s);
     else
-      mx4_few_kernel<2, 2><<<dim3((rows + 1) / 2, (p.tokens + 31) / 32), 64 * kFewWaves, 0, s>>>(p);
+      launch_few_lines<2, 1>(p, s);
   } else if (misaligned(p.x, 16) || p.ldx % 8 || p.ldx >= 1 << 23) {
     sub1::note_kernel("mx4_many_kernel");
     if (small_tiles < 1024)
