@@ -1053,16 +1053,20 @@ void launch_few_lines(const ProductArgs &p, hipStream_t s) {
 // through 4096 x 1024, 256 tiles: 5.9, 5.5, 5.9; 568, 576 tiles: 14.3, 10.9, 8.9), and of 128 x 128 from four
 // of the small ones a compute unit on (2272 through 6144 x 2080, 3456 tiles: 72, small ones 94).
 // Activations whose rows do not lie on 16 bytes cannot be fetched into LDS without registers
-// (2272 through 6144 x 2080 86, 568 through 4096 x 1024 13.3).
+// (2272 through 6144 x 2080 86, 568 through 4096 x 1024 13.3), by tiles that no groups share: wavefronts that take rows
+// then pay to three tiles of 32 x 16 a compute unit (200 through 2080 x 6143, 845: 37 us, through registers 57; 50
+// through 6144 x 2079, 768: 13.4 and 15.3; 100 through 3756 x 1036, 826: 10.0 and 9.5; 400 through 2080 x 6143, 1625:
+// 68 and 58).
 int launch_product(const ProductArgs &p, hipStream_t s) {
   auto tiles = [&](int rows, int tokens) {
     return static_cast<int64_t>((p.height + rows - 1) / rows) * ((p.tokens + tokens - 1) / tokens);
   };
   const int64_t small_tiles = tiles(64, 64);
+  const bool in_lines = !misaligned(p.x, 16) && p.ldx % 8 == 0 && p.ldx < 1 << 23;   // fetch() takes them
   if (p.tokens == 1) {
     sub1::note_kernel("mx4_one_kernel");
     return halves_pay(p.width, p.height) ? launch_one<32>(p, s) : launch_one<64>(p, s);
-  } else if (p.tokens <= 32 || p.width < 64 || tiles(32, 16) <= 256) {
+  } else if (p.tokens <= 32 || p.width < 64 || tiles(32, 16) <= (in_lines ? 256 : 768)) {
     const int64_t rows = tiles(16, 1 << 20);
     if (p.width < 64 || (p.tokens > 16 && p.tokens <= 32 && rows > 256))
       launch_few<2, 2>(p, s);
@@ -1072,7 +1076,7 @@ int launch_product(const ProductArgs &p, hipStream_t s) {
       launch_few_lines<1, 1>(p, s);
     else
       launch_few_lines<2, 1>(p, s);
-  } else if (misaligned(p.x, 16) || p.ldx % 8 || p.ldx >= 1 << 23) {
+  } else if (!in_lines) {
     sub1::note_kernel("mx4_many_kernel");
     if (small_tiles < 1024)
       launch_many<1, 1, 4>(p, s);

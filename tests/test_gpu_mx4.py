@@ -151,7 +151,8 @@ def test_more_blocks_than_one_launch_counts():
 SHAPES = [(1, 1, 1), (16, 32, 1), (17, 33, 2), (3, 127, 16), (48, 129, 17), (100, 1000, 33), (65, 2080, 64), (130, 160, 65),
           (257, 96, 200), (200, 3001, 13), (300, 515, 300), (40, 64, 70), (40, 63, 70), (4100, 96, 30), (1000, 1056, 700), (77, 2049, 1), (9, 6144, 1), (2081, 100, 1),
           (3000, 416, 1100), (2050, 2080, 2100), (4100, 515, 40), (2600, 1000, 150), (4099, 225, 66), (2100, 96, 200),
-          (8200, 64, 33), (2801, 2080, 100), (333, 2079, 15), (70, 1100, 29), (4081, 1024, 17), (100, 97, 140)]
+          (8200, 64, 33), (2801, 2080, 100), (333, 2079, 15), (70, 1100, 29), (4081, 1024, 17), (100, 97, 140),
+          (8300, 70, 35), (3000, 417, 1100)]
 
 
 @pytest.mark.parametrize('height,width,tokens', SHAPES)
@@ -224,7 +225,7 @@ def test_the_forms_of_the_product():
             (1, 700, 128, False, b'mx4_one_kernel'), (1, 300, 65536, False, b'mx4_one_kernel'), (2, 700, 128, True, b'mx4_few_kernel'),
             (16, 700, 992, False, b'mx4_few_kernel'), (16, 700, 993, True, b'mx4_few_lines_kernel'), (32, 4097, 128, False, b'mx4_few_kernel'),
             (32, 4096, 128, False, b'mx4_few_lines_kernel'), (33, 2720, 128, True, b'mx4_few_lines_kernel'), (33, 2721, 128, False, b'mx4_many_direct_kernel'),
-            (33, 700, 63, False, b'mx4_few_kernel'), (33, 2721, 128, True, b'mx4_many_kernel')):
+            (33, 700, 63, False, b'mx4_few_kernel'), (33, 8192, 128, True, b'mx4_few_lines_kernel'), (33, 8193, 128, True, b'mx4_many_kernel')):
         codes, scales, w = matrix(height, width, tokens)
         x = activations(tokens, width, tokens + 1, strided)
         y = mx4.product(x, codes, scales)
