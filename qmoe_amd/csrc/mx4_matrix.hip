@@ -313,12 +313,14 @@ struct Many {
 };
 
 // The sums of a workgroup's first 256 threads to y, past LDS, so that whole lines of y are written: the lanes
-// have four rows of a token each, 8 bytes of a line.
-template <int kRows, int kTokens>
-__device__ __forceinline__ void store_tile(const f32x16 (&sum)[kRows][kTokens], uint16_t *lds, uint16_t *y, int64_t ldy,
-                                           int row0, int token0, int height, int tokens) {
+// have four rows of a token each, 8 bytes of a line.  `place` is all of the workgroup's LDS that the tile may take.
+template <int kRows, int kTokens, int kPlace>
+__device__ __forceinline__ void store_tile(const f32x16 (&sum)[kRows][kTokens], u32x4 (&place)[kPlace], uint16_t *y,
+                                           int64_t ldy, int row0, int token0, int height, int tokens) {
   using M = Many<kRows, kTokens>;
   constexpr int kPitch = M::rows + 8;   // 16 bytes further: neighbouring tokens in other banks
+  static_assert(M::tokens * kPitch * 2 <= kPlace * 16, "the tile has room");
+  uint16_t *const lds = reinterpret_cast<uint16_t *>(place);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, in_tile = lane & 31;
   const bool has_sums = tid < 256;
 #pragma unroll
@@ -364,9 +366,11 @@ __global__ __launch_bounds__(256, kWaves) void mx4_many_kernel(const ProductArgs
   constexpr int kQuarter = M::rows / 4;                       // rows
   constexpr int kCodes = (kQuarter + 31) / 32;                // loads of 16 bytes of codes, a thread and step
   // a row's or token's eight parts of 16 bytes, part i at i ^ (row % 8): eight lanes of neighbouring rows
-  // that read the same part find it in different banks
-  __shared__ u32x4 lds_x[2][M::tokens * 8], lds_w[2][M::rows * 8];
-  __shared__ uint8_t lds_s[2][M::rows * 8];
+  // that read the same part find it in different banks.  Activations, codes and scales, and the sums of all in their place
+  __shared__ u32x4 lds[2 * M::tokens * 8 + 2 * M::rows * 8 + 2 * M::rows / 2];
+  u32x4(*const lds_x)[M::tokens * 8] = reinterpret_cast<u32x4(*)[M::tokens * 8]>(lds);
+  u32x4(*const lds_w)[M::rows * 8] = reinterpret_cast<u32x4(*)[M::rows * 8]>(lds + 2 * M::tokens * 8);
+  uint8_t(*const lds_s)[M::rows * 8] = reinterpret_cast<uint8_t(*)[M::rows * 8]>(lds + 2 * M::tokens * 8 + 2 * M::rows * 8);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, in_tile = lane & 31;
   const int row0 = blockIdx.x * M::rows, token0 = blockIdx.y * M::tokens;
   const int blocks = blocks_of(p.width), steps = (blocks + 1) / 2, whole = p.width / 64;
@@ -490,7 +494,7 @@ __global__ __launch_bounds__(256, kWaves) void mx4_many_kernel(const ProductArgs
     multiply(whole);
   }
   __syncthreads();
-  store_tile<kRows, kTokens>(sum, reinterpret_cast<uint16_t *>(lds_x), p.y, p.ldy, row0, token0, p.height, p.tokens);
+  store_tile<kRows, kTokens>(sum, lds, p.y, p.ldy, row0, token0, p.height, p.tokens);
 }
 
 typedef __attribute__((address_space(3))) unsigned char *lds_bytes;
@@ -685,7 +689,7 @@ __global__ __launch_bounds__(256 * kParts, kWaves) void mx4_many_direct_kernel(c
     }
     __syncthreads();
   }
-  store_tile<kRows, kTokens>(sum, reinterpret_cast<uint16_t *>(all_lds), p.y, p.ldy, row0, token0, p.height, p.tokens);
+  store_tile<kRows, kTokens>(sum, all_lds, p.y, p.ldy, row0, token0, p.height, p.tokens);
 }
 
 template <int kRows, int kTokens, int kParts, int kWaves>
@@ -847,6 +851,7 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides, 2) void mx4_both_kern
   // to y past LDS, half of the tokens at a time
   uint16_t *out = reinterpret_cast<uint16_t *>(lds);
   constexpr int kPitch = kBothRows + 8, kPieces = kBothRows / 8, kAtOnce = kThreads / kPieces, kHalf = kBothTokens / 2;
+  static_assert(kHalf * kPitch * 2 <= sizeof(lds), "the tile has room");
 #pragma unroll
   for (int side = 0; side < 2; side++) {
     if (token_side / (kTokenSides / 2) == side) {

@@ -241,6 +241,17 @@ def test_the_forms_of_the_product():
         within(y, *mo.product_bound(x, w))
 
 
+@pytest.mark.parametrize('height,width,tokens', [(2048, 130, 2048), (2176, 2081, 2049)])
+def test_whole_tiles_of_unaligned_activations(height, width, tokens):
+    """A tile's sums lie in LDS at a pitch wider than its rows; the last tokens' are the ones that need its room."""
+    codes, scales, w = matrix(height, width, 17, spread=3)
+    x = activations(tokens, width, 18, strided=True)
+    for _ in range(2):
+        y = mx4.product(x, codes, scales)
+        assert _lib.load().sub1_last_kernel() == b'mx4_many_kernel'
+        within(y, *mo.product_bound(host(x), w))
+
+
 def test_a_few_tokens_get_the_same_bits_whatever_tokens_they_come_with():
     codes, scales, _ = matrix(200, 1000, 11)
     x = activations(32, 1000, 12)
