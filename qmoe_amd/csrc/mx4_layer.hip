@@ -620,9 +620,12 @@ extern "C" int sub1_mx4_layer_forward(const sub1_mx4_layer *layer, const void *x
                 static_cast<long long>(at.bytes));
   hipStream_t s = static_cast<hipStream_t>(stream);
   char *base = static_cast<char *>(scratch);
+  // one that no sequence reaches is none: its choice would be a launch more (a token at a time), or workgroups that
+  // look for tokens that keep their input
+  const int capacity = layer->capacity < length ? layer->capacity : 0;
   LayerArgs a{layer->router, layer->wi_codes, layer->wi_scales, layer->wo_codes, layer->wo_scales,
               static_cast<const uint16_t *>(x), static_cast<uint16_t *>(y), logits, index, tokens, length,
-              layer->experts, layer->d_model, layer->d_ff, layer->top_k, layer->normalize, layer->capacity,
+              layer->experts, layer->d_model, layer->d_ff, layer->top_k, layer->normalize, capacity,
               reinterpret_cast<int32_t *>(base + at.tiles), reinterpret_cast<int32_t *>(base + at.pairs),
               reinterpret_cast<int32_t *>(base + at.chosen), reinterpret_cast<float *>(base + at.p), reinterpret_cast<uint16_t *>(base + at.h),
               reinterpret_cast<float *>(base + at.out)};

@@ -425,6 +425,36 @@ def test_a_capacity_that_no_sequence_reaches(capacity):
         mx4.Mx4SparseMLP(router, wi, wo, capacity=299)(hidden)
 
 
+def launches(call):
+    """How many nodes the call's launches make in a captured graph, which is not run."""
+    call()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    count = ctypes.c_size_t()
+    assert _lib.load().hipGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(count)) == 0
+    return count.value
+
+
+@pytest.mark.parametrize('shape,free_launches', [((1, 1), 3), ((2, 3), 3), ((5, 4), 3), ((9, 5), 4)])
+def test_a_capacity_that_cannot_bind_takes_no_launch(shape, free_launches):
+    """Sequences no longer than the capacity: launches and bits of a layer without one.  The choice among a
+    sequence's tokens is a launch of its own in the form for a token at a time, and part of the plan in the other."""
+    wi, wo, dense_wi, dense_wo = experts(8, 64, 96, 38)
+    router = torch.randn((8, 64), generator=gen(39)).cuda()
+    hidden = activations(shape[0] * shape[1], 64, 40).view(shape + (64,))
+    free = mx4.Mx4SparseMLP(router, wi, wo, router_outputs=False)
+    assert launches(lambda: free(hidden)) == free_launches
+    for capacity in (shape[1], 64):
+        layer = mx4.Mx4SparseMLP(router, wi, wo, capacity=capacity, router_outputs=False)
+        assert launches(lambda: layer(hidden)) == free_launches
+        assert torch.equal(layer(hidden), free(hidden))
+    if shape[1] > 1:
+        layer = mx4.Mx4SparseMLP(router, wi, wo, capacity=shape[1] - 1)
+        assert launches(lambda: layer(hidden)) == 4
+        against_the_oracle(layer, hidden, dense_wi, dense_wo)
+
+
 def test_all_tokens_to_one_expert():
     wi, wo, dense_wi, dense_wo = experts(5, 100, 90, 40)
     router = torch.zeros((5, 100))
