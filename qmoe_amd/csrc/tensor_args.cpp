@@ -265,17 +265,18 @@ PyObject *mx4_dequantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
   }
 }
 
-// mx4_product(entry, None or the entry that quantizes x first, x, codes, scales, device, stream)
+// mx4_product(entry, None or the entry that quantizes x first, x, codes, scales, the matrix' width or 0 for x's, device,
+// stream)
 PyObject *mx4_product(PyObject *, PyObject *const *args, Py_ssize_t n) {
   void *entry, *quantize = nullptr, *stream;
-  int64_t device, rows, width, ld;
-  if (n != 7 || !address(args[0], &entry) || (args[1] != Py_None && !address(args[1], &quantize)) ||
-      !integer(args[5], &device) || !address(args[6], &stream))
+  int64_t device, rows, width, ld, expected;
+  if (n != 8 || !address(args[0], &entry) || (args[1] != Py_None && !address(args[1], &quantize)) ||
+      !integer(args[5], &expected) || !integer(args[6], &device) || !address(args[7], &stream))
     Py_RETURN_NONE;
   try {
     const at::Tensor *x = plain(args[2], device), *codes = plain(args[3], device), *scales = plain(args[4], device);
     if (!x || !codes || !scales || x->scalar_type() != at::kBFloat16 || !rows_of(*x, &rows, &width, &ld) || rows < 1 ||
-        rows > SUB1_MX4_MAX_TOKENS || !matrix_in_format(*codes, *scales, width, 2))
+        rows > SUB1_MX4_MAX_TOKENS || (expected && width != expected) || !matrix_in_format(*codes, *scales, width, 2))
       Py_RETURN_NONE;
     const int64_t height = codes->size(0);
     if (height > SUB1_MX4_MAX_WIDTH) Py_RETURN_NONE;

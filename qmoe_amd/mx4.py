@@ -134,7 +134,7 @@ def _fewer_tokens(x, what):
 
 def product(x, codes, scales):
     """bf16 [.., H] = x W^T for x bf16 [.., W] and W [H, W] in the format; fp32 sums."""
-    got = _quick('mx4_product', _entry('sub1_mx4_product'), None, x, codes, scales)
+    got = _quick('mx4_product', _entry('sub1_mx4_product'), None, x, codes, scales, 0)
     if got is not None:
         return got
     rows, ld = _rows(x, 'x')
@@ -203,11 +203,14 @@ class Mx4Linear(nn.Module):
         buffers = self._buffers
         codes, scales = buffers['codes'], buffers['scales']
         if self.quantize_activations:
-            got = _quick('mx4_product', _entry('sub1_mx4_product_quantized'), _entry('sub1_mx4_quantize'), x, codes, scales)
+            got = _quick('mx4_product', _entry('sub1_mx4_product_quantized'), _entry('sub1_mx4_quantize'), x, codes, scales,
+                         self.width)
         else:
-            got = _quick('mx4_product', _entry('sub1_mx4_product'), None, x, codes, scales)
-        if got is not None and x.shape[-1] == self.width:
+            got = _quick('mx4_product', _entry('sub1_mx4_product'), None, x, codes, scales, self.width)
+        if got is not None:
             return got
+        if not isinstance(x, torch.Tensor):
+            raise TypeError('x must be a torch.Tensor')
         if x.shape[-1:] != (self.width,):
             raise ValueError('x must be [.., %d], got %s' % (self.width, tuple(x.shape)))
         if not self.quantize_activations:

@@ -296,6 +296,23 @@ def test_linear_layers():
                 layer(wrong)
 
 
+@pytest.mark.parametrize('quantized', [False, True])
+def test_another_width_of_as_many_blocks_runs_nothing(quantized):
+    codes, scales, _ = matrix(50, 60, 41)
+    layer = mx4.Mx4Linear(codes, scales, 60, quantize_activations=quantized)
+    lib = _lib.load()
+    mx4.product(activations(1, 60, 42), codes, scales)
+    before = lib.sub1_last_kernel()
+    assert before == b'mx4_one_kernel'
+    for width in (64, 33):
+        with pytest.raises(ValueError, match='x must be'):
+            layer(activations(5, width, 43))
+        assert lib.sub1_last_kernel() == before
+    for wrong, error in ((None, TypeError), ([1.0] * 60, TypeError), (torch.zeros((), device='cuda').bfloat16(), ValueError)):
+        with pytest.raises(error):
+            layer(wrong)
+
+
 # ----------------------------------------------------------------- the sparse MLP ---
 
 def experts(count, d_model, d_ff, seed):

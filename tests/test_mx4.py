@@ -117,6 +117,19 @@ def test_modules_refuse_what_is_not_a_matrix_in_the_format():
         mx4.dequantize(codes, scales, 64, torch.int32)
 
 
+@pytest.mark.parametrize('quantized', [False, True])
+def test_a_layer_refuses_another_width_before_it_looks_further(quantized):
+    layer = mx4.Mx4Linear(torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 2, dtype=torch.uint8), 60, quantized)
+    for wrong in (torch.zeros(2, 64).bfloat16(), torch.zeros(2, 33), torch.tensor(1.0)):
+        with pytest.raises(ValueError, match='x must be \\[.., 60\\]'):
+            layer(wrong)
+    for wrong in (None, [0.0] * 60):
+        with pytest.raises(TypeError):
+            layer(wrong)
+    with pytest.raises(ValueError, match='GPU'):
+        layer(torch.zeros(2, 60).bfloat16())
+
+
 def test_the_sparse_mlp_refuses():
     def stack(experts, height, width):
         nb = mo.blocks_of(width)
