@@ -140,11 +140,12 @@ PyObject *layer_addresses(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // ---- calls on microscaled 4-bit matrices ----
 
-// The tensor behind a plain one on GPU `device`; null if it is anything else.
+// The tensor behind a plain one on GPU `device`; null if it is anything else, one whose values torch negates when it reads
+// them among it.
 const at::Tensor *plain(PyObject *object, int64_t device) {
   if (!THPVariable_CheckExact(object)) return nullptr;
   const at::Tensor &t = THPVariable_Unpack(object);
-  return t.defined() && t.is_cuda() && t.device().index() == device && t.layout() == at::kStrided ? &t : nullptr;
+  return t.defined() && t.is_cuda() && t.device().index() == device && t.layout() == at::kStrided && !t.is_neg() ? &t : nullptr;
 }
 
 bool address(PyObject *object, void **out) {

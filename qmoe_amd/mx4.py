@@ -67,6 +67,7 @@ def _rows(x, name, device=None):
         raise ValueError('%s must have a last dimension, got %s' % (name, tuple(x.shape)))
     if x.shape[-1] > _lib.MX4_MAX_WIDTH:
         raise ValueError('%s has rows of %d, more than %d' % (name, x.shape[-1], _lib.MX4_MAX_WIDTH))
+    x = x.resolve_neg()
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
     if x.stride(1) != 1 and x.shape[1] > 1 or x.stride(0) < x.shape[1] and x.shape[0] > 1:
@@ -310,7 +311,7 @@ class Mx4SparseMLP(nn.Module):
         if hidden.dim() < 2 or hidden.shape[-1] != self.d_model:
             raise ValueError('hidden must be [.., S, %d], got %s' % (self.d_model, tuple(hidden.shape)))
         device, shape = self.router.device, hidden.shape
-        x = hidden.contiguous()
+        x = hidden.contiguous().resolve_neg()
         p_x = _need(x, torch.bfloat16, 'hidden', device)
         if self.router.dtype not in (torch.bfloat16, torch.float32):
             raise TypeError('router must be bf16 or fp32, got %s' % self.router.dtype)

@@ -574,6 +574,22 @@ def test_a_dense_switch_layer_brought_to_the_format():
     within(layer(hidden).view(22, 64), exact, bound)
 
 
+def test_values_that_torch_keeps_with_the_other_sign():
+    """A conjugate's imaginary part is a view whose values torch negates when they are read."""
+    parts = torch.view_as_complex(torch.randn((40, 3, 2), generator=gen(44)).cuda()).conj().imag
+    for x in (parts[:, :1], parts, torch._neg_view(parts.contiguous())):
+        assert x.is_neg()
+        codes, scales = mx4.quantize(x)
+        want_codes, want_scales = mo.quantize(host(x))
+        assert np.array_equal(codes.cpu().numpy(), want_codes) and np.array_equal(scales.cpu().numpy(), want_scales)
+    codes, scales, w = matrix(70, 100, 45)
+    x = torch._neg_view(activations(9, 100, 46))
+    within(mx4.product(x, codes, scales), *mo.product_bound(host(x), w))
+    wi, wo, dense_wi, dense_wo = experts(4, 100, 96, 47)
+    layer = mx4.Mx4SparseMLP(torch.randn((4, 100), generator=gen(48)).cuda(), wi, wo)
+    against_the_oracle(layer, x, dense_wi, dense_wo)
+
+
 def test_quantised_layers_in_a_row_as_a_block_runs_them():
     """A 4-bit projection, the sparse MLP on its result, a 4-bit projection with 4-bit activations."""
     g = gen(80)
