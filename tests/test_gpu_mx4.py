@@ -313,6 +313,44 @@ def test_another_width_of_as_many_blocks_runs_nothing(quantized):
             layer(wrong)
 
 
+@pytest.mark.parametrize('height,width,tokens,strided', [
+    (300, 65536, 1, False), (300, 65535, 1, True), (300, 40000, 1, False), (40, 32769, 1, True), (300, 6144, 1, False),
+    (4097, 1024, 1, False), (50, 65536, 5, False), (50, 65535, 13, True), (700, 993, 16, True), (4100, 900, 31, False),
+    (2721, 2081, 33, True), (130, 65536, 70, False), (130, 65533, 90, True), (1000, 3008, 300, False), (2048, 130, 2048, True),
+    (2048, 2080, 2050, False)])
+@pytest.mark.parametrize('quantized', [False, True])
+def test_sums_that_are_exact(height, width, tokens, strided, quantized):
+    """Activations of a few whole numbers under one scale: fp32 adds them up exactly in any order, so y is the
+    exact value, rounded once.  A value left out shows, at whatever width."""
+    codes, scales, w = matrix(height, width, 90)
+    x = torch.randint(-3, 4, (tokens, width), generator=gen(91)).bfloat16()
+    x[:, [0, -1]] = 3.0
+    unit = np.abs(w[w != 0]).min()
+    assert (host(x[:1].abs()) @ np.abs(w).T).max() / unit < 2 ** 24 and (3 * np.abs(w).sum(-1)).max() / unit < 2 ** 24
+    want = torch.from_numpy(host(x) @ w.T).float().bfloat16()         # (exact in fp32)
+    if strided:
+        whole = torch.full((tokens, width + 7), float('nan'), dtype=torch.bfloat16)
+        whole[:, 3:3 + width] = x
+        x = whole.cuda()[:, 3:3 + width]
+    layer = mx4.Mx4Linear(codes, scales, width, quantize_activations=quantized)
+    assert torch.equal(layer(x.cuda()).cpu(), want)
+
+
+@pytest.mark.parametrize('width', [900, 993, 2080, 2081])
+def test_both_forms_for_a_few_tokens_sum_alike(width):
+    """From the row's length alone: a token's bits are the same with 31 others, fifteen or one."""
+    lib = _lib.load()
+    codes, scales, _ = matrix(4112, width, 95, spread=3)
+    x = activations(32, width, 96)
+    want = mx4.product(x, codes, scales)
+    assert lib.sub1_last_kernel() == b'mx4_few_kernel'
+    for some in (slice(0, 16), slice(16, 32), slice(30, 32)):
+        assert torch.equal(mx4.product(x[some], codes, scales), want[some])
+        assert lib.sub1_last_kernel() == (b'mx4_few_kernel' if width < 993 else b'mx4_few_lines_kernel')
+    assert torch.equal(mx4.product(x, codes[:2000], scales[:2000]), want[:, :2000])
+    assert lib.sub1_last_kernel() == b'mx4_few_lines_kernel'
+
+
 # ----------------------------------------------------------------- the sparse MLP ---
 
 def experts(count, d_model, d_ff, seed):
@@ -470,6 +508,54 @@ def test_a_capacity_that_cannot_bind_takes_no_launch(shape, free_launches):
         layer = mx4.Mx4SparseMLP(router, wi, wo, capacity=shape[1] - 1)
         assert launches(lambda: layer(hidden)) == 4
         against_the_oracle(layer, hidden, dense_wi, dense_wo)
+
+
+@pytest.mark.parametrize('d_model,d_ff,tokens,capacity', [
+    (64, 40000, 1, None), (64, 65536, 3, None), (64, 65535, 6, 2), (40000, 64, 1, None), (65536, 96, 6, None), (65535, 70, 5, 1),
+    (64, 40000, 20, None), (40000, 64, 20, None), (64, 65536, 20, 7)])
+def test_wide_experts_exactly(d_model, d_ff, tokens, capacity):
+    """Rows that need more LDS than a launch has without asking, in numbers whose sums are exact: tokens go to
+    the two experts in turn with a share of one, h is small."""
+    wi, wo = matrix(2 * d_ff, d_model, 92), matrix(2 * d_model, d_ff, 93)
+    wi[0][:, 0] &= 0xf0                                       # the first value chooses the expert and does nothing else
+    dense_wi, dense_wo = wi[2].reshape(2, d_ff, d_model), wo[2].reshape(2, d_model, d_ff)
+    dense_wi[:, :, 0] = 0
+    shaped = [tuple(t.view(2, -1, t.shape[-1]) for t in m[:2]) for m in (wi, wo)]
+    router = torch.zeros((2, d_model))
+    router[0, 0], router[1, 0] = 4, -4
+    x = torch.zeros((tokens, d_model))
+    at = torch.randint(1, d_model - 1, (tokens, 2), generator=gen(94))
+    x.scatter_(1, at, 1.0)
+    x[:, -1] = -1
+    x[:, 0] = 64.0 * (1 - 2 * (torch.arange(tokens) % 2))
+    layer = mx4.Mx4SparseMLP(router.cuda(), *shaped, capacity=capacity)
+    y, (logits, index) = layer(x.bfloat16().cuda().view(1, tokens, d_model))
+    assert index.flatten().tolist() == [t % 2 for t in range(tokens)]
+    for t in range(tokens):
+        if capacity is not None and t // 2 >= capacity:
+            want = x[t].numpy().astype(np.float64)
+        else:
+            h = host(torch.from_numpy(np.maximum(dense_wi[t % 2] @ x[t].double().numpy(), 0)).float().bfloat16())
+            unit = np.abs(dense_wo[dense_wo != 0]).min() * np.abs(h[h != 0]).min()
+            assert (np.abs(dense_wo[t % 2]) @ h).max() / unit < 2 ** 24
+            want = dense_wo[t % 2] @ h
+        assert torch.equal(y[0, t].cpu(), torch.from_numpy(want).float().bfloat16()), t
+
+
+@pytest.mark.parametrize('capacity', [1, 2, 3])
+@pytest.mark.parametrize('count', [6, 2])
+def test_a_capacity_beside_tokens_that_are_no_numbers(capacity, count):
+    """They take places of the experts that they go to; the others' results are the oracle's."""
+    wi, wo, dense_wi, dense_wo = experts(count, 64, 96, 30)
+    router = torch.randn((count, 64), generator=gen(31))
+    hidden = activations(18, 64, 32).view(2, 9, 64)
+    hidden[0, 2] = 0
+    hidden[:, 5, 3] = float('nan')
+    hidden[1, 7, 9] = float('inf')
+    y, _, _ = against_the_oracle(mx4.Mx4SparseMLP(router.cuda(), wi, wo, capacity=capacity), hidden, dense_wi, dense_wo)
+    nan = torch.zeros(2, 9, dtype=torch.bool)
+    nan[:, 5] = nan[1, 7] = True
+    assert torch.equal(y.isnan().all(-1).cpu(), nan) and torch.equal(y.isnan().any(-1).cpu(), nan)
 
 
 def test_all_tokens_to_one_expert():
