@@ -68,8 +68,8 @@ __device__ __forceinline__ double wave_sum(double v) {   // in lane 63
 }
 
 // kExperts by kTokens a workgroup, whose four wavefronts share a row's length, 256 values at a time, or (kShare false) a
-// wavefront, where there are enough of them.  Sums in 64 bits, in which the products are exact: which of two close logits is the larger then follows from the values,
-// not from the order of the sum.
+// wavefront, where there are enough of them.  Sums in 64 bits, in which the products are exact: which of two close
+// logits is the larger then follows from the values, not from the order of the sum.
 template <class R, int kExperts, int kTokens, bool kShare>
 __global__ __launch_bounds__(256) void mx4_logits_kernel(const LayerArgs a) {
   __shared__ double parts[4][kExperts * kTokens];
@@ -437,7 +437,8 @@ __global__ __launch_bounds__(64 * kOneWaves) void mx4_one_wi_kernel(const LayerA
 #pragma unroll
   for (int r = 0; r < kRows; r++) {
     const int row = row0 + r * kOneRows<kLanes>;
-    const OneFirst begin = next;   // the next row's first blocks are on their way meanwhile (all rows' at once: more registers, 10 % longer)
+    // the next row's first blocks are on their way meanwhile (all rows' at once: more registers, 10 % longer)
+    const OneFirst begin = next;
     if (r + 1 < kRows) next = one_block(a.wi_codes, a.wi_scales, first_of(r + 1), threadIdx.x % kLanes, blocks);
     const float sum = one_product<kLanes>(begin, a.wi_codes, a.wi_scales, first_of(r), blocks, one_lds);
     // (bf16 between the layers, and zeros behind the last row, as above)
@@ -508,7 +509,8 @@ int launch_one_wi(const LayerArgs &a, hipStream_t s) {
   constexpr int kAll = kRows * kOneRows<kLanes>;
   if (one_lds_bytes(a.d_model) > kPlainLds) HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx4_one_wi_kernel<kRows, kLanes, kChosen>));
   mx4_one_wi_kernel<kRows, kLanes, kChosen>
-      <<<dim3((blocks_of(a.d_ff) * kBlock + kAll - 1) / kAll, a.tokens * a.top_k), 64 * kOneWaves, one_lds_bytes(a.d_model), s>>>(a);
+      <<<dim3((blocks_of(a.d_ff) * kBlock + kAll - 1) / kAll, a.tokens * a.top_k), 64 * kOneWaves,
+         one_lds_bytes(a.d_model), s>>>(a);
   HIP_TRY(hipGetLastError());
   return SUB1_OK;
 }
@@ -627,8 +629,8 @@ extern "C" int sub1_mx4_layer_forward(const sub1_mx4_layer *layer, const void *x
               static_cast<const uint16_t *>(x), static_cast<uint16_t *>(y), logits, index, tokens, length,
               layer->experts, layer->d_model, layer->d_ff, layer->top_k, layer->normalize, capacity,
               reinterpret_cast<int32_t *>(base + at.tiles), reinterpret_cast<int32_t *>(base + at.pairs),
-              reinterpret_cast<int32_t *>(base + at.chosen), reinterpret_cast<float *>(base + at.p), reinterpret_cast<uint16_t *>(base + at.h),
-              reinterpret_cast<float *>(base + at.out)};
+              reinterpret_cast<int32_t *>(base + at.chosen), reinterpret_cast<float *>(base + at.p),
+              reinterpret_cast<uint16_t *>(base + at.h), reinterpret_cast<float *>(base + at.out)};
   rc = layer->router_type == SUB1_MX4_FP32 ? launch_logits<float>(a, s) : launch_logits<uint16_t>(a, s);
   if (rc) return rc;
   // A token at a time up to three pairs an expert (us, grouped by expert in brackets: one pair of 2080 x 6144 11.9 (18.4),

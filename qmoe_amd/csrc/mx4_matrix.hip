@@ -178,9 +178,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(const ProductAr
   });
 }
 
-// The same for rows of a step a wavefront or more: neighbouring lanes read a row's pieces as they lie and hand them round through LDS, a part of
-// the wavefront's own, while the next step's are on their way; the lanes that multiply are rows apart, and their own
-// loads are pieces of 16 bytes, one by one in the L1.  Sums are added up in the same order.  What bounds it: the
+// The same for rows of a step a wavefront or more: neighbouring lanes read a row's pieces as they lie and hand them
+// round through LDS, a part of the wavefront's own, while the next step's are on their way; the lanes that multiply
+// are rows apart, and their own loads are pieces of 16 bytes, one by one in the L1.  Sums are added up in the same order.  What bounds it: the
 // activations, of which a workgroup reads four times the bytes of its 16 rows, on their way one step ahead (two and
 // three steps ahead measured alike: 13 tokens through 2080 x 6144 8.0 us each, 2 tokens 5.4).
 template <int kRows, int kTokens>
@@ -267,7 +267,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_few_lines_kernel(const Pro
       for (int r = 0; r < kRows; r++) {
         const bf16x8 a = expand8(w[r][k], scale[r]);
 #pragma unroll
-        for (int n = 0; n < kTokens; n++) sums.of[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, v[n], sums.of[r][n], 0, 0, 0);
+        for (int n = 0; n < kTokens; n++)
+          sums.of[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, v[n], sums.of[r][n], 0, 0, 0);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -487,7 +488,8 @@ __global__ __launch_bounds__(256, kWaves) void mx4_many_kernel(const ProductArgs
     if (step < whole) turn(even, odd, step);
   }
   if (whole < steps) {   // the last step, where the row ends inside it: its codes are there
-        for (int i = 0; i < kLoads; i++)
+#pragma unroll
+    for (int i = 0; i < kLoads; i++)
       lds_x[whole & 1][(mine + 32 * i) * 8 + (part ^ (mine >> 1 & 7))] =
           load8(p.x + min(token0 + mine + 32 * i, p.tokens - 1) * p.ldx, whole * 64 + part * 8, p.width);
     __syncthreads();
@@ -719,8 +721,8 @@ __device__ __forceinline__ i32x8 wide(u32x4 v) {
 }
 
 // Both sides in the format, many tokens: kRowSides by kTokenSides wavefronts, each with 32 kRows rows of the matrix and
-// 32 kTokens tokens, 128 values of a row a step, as mx4_many_direct_kernel fetches them; v_mfma_scale_f32_32x32x64_f8f6f4 takes a lane's
-// block of 32 values as it is, and one byte of a register for its scale.  The scales come through registers, a
+// 32 kTokens tokens, 128 values of a row a step, as mx4_many_direct_kernel fetches them;
+// v_mfma_scale_f32_32x32x64_f8f6f4 takes a lane's block of 32 values as it is, and one byte of a register for its scale.  The scales come through registers, a
 // row's eight at a time: of one byte each they would be too many fetches, and of four they do not lie on four.
 // That load's wait is the compiler's, which waits for all fetches; it costs an eighth of the time (8192 x 8192 x 8192
 // 293 us, 3.8 PFLOP/s; without scales 256; the matrix cores are busy for 45 % of it, at 8.8 PFLOP/s).
@@ -729,7 +731,8 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides, 2) void mx4_both_kern
   constexpr int kBothRows = 32 * kRows * kRowSides, kBothTokens = 32 * kTokens * kTokenSides;
   constexpr int kWaves = kRowSides * kTokenSides, kThreads = 64 * kWaves;
   constexpr int kWFetches = kBothRows / 16 / kWaves, kXFetches = kBothTokens / 16 / kWaves, kScaleRows = kBothRows + kBothTokens;
-  constexpr int kStepBytes = (kBothRows + kBothTokens) * 64, kScales = 3 * kStepBytes, kScaleBytes = (kBothRows + kBothTokens) * 8;
+  constexpr int kStepBytes = (kBothRows + kBothTokens) * 64, kScales = 3 * kStepBytes,
+                kScaleBytes = (kBothRows + kBothTokens) * 8;
   // three steps of codes, rows first, then tokens: four parts of 16 bytes, part i at i ^ (row / 4 % 4); two
   // pairs of steps of scales, eight bytes a row
   __shared__ u32x4 lds[(kScales + 2 * kScaleBytes) / 16];
@@ -808,12 +811,14 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides, 2) void mx4_both_kern
     for (int r = 0; r < kRows; r++)
 #pragma unroll
       for (int n = 0; n < kTokens; n++)
-        sum[r][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a[0][r]), wide(b[0][n]), sum[r][n], 4, 4, 0, ws[r], 0, xs[n]);
+        sum[r][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a[0][r]), wide(b[0][n]), sum[r][n], 4, 4, 0,
+                                                                    ws[r], 0, xs[n]);
 #pragma unroll
     for (int r = 0; r < kRows; r++)
 #pragma unroll
       for (int n = 0; n < kTokens; n++)
-        sum[r][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a[1][r]), wide(b[1][n]), sum[r][n], 4, 4, 2, ws[r], 2, xs[n]);
+        sum[r][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a[1][r]), wide(b[1][n]), sum[r][n], 4, 4, 2,
+                                                                    ws[r], 2, xs[n]);
     __builtin_amdgcn_sched_barrier(0);
   };
   uint64_t scales = load_scales(0);
@@ -937,7 +942,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_both_few_kernel(const Quan
 #pragma unroll
     for (int i = 0; i < kSides; i++)
 #pragma unroll
-      for (int h = 0; h < 2; h++) next[i][h] = *reinterpret_cast<const u32x4 *>(codes[i >= kRows] + (first[i][h] + block) * kBlockBytes);
+      for (int h = 0; h < 2; h++)
+        next[i][h] = *reinterpret_cast<const u32x4 *>(codes[i >= kRows] + (first[i][h] + block) * kBlockBytes);
 #pragma unroll
     for (int i = 0; i < kSides; i++) {
       const uint8_t *from = scales[i >= kRows] + scale_first[i];
