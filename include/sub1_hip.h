@@ -643,7 +643,8 @@ int sub1_unregister_dec(const int32_t *dec);
  *                                       (8) over the magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6.  16-byte aligned
  *   scales  uint8 [rows, blocks]        the block's scale is 2^(byte - 127); 255: the block is no number
  * Values behind W in the last block have code 0.  Codes and scales may hold anything: no value of theirs is
- * followed as an address.  Any width and height from 1 to SUB1_MX4_MAX_WIDTH.
+ * followed as an address.  What passes fp32's range (2^128 and above: codes of 4 and 6 under a scale of 253, of 2 and more
+ * under 254, which sub1_mx4_quantize does not give) is infinite, but in a product whose both sides are in the format.  Any width and height from 1 to SUB1_MX4_MAX_WIDTH.
  */
 #define SUB1_MX4_BF16 0
 #define SUB1_MX4_FP16 1

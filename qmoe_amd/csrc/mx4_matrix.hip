@@ -181,8 +181,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(const ProductAr
 // The same for rows of a step a wavefront or more: neighbouring lanes read a row's pieces as they lie and hand them
 // round through LDS, a part of the wavefront's own, while the next step's are on their way; the lanes that multiply
 // are rows apart, and their own loads are pieces of 16 bytes, one by one in the L1.  Sums are added up in the same order.  What bounds it: the
-// activations, of which a workgroup reads four times the bytes of its 16 rows, on their way one step ahead (two and
-// three steps ahead measured alike: 13 tokens through 2080 x 6144 8.0 us each, 2 tokens 5.4).
+// activations, of which a workgroup reads four times the bytes of its 16 rows, on their way one step ahead.  (Asked for
+// two and three steps ahead they measured alike, 13 tokens through 2080 x 6144 8.0 us each, 2 tokens 5.4; that says
+// nothing of more on its way: where fetch()'s branches meet, the compiler waits for all loads.)
 template <int kRows, int kTokens>
 __global__ __launch_bounds__(64 * kFewWaves) void mx4_few_lines_kernel(const ProductArgs p) {
   constexpr int kStage = kRows * 64 + kTokens * 256;   // a wavefront's rows of 64 bytes, tokens of 256
@@ -522,10 +523,10 @@ __device__ __forceinline__ void meet() {
 
 // Straight into LDS, three steps of activations and three pairs of steps of codes and scales, each asked for two
 // steps or more ahead: no registers hold what is on its way, and a wavefront's turn is its reads of LDS and its
-// products (a 128 x 128 tile's turn 0.47 us, through registers 0.67; its MFMAs alone take 0.21).  What bounds it
-// with two workgroups a compute unit: LDS and L1 are each busy for more than half of the MFMAs' time, and their
-// wavefronts meet once a step (4096 x 4096 x 4096 124 us, 1.1 PFLOP/s; of 1.3 that a library product in bf16
-// reaches at twice that size).
+// products (a 128 x 128 tile's turn 0.47 us, through registers 0.67; its MFMAs alone take 0.21).  Nothing is busy all
+// the time with two workgroups a compute unit (2272 tokens through 6144 x 2080, by counters: the matrix cores for 39 % of
+// the launch, L1 33, LDS 19, VALU 20): the wavefronts meet once a step, and 864 tiles fill a second round of 512 by
+// two thirds (4096 x 4096 x 4096 121 us, 1.1 PFLOP/s; of 1.4 that a library product in bf16 reaches at twice that size).
 // kParts groups of four wavefronts share a tile's steps, where tiles alone would leave compute units idle.
 template <int kRows, int kTokens, int kParts, int kWaves>
 __global__ __launch_bounds__(256 * kParts, kWaves) void mx4_many_direct_kernel(const ProductArgs p) {
@@ -724,8 +725,11 @@ __device__ __forceinline__ i32x8 wide(u32x4 v) {
 // 32 kTokens tokens, 128 values of a row a step, as mx4_many_direct_kernel fetches them;
 // v_mfma_scale_f32_32x32x64_f8f6f4 takes a lane's block of 32 values as it is, and one byte of a register for its scale.  The scales come through registers, a
 // row's eight at a time: of one byte each they would be too many fetches, and of four they do not lie on four.
-// That load's wait is the compiler's, which waits for all fetches; it costs an eighth of the time (8192 x 8192 x 8192
-// 293 us, 3.8 PFLOP/s; without scales 256; the matrix cores are busy for 45 % of it, at 8.8 PFLOP/s).
+// That load's wait is the compiler's, which knows nothing of the fetches and waits for all of them, every second step; with
+// the scales it costs an eighth of the time (8192 x 8192 x 8192 293 to 302 us, 3.7 of the 8.8 PFLOP/s that the matrix cores
+// reach alone; without scales 256).  At 17 steps a tile, 8192 tokens through 6144 x 2080, the matrix cores are busy for 29 %
+// of the launch, L1 for 35, LDS for 21: a compute unit holds one workgroup, whose first fetches and last stores
+// overlap with nobody's products.
 template <int kRows, int kTokens, int kRowSides, int kTokenSides>
 __global__ __launch_bounds__(64 * kRowSides * kTokenSides, 2) void mx4_both_kernel(const QuantizedArgs p) {
   constexpr int kBothRows = 32 * kRows * kRowSides, kBothTokens = 32 * kTokens * kTokenSides;
@@ -1062,9 +1066,9 @@ void launch_few_lines(const ProductArgs &p, hipStream_t s) {
 // rows enough for two tiles each way (32 through 6144 x 2080 7.4 and 6.6).  Then tiles of 64 x 64, as there are few of
 // them shared by four, two or one group of four wavefronts (70 through 2080 x 6144, 66 tiles: 13.7, 15.7, 20.5; 200
 // through 4096 x 1024, 256 tiles: 5.9, 5.5, 5.9; 568, 576 tiles: 14.3, 10.9, 8.9), and of 128 x 128 from four
-// of the small ones a compute unit on (2272 through 6144 x 2080, 3456 tiles: 72, small ones 94).
+// of the small ones a compute unit on (2272 through 6144 x 2080, 3456 tiles: 65, small ones 90; 1136, 1728: 34 and 47).
 // Activations whose rows do not lie on 16 bytes cannot be fetched into LDS without registers
-// (2272 through 6144 x 2080 86, 568 through 4096 x 1024 13.3), by tiles that no groups share: wavefronts that take rows
+// (2272 through 6144 x 2080 77, 568 through 4096 x 1024 12.3), by tiles that no groups share: wavefronts that take rows
 // then pay to three tiles of 32 x 16 a compute unit (200 through 2080 x 6143, 845: 37 us, through registers 57; 50
 // through 6144 x 2079, 768: 13.4 and 15.3; 100 through 3756 x 1036, 826: 10.0 and 9.5; 400 through 2080 x 6143, 1625:
 // 68 and 58).

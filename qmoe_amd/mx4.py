@@ -237,7 +237,8 @@ class Mx4SparseMLP(nn.Module):
     router_outputs  whether forward returns (hidden, (logits, index)) or hidden alone
 
     Logits are summed in 64 bits and rounded to fp32; of equal ones the expert of the lower index comes
-    first.  Batches of more than 256 tokens run in parts, each of which reads its experts anew."""
+    first.  What goes from an expert's first product to its second is rounded to bf16, as between two layers
+    of a bf16 model.  Batches of more than 256 tokens run in parts, each of which reads its experts anew."""
 
     def __init__(self, router, wi, wo, top_k=1, normalize=False, capacity=None, router_outputs=True):
         super().__init__()
@@ -270,7 +271,8 @@ class Mx4SparseMLP(nn.Module):
     @staticmethod
     def from_mlp(mlp, top_k=1, normalize=False, router_outputs=True):
         """The layer of a `SwitchTransformersSparseMLP`-shaped module on the GPU: `mlp.router` with a
-        linear `classifier` (and `expert_capacity`, taken where there is one), `mlp.experts` (a
+        linear `classifier` (and `expert_capacity`, with one expert a token taken where there is one, for
+        which forward refuses sequences of more than 256 tokens that are longer than it), `mlp.experts` (a
         ModuleDict of modules with dense `wi`/`wo`), whose matrices are rounded to the format."""
         experts = list(mlp.experts.values())
         for expert in experts:
