@@ -51,6 +51,13 @@ def _quick(name, *args):
     return got
 
 
+def _whole(value, name):
+    """value as int, of whatever type of number."""
+    if int(value) != value:
+        raise ValueError('%s must be a whole number, got %r' % (name, value))
+    return int(value)
+
+
 def _blocks(width):
     return (width + BLOCK - 1) // BLOCK
 
@@ -181,6 +188,7 @@ class Mx4Linear(nn.Module):
             raise ValueError('codes must be [height, 16 * blocks], got %s' % (tuple(codes.shape),))
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise TypeError('codes and scales must be torch.uint8')
+        width = _whole(width, 'width')
         blocks = _blocks(width)
         if codes.shape[1] != 16 * blocks or tuple(scales.shape) != (codes.shape[0], blocks):
             raise ValueError('codes must be [H, %d] and scales [H, %d] for a width of %d, got %s and %s' % (
@@ -255,10 +263,12 @@ class Mx4SparseMLP(nn.Module):
                     (name,) + want + (tuple(codes.shape), tuple(scales.shape))))
             if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
                 raise TypeError('%s must be torch.uint8' % name)
+        top_k = _whole(top_k, 'top_k')
         if not 1 <= top_k <= min(experts, _lib.MX4_LAYER_TOP_K):
             raise ValueError('top_k must be 1..%d, got %d' % (min(experts, _lib.MX4_LAYER_TOP_K), top_k))
         if experts > _lib.MX4_LAYER_EXPERTS or max(d_model, d_ff) > _lib.MX4_MAX_WIDTH:
             raise ValueError('at most %d experts of %d' % (_lib.MX4_LAYER_EXPERTS, _lib.MX4_MAX_WIDTH))
+        capacity = None if capacity is None else _whole(capacity, 'capacity')
         if capacity is not None and (top_k != 1 or capacity < 1):
             raise ValueError('a capacity is at least 1 and goes with one expert a token')
         self.experts, self.d_model, self.d_ff = experts, d_model, d_ff

@@ -676,6 +676,23 @@ def test_values_that_torch_keeps_with_the_other_sign():
     against_the_oracle(layer, x, dense_wi, dense_wo)
 
 
+@pytest.mark.parametrize('kind', [int, np.int64, np.int32, float])
+def test_whole_numbers_of_any_type(kind):
+    codes, scales, w = matrix(50, 60, 41)
+    x = activations(5, 60, 42)
+    for quantized in (False, True):
+        layer = mx4.Mx4Linear(codes, scales, kind(60), quantized)
+        assert type(layer.width) is int
+        flat = mo.dequantize(*mo.quantize(host(x)), 60) if quantized else host(x)
+        within(layer(x), *mo.product_bound(flat, w))
+    wi, wo, dense_wi, dense_wo = experts(4, 64, 96, 49)
+    router = torch.randn((4, 64), generator=gen(50)).cuda()
+    hidden = activations(300, 64, 51).view(50, 6, 64)          # in two parts, and in one
+    for some in (hidden, hidden[:2]):
+        against_the_oracle(mx4.Mx4SparseMLP(router, wi, wo, kind(1), False, kind(2)), some, dense_wi, dense_wo)
+        against_the_oracle(mx4.Mx4SparseMLP(router, wi, wo, kind(2)), some, dense_wi, dense_wo)
+
+
 def test_quantised_layers_in_a_row_as_a_block_runs_them():
     """A 4-bit projection, the sparse MLP on its result, a 4-bit projection with 4-bit activations."""
     g = gen(80)

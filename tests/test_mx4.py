@@ -158,6 +158,20 @@ def test_the_sparse_mlp_refuses():
     assert mx4.Mx4SparseMLP(router, wi, wo)._parts(600, 300) == [(0, 256), (256, 256), (512, 88)]
 
 
+def test_numbers_that_are_not_whole_are_refused():
+    codes, scales = torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 2, dtype=torch.uint8)
+    for width in (60, 60.0, np.int64(60), np.float32(60)):
+        assert type(mx4.Mx4Linear(codes, scales, width).width) is int
+    experts = torch.zeros(4, 64, 32, dtype=torch.uint8), torch.zeros(4, 64, 2, dtype=torch.uint8)
+    layer = mx4.Mx4SparseMLP(torch.zeros(4, 64), experts, experts, np.int32(1), capacity=np.int64(3))
+    assert type(layer.top_k) is int and type(layer.capacity) is int
+    with pytest.raises(ValueError, match='width'):
+        mx4.Mx4Linear(codes, scales, 60.5)
+    for wrong in (dict(top_k=1.5), dict(capacity=2.5)):
+        with pytest.raises(ValueError, match=list(wrong)[0]):
+            mx4.Mx4SparseMLP(torch.zeros(4, 64), experts, experts, **wrong)
+
+
 def test_a_module_with_other_experts_is_refused():
     import types
 
