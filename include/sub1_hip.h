@@ -704,6 +704,76 @@ int64_t sub1_mx4_layer_scratch_bytes(const sub1_mx4_layer *layer, int tokens);
 int sub1_mx4_layer_forward(const sub1_mx4_layer *layer, const void *x, int tokens, int length, void *y, float *logits,
                            int64_t *index, void *scratch, int64_t scratch_bytes, void *stream);
 
+/*
+ * Microscaled 8-bit activations (OCP Microscaling Formats 1.0, MXFP8 with e4m3 elements) for the 4-bit matrices
+ * above: blocks as theirs, but 32 bytes of codes each, codes uint8 [rows, 32 * blocks] on 16 bytes, an e4m3 a
+ * byte (no infinities, 0x7f and 0xff are no number); scales uint8 [rows, blocks] as there.  To the format: the
+ * scale is the smallest 2^e, e not below -127, under which a block's largest magnitude is at most 448 (0: 2^-127);
+ * a value becomes the nearest e4m3 times 2^e, of two the even one.  A block that holds an infinity or something that
+ * is no number gets scale 255 and codes 0.  Types, strides and limits as in sub1_mx4_quantize and
+ * sub1_mx4_dequantize; from the format, a value is rounded to `type` (in bf16 exact from 2^-126 on, in fp32 everywhere).
+ *
+ * sub1_mx8_product: r[t, h] = sum_k W[h, k] x[t, k], fp32 sums, W in 4 bits and x in 8; with `relu` those below
+ * zero become zero.  Either to y, bf16 [tokens, height] of row stride ldy (not accumulated into it), or, with y NULL,
+ * to y_codes and y_scales, rounded to 8 bits once, as the next product takes them.  Nothing is kept between calls and
+ * no scratch memory is needed.  Codes and scales may hold anything: no value of theirs is followed as an address.
+ */
+int sub1_mx8_quantize(const void *x, int type, int64_t ldx, int64_t rows, int width, uint8_t *codes, uint8_t *scales,
+                      void *stream);
+int sub1_mx8_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int width, void *out, int type,
+                        int64_t ldo, void *stream);
+int sub1_mx8_product(const uint8_t *codes, const uint8_t *scales, int height, int width, const uint8_t *x_codes,
+                     const uint8_t *x_scales, int relu, void *y, int64_t ldy, uint8_t *y_codes, uint8_t *y_scales, int tokens,
+                     void *stream);
+
+/*
+ * Root-mean-square norm of the rows of x [rows, width], the residual's addition before it:
+ *   s = x + residual, rounded to the residual's type, to `total` (residual and total both NULL: s = x)
+ *   y = s / sqrt(mean(s^2) + eps) * weight
+ * y in x's type, or, with y NULL, in 8 bits as above to codes and scales.  Sums in 64 bits, one rounding of y.
+ * Types SUB1_MX4_BF16, _FP16 or _FP32; residual (and total) and weight each in x's or in _FP32.  Strides in elements.
+ * y may be x and total the residual, of the same strides; otherwise results overlap nothing.  eps is at least
+ * SUB1_NORM_LEAST_EPS.
+ */
+#define SUB1_NORM_MAX_ROWS (1 << 30)
+#define SUB1_NORM_LEAST_EPS 1e-30
+typedef struct sub1_norm {
+  const void *weight;
+  double eps;
+  int32_t width, type, residual_type, weight_type;
+} sub1_norm;
+int sub1_rms_norm(const sub1_norm *norm, const void *x, int64_t ldx, const void *residual, int64_t ldr, void *total, int64_t ldt,
+                  void *y, int64_t ldy, uint8_t *codes, uint8_t *scales, int64_t rows, void *stream);
+
+/*
+ * Which experts a token goes to, from its router's logits [tokens, experts] of `type` and row stride ldl:
+ *   s = softmax(logits), or with SUB1_ROUTE_SIGMOID 1 / (1 + exp(-logits)); c = s + bias (fp32 [experts], or NULL: s)
+ *   of `groups` groups of experts that lie together those top_groups with the largest marks: a mark is the sum of a
+ *   group's group_mark (1 or 2) largest c
+ *   index [t, :] the top_k experts with the largest c in those groups, the largest first
+ *   shares [t, :] = s at those, with `normalize` over their sum (unless that is zero), times scale
+ * What decides is compared in 64 bits, without a bias experts in the order of their logits; of equal ones the
+ * lower index comes first, what is no number last.  A logit of -infinity has the score 0, and a row of nothing
+ * else shares of 0.  `index` holds int32 or int64, by index_bytes.
+ *
+ * sub1_combine: y[t, :] = sum_j shares[t, j] outputs[t, j, :] (+ residual[t, :]), fp32 sums, all of `type` and
+ * contiguous (shares fp32); y may be the residual.
+ */
+#define SUB1_ROUTE_SOFTMAX 0
+#define SUB1_ROUTE_SIGMOID 1
+#define SUB1_ROUTE_MAX_EXPERTS 4096
+#define SUB1_ROUTE_MAX_TOP_K 64
+#define SUB1_ROUTE_MAX_TOKENS (1 << 24)
+typedef struct sub1_router {
+  const float *bias;
+  int32_t experts, top_k, groups, top_groups, group_mark, scores, normalize;
+  float scale;
+} sub1_router;
+int sub1_route(const sub1_router *router, const void *logits, int type, int64_t ldl, int64_t tokens, float *shares, void *index,
+               int index_bytes, void *stream);
+int sub1_combine(const void *outputs, int type, const float *shares, const void *residual, int64_t tokens, int top_k, int width,
+                 void *y, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,13 @@ MX4_LAYER_TOKENS = 256            # SUB1_MX4_LAYER_TOKENS
 MX4_LAYER_TOP_K = 8               # SUB1_MX4_LAYER_TOP_K
 MX4_LAYER_EXPERTS = 4096          # SUB1_MX4_LAYER_EXPERTS
 
+NORM_MAX_ROWS = 1 << 30           # SUB1_NORM_MAX_ROWS
+NORM_LEAST_EPS = 1e-30            # SUB1_NORM_LEAST_EPS
+ROUTE_MAX_EXPERTS = 4096          # SUB1_ROUTE_MAX_EXPERTS
+ROUTE_MAX_TOP_K = 64              # SUB1_ROUTE_MAX_TOP_K
+ROUTE_MAX_TOKENS = 1 << 24        # SUB1_ROUTE_MAX_TOKENS
+ROUTE_MAX_GROUPS = 64             # (a lane each)
+
 _vp = ctypes.c_void_p
 _int = ctypes.c_int
 _i64 = ctypes.c_int64
@@ -75,6 +82,19 @@ class Mx4Layer(ctypes.Structure):
                 ('experts', ctypes.c_int32), ('d_model', ctypes.c_int32), ('d_ff', ctypes.c_int32),
                 ('top_k', ctypes.c_int32), ('router_type', ctypes.c_int32), ('normalize', ctypes.c_int32),
                 ('capacity', ctypes.c_int32)]
+
+
+class Norm(ctypes.Structure):
+    """struct sub1_norm"""
+    _fields_ = [('weight', _vp), ('eps', ctypes.c_double), ('width', ctypes.c_int32), ('type', ctypes.c_int32),
+                ('residual_type', ctypes.c_int32), ('weight_type', ctypes.c_int32)]
+
+
+class Router(ctypes.Structure):
+    """struct sub1_router"""
+    _fields_ = [('bias', _vp), ('experts', ctypes.c_int32), ('top_k', ctypes.c_int32), ('groups', ctypes.c_int32),
+                ('top_groups', ctypes.c_int32), ('group_mark', ctypes.c_int32), ('scores', ctypes.c_int32),
+                ('normalize', ctypes.c_int32), ('scale', ctypes.c_float)]
 
 
 # every symbol include/sub1_hip.h declares, with its prototype
@@ -138,6 +158,12 @@ PROTOTYPES = {
     'sub1_mx4_product_quantized': (_int, [_vp, _vp, _int, _int, _vp, _vp, _vp, _i64, _int, _vp]),
     'sub1_mx4_layer_scratch_bytes': (_i64, [ctypes.POINTER(Mx4Layer), _int]),
     'sub1_mx4_layer_forward': (_int, [ctypes.POINTER(Mx4Layer), _vp, _int, _int, _vp, _vp, _vp, _vp, _i64, _vp]),
+    'sub1_mx8_quantize': (_int, [_vp, _int, _i64, _i64, _int, _vp, _vp, _vp]),
+    'sub1_mx8_dequantize': (_int, [_vp, _vp, _i64, _int, _vp, _int, _i64, _vp]),
+    'sub1_mx8_product': (_int, [_vp, _vp, _int, _int, _vp, _vp, _int, _vp, _i64, _vp, _vp, _int, _vp]),
+    'sub1_rms_norm': (_int, [ctypes.POINTER(Norm), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp]),
+    'sub1_route': (_int, [ctypes.POINTER(Router), _vp, _int, _i64, _i64, _vp, _vp, _int, _vp]),
+    'sub1_combine': (_int, [_vp, _int, _vp, _vp, _i64, _int, _int, _vp, _vp]),
     'sub1_timing_begin': (_int, [_vp]),
     'sub1_timing_end': (_int, [_vp, ctypes.POINTER(ctypes.c_double)]),
     'sub1_init': (_int, []),

@@ -15,6 +15,9 @@ SOURCES = [os.path.join(HERE, 'csrc', 'sub1_kernels.hip'),
            os.path.join(HERE, 'csrc', 'sub1_tiles.hip'),
            os.path.join(HERE, 'csrc', 'mx4_matrix.hip'),
            os.path.join(HERE, 'csrc', 'mx4_layer.hip'),
+           os.path.join(HERE, 'csrc', 'mx8_matrix.hip'),
+           os.path.join(HERE, 'csrc', 'norm.hip'),
+           os.path.join(HERE, 'csrc', 'routing.hip'),
            os.path.join(HERE, 'csrc', 'sub1_tables.cpp')]
 
 HIPCC_FLAGS = [

@@ -69,6 +69,92 @@ __device__ __forceinline__ uint32_t two_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(a), static_cast<__bf16>(b)});
 }
 
+// The type of the values that a kernel reads or writes, as eight of them at once.
+template <class T>
+struct Eight;
+template <>
+struct Eight<__bf16> {
+  u32x4 raw;
+  __device__ __forceinline__ void load(const uint8_t *row, int first, int width) {
+    raw = load8(reinterpret_cast<const uint16_t *>(row), first, width);
+  }
+  __device__ __forceinline__ float at(int i) const {
+    return __uint_as_float(i & 1 ? raw[i / 2] & 0xffff0000u : raw[i / 2] << 16);
+  }
+  static __device__ __forceinline__ void store(uint8_t *row, int first, int width, const float (&v)[8]) {
+    uint16_t *p = reinterpret_cast<uint16_t *>(row) + first;
+    uint32_t two[4];   // exact: a bf16 has room for a code under any scale
+#pragma unroll
+    for (int i = 0; i < 4; i++) two[i] = __float_as_uint(v[2 * i]) >> 16 | (__float_as_uint(v[2 * i + 1]) & 0xffff0000u);
+    if (first + 8 <= width) {
+      __builtin_memcpy(p, two, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (first + i < width) p[i] = static_cast<uint16_t>(two[i / 2] >> (16 * (i & 1)));
+    }
+  }
+};
+template <>
+struct Eight<_Float16> {
+  u32x4 raw;
+  __device__ __forceinline__ void load(const uint8_t *row, int first, int width) {
+    raw = load8(reinterpret_cast<const uint16_t *>(row), first, width);
+  }
+  __device__ __forceinline__ float at(int i) const {
+    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(raw[i / 2] >> (16 * (i & 1)))));
+  }
+  static __device__ __forceinline__ void store(uint8_t *row, int first, int width, const float (&v)[8]) {
+    _Float16 *p = reinterpret_cast<_Float16 *>(row) + first;
+    _Float16 half[8];   // to nearest: large scales leave this type's range, small ones its steps
+#pragma unroll
+    for (int i = 0; i < 8; i++) half[i] = static_cast<_Float16>(v[i]);
+    if (first + 8 <= width) {
+      __builtin_memcpy(p, half, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (first + i < width) p[i] = half[i];
+    }
+  }
+};
+template <>
+struct Eight<float> {
+  float raw[8];
+  __device__ __forceinline__ void load(const uint8_t *row, int first, int width) {
+    const float *p = reinterpret_cast<const float *>(row) + first;
+    if (first + 8 <= width) {
+      __builtin_memcpy(raw, p, 32);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) raw[i] = first + i < width ? p[i] : 0.0f;
+    }
+  }
+  __device__ __forceinline__ float at(int i) const { return raw[i]; }
+  static __device__ __forceinline__ void store(uint8_t *row, int first, int width, const float (&v)[8]) {
+    float *p = reinterpret_cast<float *>(row) + first;
+    if (first + 8 <= width) {
+      __builtin_memcpy(p, v, 32);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (first + i < width) p[i] = v[i];
+    }
+  }
+};
+
+// Four rows of one token's y, from `row` on.
+__device__ __forceinline__ void store_four(uint16_t *y, int row, int height, f32x4 sum) {
+  const uint32_t two[2] = {two_bf16(sum[0], sum[1]), two_bf16(sum[2], sum[3])};
+  if (row + 4 <= height) {
+    __builtin_memcpy(y + row, two, 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (row + i < height) y[row + i] = static_cast<uint16_t>(two[i / 2] >> (16 * (i & 1)));
+  }
+}
+
 // Few tokens: a workgroup of kFewWaves wavefronts multiplies 16 * kRows rows of a matrix with 16 *
 // kTokens tokens.  A step is 128 values of a row, four blocks: lane l holds block l / 16 of row l % 16
 // in one 16-byte load, and the same block of token l % 16, so that the k-th of four v_mfma_f32_16x16x32_bf16
@@ -256,6 +342,50 @@ __device__ __forceinline__ float one_product(OneFirst v, const uint8_t *__restri
     }
   }
   return lanes_sum<kLanes>(sum);
+}
+
+// Over the 64 lanes, in the last of them.
+__device__ __forceinline__ double wave_sum(double v) {
+  auto add = [&](auto control, auto rows) {
+    constexpr int kControl = decltype(control)::value, kMask = decltype(rows)::value;
+    const unsigned long long u = __double_as_longlong(v);
+    const uint32_t low = sub1::dpp_or_zero<kControl, kMask>(static_cast<int>(u));
+    const uint32_t high = sub1::dpp_or_zero<kControl, kMask>(static_cast<int>(u >> 32));
+    v += __longlong_as_double(static_cast<unsigned long long>(high) << 32 | low);
+  };
+  add(std::integral_constant<int, sub1::kDppRowShr1>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, sub1::kDppRowShr2>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, sub1::kDppRowShr4>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, sub1::kDppRowShr8>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, sub1::kDppBcast15>{}, std::integral_constant<int, 0xa>{});
+  add(std::integral_constant<int, sub1::kDppBcast31>{}, std::integral_constant<int, 0xc>{});
+  return v;
+}
+
+typedef __attribute__((address_space(3))) unsigned char *lds_bytes;
+__device__ __forceinline__ uint32_t lds_address(void *p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_bytes)p));
+}
+
+// 16 bytes a lane, or one byte (as 32 bits), from base + at into LDS, the lanes' back to back from `to` on.  The
+// compiler is not told what these are: it would let every read of LDS wait for all that is on its way
+// there, the steps after the next among it.  Their caller counts them, waits and meets the others (meet()).
+__device__ __forceinline__ void fetch(const void *base, uint32_t at, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(at), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void fetch_byte(const void *base, uint32_t at, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(to), "v"(at), "s"(base) : "memory", "m0");
+}
+// Waits until at most kLeft of this wavefront's loads are on their way and it has done with LDS, then for the other
+// wavefronts.
+template <int kLeft>
+__device__ __forceinline__ void meet() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
+}
+
+// sixteen bytes of codes as the scaled MFMAs take an operand of any of their types
+__device__ __forceinline__ i32x8 wide(u32x4 v) {
+  return i32x8{static_cast<int>(v[0]), static_cast<int>(v[1]), static_cast<int>(v[2]), static_cast<int>(v[3]), 0, 0, 0, 0};
 }
 
 }  // namespace mx4

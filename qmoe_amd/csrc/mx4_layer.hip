@@ -50,23 +50,6 @@ __device__ __forceinline__ void load4(const uint16_t *row, int first, int width,
   }
 }
 
-__device__ __forceinline__ double wave_sum(double v) {   // in lane 63
-  auto add = [&](auto control, auto rows) {
-    constexpr int kControl = decltype(control)::value, kMask = decltype(rows)::value;
-    const unsigned long long u = __double_as_longlong(v);
-    const uint32_t low = sub1::dpp_or_zero<kControl, kMask>(static_cast<int>(u));
-    const uint32_t high = sub1::dpp_or_zero<kControl, kMask>(static_cast<int>(u >> 32));
-    v += __longlong_as_double(static_cast<unsigned long long>(high) << 32 | low);
-  };
-  add(std::integral_constant<int, sub1::kDppRowShr1>{}, std::integral_constant<int, 0xf>{});
-  add(std::integral_constant<int, sub1::kDppRowShr2>{}, std::integral_constant<int, 0xf>{});
-  add(std::integral_constant<int, sub1::kDppRowShr4>{}, std::integral_constant<int, 0xf>{});
-  add(std::integral_constant<int, sub1::kDppRowShr8>{}, std::integral_constant<int, 0xf>{});
-  add(std::integral_constant<int, sub1::kDppBcast15>{}, std::integral_constant<int, 0xa>{});
-  add(std::integral_constant<int, sub1::kDppBcast31>{}, std::integral_constant<int, 0xc>{});
-  return v;
-}
-
 // kExperts by kTokens a workgroup, whose four wavefronts share a row's length, 256 values at a time, or (kShare false) a
 // wavefront, where there are enough of them.  Sums in 64 bits, in which the products are exact: which of two close
 // logits is the larger then follows from the values, not from the order of the sum.

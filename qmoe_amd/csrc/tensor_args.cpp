@@ -13,7 +13,8 @@
 //
 // The calls on microscaled 4-bit matrices go all the way here: tensors looked over, results
 // made, the library's entry called (its address comes from the caller, which has the library).
-// Host time of a product 8.7 -> 4.4 us, of a sparse MLP's call 36 -> 18 (14 with three launches).
+// Host time of a product 8.7 -> 4.4 us, of a sparse MLP's call 36 -> 18 (14 with three launches).  So do those on
+// 8-bit activations, the norm's and the routing's.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -170,9 +171,10 @@ bool rows_of(const at::Tensor &x, int64_t *rows, int64_t *width, int64_t *ld) {
   return true;
 }
 
-bool matrix_in_format(const at::Tensor &codes, const at::Tensor &scales, int64_t width, int64_t dims) {
+// (a block's codes have 16 bytes in the 4-bit format, 32 in the 8-bit one)
+bool matrix_in_format(const at::Tensor &codes, const at::Tensor &scales, int64_t width, int64_t dims, int64_t block_bytes = 16) {
   if (codes.scalar_type() != at::kByte || scales.scalar_type() != at::kByte || codes.dim() != dims ||
-      scales.dim() != dims || !codes.is_contiguous() || !scales.is_contiguous() || codes.size(-1) != 16 * blocks_of(width) ||
+      scales.dim() != dims || !codes.is_contiguous() || !scales.is_contiguous() || codes.size(-1) != block_bytes * blocks_of(width) ||
       scales.size(-1) != blocks_of(width) || reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16)
     return false;
   for (int64_t i = 0; i + 1 < dims; i++)
@@ -347,6 +349,215 @@ PyObject *mx4_layer(PyObject *, PyObject *const *args, Py_ssize_t n) {
   }
 }
 
+// ---- 8-bit activations, norm, routing ----
+
+typedef decltype(&sub1_mx8_product) Product8;
+typedef decltype(&sub1_rms_norm) RmsNorm;
+typedef decltype(&sub1_route) Route;
+typedef decltype(&sub1_combine) Combine;
+
+bool truth(PyObject *object, bool *out) {   // True or False themselves
+  *out = object == Py_True;
+  return object == Py_True || object == Py_False;
+}
+
+bool real(PyObject *object, double *out) {
+  if (!PyFloat_CheckExact(object)) return false;
+  *out = PyFloat_AS_DOUBLE(object);
+  return true;
+}
+
+// mx8_quantize(entry, x, device, stream)
+PyObject *mx8_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  void *entry, *stream;
+  int64_t device, rows, width, ld;
+  if (n != 4 || !address(args[0], &entry) || !integer(args[2], &device) || !address(args[3], &stream)) Py_RETURN_NONE;
+  try {
+    const at::Tensor *x = plain(args[1], device);
+    if (!x || type_of(*x) < 0 || !rows_of(*x, &rows, &width, &ld) || rows < 1) Py_RETURN_NONE;
+    at::Tensor codes = like(*x, 32 * blocks_of(width), at::kByte), scales = like(*x, blocks_of(width), at::kByte);
+    const int status = reinterpret_cast<Quantize>(entry)(x->data_ptr(), type_of(*x), ld, rows, static_cast<int>(width),
+                                                         codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), stream);
+    return result(status, {codes, scales});
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// mx8_dequantize(entry, codes, scales, width, dtype, device, stream)
+PyObject *mx8_dequantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  void *entry, *stream;
+  int64_t device, width;
+  if (n != 7 || !address(args[0], &entry) || !integer(args[3], &width) || !THPDtype_Check(args[4]) ||
+      !integer(args[5], &device) || !address(args[6], &stream) || width < 1 || width > SUB1_MX4_MAX_WIDTH)
+    Py_RETURN_NONE;
+  try {
+    const at::Tensor *codes = plain(args[1], device), *scales = plain(args[2], device);
+    if (!codes || !scales || codes->dim() < 1 || !matrix_in_format(*codes, *scales, width, codes->dim(), 32)) Py_RETURN_NONE;
+    const at::ScalarType type = reinterpret_cast<THPDtype *>(args[4])->scalar_type;
+    if (type != at::kBFloat16 && type != at::kHalf && type != at::kFloat) Py_RETURN_NONE;
+    at::Tensor out = like(*codes, width, type);
+    const int status = reinterpret_cast<Dequantize>(entry)(codes->data_ptr<uint8_t>(), scales->data_ptr<uint8_t>(),
+                                                           out.numel() / width, static_cast<int>(width), out.data_ptr(),
+                                                           type_of(out), width, stream);
+    return result(status, {out});
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// mx8_product(entry, x_codes, x_scales, codes, scales, width, relu, quantize, device, stream): y or (codes, scales)
+PyObject *mx8_product(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  void *entry, *stream;
+  int64_t device, width;
+  bool relu, quantize;
+  if (n != 10 || !address(args[0], &entry) || !integer(args[5], &width) || !truth(args[6], &relu) || !truth(args[7], &quantize) ||
+      !integer(args[8], &device) || !address(args[9], &stream) || width < 1 || width > SUB1_MX4_MAX_WIDTH)
+    Py_RETURN_NONE;
+  try {
+    const at::Tensor *t[4];
+    for (int i = 0; i < 4; i++) {
+      t[i] = plain(args[1 + i], device);
+      if (!t[i]) Py_RETURN_NONE;
+    }
+    if (t[0]->dim() < 1 || !matrix_in_format(*t[0], *t[1], width, t[0]->dim(), 32) || !matrix_in_format(*t[2], *t[3], width, 2))
+      Py_RETURN_NONE;
+    const int64_t height = t[2]->size(0), tokens = t[0]->numel() / t[0]->size(-1);
+    if (height > SUB1_MX4_MAX_WIDTH || tokens > SUB1_MX4_MAX_TOKENS) Py_RETURN_NONE;
+    auto call = [&](void *y, uint8_t *codes, uint8_t *scales) {
+      return reinterpret_cast<Product8>(entry)(t[2]->data_ptr<uint8_t>(), t[3]->data_ptr<uint8_t>(), static_cast<int>(height),
+                                               static_cast<int>(width), t[0]->data_ptr<uint8_t>(), t[1]->data_ptr<uint8_t>(), relu,
+                                               y, height, codes, scales, static_cast<int>(tokens), stream);
+    };
+    if (quantize) {
+      at::Tensor codes = like(*t[0], 32 * blocks_of(height), at::kByte), scales = like(*t[0], blocks_of(height), at::kByte);
+      return result(call(nullptr, codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>()), {codes, scales});
+    }
+    at::Tensor y = like(*t[0], height, at::kBFloat16);
+    return result(call(y.data_ptr(), nullptr, nullptr), {y});
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// rms_norm(entry, x, weight, eps, residual or None, quantize, device, stream): y, (y, total), (codes, scales) or
+// ((codes, scales), total)
+PyObject *rms_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  void *entry, *stream;
+  int64_t device, rows, width, ldx, ldr = 0;
+  double eps;
+  bool quantize;
+  if (n != 8 || !address(args[0], &entry) || !real(args[3], &eps) || !truth(args[5], &quantize) || !integer(args[6], &device) ||
+      !address(args[7], &stream) || !(eps >= SUB1_NORM_LEAST_EPS && eps <= 1e30))
+    Py_RETURN_NONE;
+  try {
+    const at::Tensor *x = plain(args[1], device), *weight = plain(args[2], device);
+    if (!x || !weight || type_of(*x) < 0 || !rows_of(*x, &rows, &width, &ldx) || rows < 1 || rows > SUB1_NORM_MAX_ROWS ||
+        weight->dim() != 1 || weight->size(0) != width || !weight->is_contiguous() ||
+        (weight->scalar_type() != x->scalar_type() && weight->scalar_type() != at::kFloat))
+      Py_RETURN_NONE;
+    sub1_norm norm{weight->data_ptr(), eps, static_cast<int32_t>(width), type_of(*x), type_of(*x), type_of(*weight)};
+    const at::Tensor *r = nullptr;
+    at::Tensor total;
+    if (args[4] != Py_None) {
+      int64_t r_rows, r_width;
+      r = plain(args[4], device);
+      if (!r || r->sizes() != x->sizes() || (r->scalar_type() != x->scalar_type() && r->scalar_type() != at::kFloat) ||
+          !rows_of(*r, &r_rows, &r_width, &ldr))
+        Py_RETURN_NONE;
+      norm.residual_type = type_of(*r);
+      total = like(*x, width, r->scalar_type());
+    }
+    at::Tensor y = like(*x, quantize ? 32 * blocks_of(width) : width, quantize ? at::kByte : x->scalar_type()), scales;
+    if (quantize) scales = like(*x, blocks_of(width), at::kByte);
+    const int status = reinterpret_cast<RmsNorm>(entry)(
+        &norm, x->data_ptr(), ldx, r ? r->data_ptr() : nullptr, ldr, r ? total.data_ptr() : nullptr, width,
+        quantize ? nullptr : y.data_ptr(), width, quantize ? y.data_ptr<uint8_t>() : nullptr,
+        quantize ? scales.data_ptr<uint8_t>() : nullptr, rows, stream);
+    if (!r) return quantize ? result(status, {y, scales}) : result(status, {y});
+    if (!quantize || status) return result(status, {y, total});
+    PyObject *first = result(status, {y, scales}), *second = first ? THPVariable_Wrap(total) : nullptr;
+    PyObject *out = second ? PyTuple_Pack(2, first, second) : nullptr;
+    Py_XDECREF(first);
+    Py_XDECREF(second);
+    return out;
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// route(entry, logits, top_k, scores, bias or None, groups, top_groups, group_mark, normalize, scale, dtype, device,
+// stream): (shares, index)
+PyObject *route(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  void *entry, *stream;
+  int64_t top_k, scores, groups, top_groups, group_mark, device, tokens, experts, ld;
+  double scale;
+  bool normalize;
+  if (n != 13 || !address(args[0], &entry) || !integer(args[2], &top_k) || !integer(args[3], &scores) ||
+      !integer(args[5], &groups) || !integer(args[6], &top_groups) || !integer(args[7], &group_mark) ||
+      !truth(args[8], &normalize) || !real(args[9], &scale) || !THPDtype_Check(args[10]) || !integer(args[11], &device) ||
+      !address(args[12], &stream))
+    Py_RETURN_NONE;
+  try {
+    const at::Tensor *logits = plain(args[1], device);
+    const at::ScalarType type = reinterpret_cast<THPDtype *>(args[10])->scalar_type;
+    if (!logits || type_of(*logits) < 0 || !rows_of(*logits, &tokens, &experts, &ld) || tokens < 1 || tokens > SUB1_ROUTE_MAX_TOKENS ||
+        experts > SUB1_ROUTE_MAX_EXPERTS || (type != at::kLong && type != at::kInt) || groups < 1 || groups > experts ||
+        experts % groups || top_groups < 1 || top_groups > groups || group_mark < 1 || group_mark > 2 || top_k < 1 ||
+        top_k > SUB1_ROUTE_MAX_TOP_K || top_k > experts / groups * top_groups || scores < 0 || scores > 1 ||
+        !(scale >= -3.4e38 && scale <= 3.4e38))
+      Py_RETURN_NONE;
+    const at::Tensor *bias = nullptr;
+    if (args[4] != Py_None) {
+      bias = plain(args[4], device);
+      if (!bias || bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != experts || !bias->is_contiguous())
+        Py_RETURN_NONE;
+    }
+    const sub1_router router{bias ? bias->data_ptr<float>() : nullptr, static_cast<int32_t>(experts), static_cast<int32_t>(top_k),
+                             static_cast<int32_t>(groups), static_cast<int32_t>(top_groups), static_cast<int32_t>(group_mark),
+                             static_cast<int32_t>(scores), normalize, static_cast<float>(scale)};
+    at::Tensor shares = like(*logits, top_k, at::kFloat), index = like(*logits, top_k, type);
+    const int status = reinterpret_cast<Route>(entry)(&router, logits->data_ptr(), type_of(*logits), ld, tokens,
+                                                      shares.data_ptr<float>(), index.data_ptr(), type == at::kLong ? 8 : 4, stream);
+    return result(status, {shares, index});
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// combine(entry, outputs, shares, residual or None, device, stream): y
+PyObject *combine(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  void *entry, *stream;
+  int64_t device;
+  if (n != 6 || !address(args[0], &entry) || !integer(args[4], &device) || !address(args[5], &stream)) Py_RETURN_NONE;
+  try {
+    const at::Tensor *outputs = plain(args[1], device), *shares = plain(args[2], device);
+    if (!outputs || !shares || type_of(*outputs) < 0 || outputs->dim() < 2 || !outputs->is_contiguous() ||
+        shares->scalar_type() != at::kFloat || !shares->is_contiguous())
+      Py_RETURN_NONE;
+    const int64_t top_k = outputs->size(-2), width = outputs->size(-1);
+    if (top_k < 1 || top_k > SUB1_ROUTE_MAX_TOP_K || width < 1 || width > SUB1_MX4_MAX_WIDTH) Py_RETURN_NONE;
+    const int64_t tokens = outputs->numel() / (top_k * width);
+    if (tokens < 1 || tokens > SUB1_ROUTE_MAX_TOKENS || shares->sizes() != outputs->sizes().slice(0, outputs->dim() - 1)) Py_RETURN_NONE;
+    auto sizes = outputs->sizes().slice(0, outputs->dim() - 1).vec();
+    sizes.back() = width;
+    const at::Tensor *residual = nullptr;
+    if (args[3] != Py_None) {
+      residual = plain(args[3], device);
+      if (!residual || residual->scalar_type() != outputs->scalar_type() || residual->sizes() != at::IntArrayRef(sizes) ||
+          !residual->is_contiguous())
+        Py_RETURN_NONE;
+    }
+    at::Tensor y = at::empty(sizes, outputs->options());
+    const int status = reinterpret_cast<Combine>(entry)(outputs->data_ptr(), type_of(*outputs), shares->data_ptr<float>(),
+                                                        residual ? residual->data_ptr() : nullptr, tokens, static_cast<int>(top_k),
+                                                        static_cast<int>(width), y.data_ptr(), stream);
+    return result(status, {y});
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
 PyMethodDef kMethods[] = {
     {"addresses", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(addresses)), METH_FASTCALL, nullptr},
     {"layer_addresses", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_addresses)), METH_FASTCALL,
@@ -355,6 +566,12 @@ PyMethodDef kMethods[] = {
     {"mx4_dequantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_dequantize)), METH_FASTCALL, nullptr},
     {"mx4_product", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_product)), METH_FASTCALL, nullptr},
     {"mx4_layer", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_layer)), METH_FASTCALL, nullptr},
+    {"mx8_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx8_quantize)), METH_FASTCALL, nullptr},
+    {"mx8_dequantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx8_dequantize)), METH_FASTCALL, nullptr},
+    {"mx8_product", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx8_product)), METH_FASTCALL, nullptr},
+    {"rms_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rms_norm)), METH_FASTCALL, nullptr},
+    {"route", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(route)), METH_FASTCALL, nullptr},
+    {"combine", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(combine)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_tensor_args", nullptr, -1, kMethods,
                        nullptr,               nullptr,        nullptr, nullptr};
