@@ -1,11 +1,13 @@
 // Activations in microscaled 8 bits: values to the format and back, and their products with matrices
 // in microscaled 4 bits.
 #include "mx8.h"
+#include <cmath>
 
 using namespace mx8;
 using mx4::bf16x2;
 using mx4::bf16x8;
 using mx4::Eight;
+using mx4::f32x16;
 using mx4::f32x4;
 using mx4::FewSums;
 using mx4::i32x8;
@@ -67,6 +69,104 @@ __device__ __forceinline__ float bent(float v, int relu) { return relu && v < 0 
 __device__ __forceinline__ i32x8 operand(u32x4 a, u32x4 b) {
   return i32x8{static_cast<int>(a[0]), static_cast<int>(a[1]), static_cast<int>(a[2]), static_cast<int>(a[3]),
                static_cast<int>(b[0]), static_cast<int>(b[1]), static_cast<int>(b[2]), static_cast<int>(b[3])};
+}
+
+// One token: kLanes lanes, a wavefront or half of one, take a whole row, a block a lane at a time, as mx4_one_kernel does; the token waits in
+// LDS as bf16 (exact: an e4m3 has four bits), its scales beside it.  A block's 32 products are added without scales, then brought to the power of two of
+// both, so that no value leaves a type's range on the way.  For a result in 8 bits a workgroup has the 32 rows of a block.
+constexpr int kOneWaves = mx4::kOneWaves;
+__host__ __device__ constexpr int one_token_bytes(int width) { return mx4::one_lds_bytes(width); }
+__host__ __device__ constexpr int one_lds_bytes(int width) { return one_token_bytes(width) + (blocks_of(width) + 15) / 16 * 16; }
+constexpr int kOneMostBytes = 132 * 1024;
+static_assert(one_lds_bytes(SUB1_MX4_MAX_WIDTH) + 256 <= kOneMostBytes, "every width has room");
+
+template <int kLanes, bool kQuantize>
+__global__ __launch_bounds__(64 * kOneWaves) void mx8_one_kernel(const Product8Args p) {
+  extern __shared__ u32x4 one_lds[];
+  __shared__ float results[32];
+  constexpr int kAtOnce = 64 * kOneWaves / kLanes, kRows = kQuantize ? 32 / kAtOnce : 1;   // rows of a workgroup at a time, of a wavefront's lanes
+  const int lane = threadIdx.x % kLanes, blocks = blocks_of(p.width), row0 = blockIdx.x * kAtOnce * kRows;
+  uint8_t *const x_scales = reinterpret_cast<uint8_t *>(one_lds) + one_token_bytes(p.width);
+  int64_t first[kRows];
+  mx4::OneFirst v[kRows];
+#pragma unroll
+  for (int j = 0; j < kRows; j++) {
+    first[j] = static_cast<int64_t>(min(row0 + j * kAtOnce + static_cast<int>(threadIdx.x / kLanes), p.height - 1)) * blocks;
+    v[j] = mx4::one_block(p.codes, p.scales, first[j], lane, blocks);
+  }
+  const int parts = (blocks + kLanes - 1) / kLanes * kLanes * 4;
+  for (int i = threadIdx.x; i < parts; i += 64 * kOneWaves) {
+    u32x4 eight = {0, 0, 0, 0};
+    if (i < 4 * blocks) {
+      const u32x2 codes = reinterpret_cast<const u32x2 *>(p.x_codes)[i];
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        eight[2 * k] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[k], 1.0f, false));
+        eight[2 * k + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[k], 1.0f, true));
+      }
+    }
+    one_lds[i / (4 * kLanes) * (4 * kLanes) + (i & 3) * kLanes + (i >> 2) % kLanes] = eight;
+  }
+  for (int i = threadIdx.x; i < blocks; i += 64 * kOneWaves) x_scales[i] = p.x_scales[i];
+  __syncthreads();
+  float sum[kRows];
+#pragma unroll
+  for (int j = 0; j < kRows; j++) sum[j] = 0;
+  for (int begin = 0; begin < blocks; begin += kLanes) {
+    const bool there = begin + lane < blocks;   // behind the last block: nothing
+    const uint32_t xs = x_scales[min(begin + lane, blocks - 1)];
+    union {
+      bf16x8 all[4];
+      bf16x2 pair[16];
+    } x;
+#pragma unroll
+    for (int k = 0; k < 4; k++) x.all[k] = __builtin_bit_cast(bf16x8, one_lds[begin * 4 + k * kLanes + lane]);
+#pragma unroll
+    for (int j = 0; j < kRows; j++) {
+      const mx4::OneFirst now = v[j];
+      if (begin + kLanes < blocks) v[j] = mx4::one_block(p.codes, p.scales, first[j], begin + kLanes + lane, blocks);
+      float products = 0;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        union {
+          bf16x8 all;
+          bf16x2 pair[4];
+        } a;
+        a.all = mx4::expand8(now.w[k], 1.0f);
+#pragma unroll
+        for (int i = 0; i < 4; i++) products = __builtin_amdgcn_fdot2_f32_bf16(a.pair[i], x.pair[4 * k + i], products, false);
+      }
+      products = max(now.s, xs) == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(products, static_cast<int>(now.s + xs) - 254);
+      sum[j] += there ? products : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kRows; j++) sum[j] = bent(mx4::lanes_sum<kLanes>(sum[j]), p.relu);
+  if constexpr (!kQuantize) {
+    const int row = row0 + threadIdx.x / kLanes;
+    if (lane == kLanes - 1 && row < p.height) p.y[row] = static_cast<uint16_t>(mx4::two_bf16(sum[0], 0));
+  } else {
+    if (lane == kLanes - 1) {
+#pragma unroll
+      for (int j = 0; j < kRows; j++) results[j * kAtOnce + threadIdx.x / kLanes] = sum[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < 4) {   // eight rows each
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) y[i] = row0 + 8 * static_cast<int>(threadIdx.x) + i < p.height ? results[8 * threadIdx.x + i] : 0.0f;
+      store_block(y, p.y_codes, p.y_scales, static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x, true);
+    }
+  }
+}
+
+template <int kLanes, bool kQuantize>
+int launch_one(const Product8Args &p, hipStream_t s) {
+  constexpr int kRows = kQuantize ? 32 : 64 * kOneWaves / kLanes;
+  if (one_lds_bytes(p.width) + 256 > mx4::kPlainLds) HIP_TRY(sub1::allow_lds<kOneMostBytes>(mx8_one_kernel<kLanes, kQuantize>));
+  mx8_one_kernel<kLanes, kQuantize><<<(p.height + kRows - 1) / kRows, 64 * kOneWaves, one_lds_bytes(p.width), s>>>(p);
+  HIP_TRY(hipGetLastError());
+  return SUB1_OK;
 }
 
 // Few tokens: eight wavefronts a workgroup take eight blocks of its rows and tokens in turn; whole lines are read and the
@@ -229,12 +329,343 @@ void launch_few(const Product8Args &p, hipStream_t s) {
   mx8_few_kernel<kRows, kTokens><<<grid, 64 * kFewWaves, 0, s>>>(p);
 }
 
-int launch_product(const Product8Args &p, hipStream_t s) {
-  sub1::note_kernel("mx8_few_kernel");
-  if (p.tokens <= 16)
-    launch_few<2, 1>(p, s);
+// Many tokens: kRowSides by kTokenSides wavefronts, each with 32 kRows rows of the matrix and 32 kTokens tokens, 128 values
+// of a row a step.  Codes of both sides go straight into LDS, kStages steps of them; nothing but a wavefront's operands and sums is in
+// registers, so that three or four wavefronts a SIMD fit, one's reads of LDS under the others' products.  kParts groups of such wavefronts share a
+// tile's steps, where tiles alone would leave compute units idle.  v_mfma_scale_f32_32x32x64_f8f6f4 takes lane l's
+// block l / 32 of row l % 32 as it is, of token l % 32 the 16 values from 16 (l / 32) on and the 16 from 32 + 16 (l / 32) on, and each
+// side's scale for block l / 32 as one byte of a register.  Scales come through registers, sixteen (four steps') of a row or token a
+// thread, and LDS: loaded by each wavefront for itself they were two of three requests to L2, which bound the launch.
+template <int kRows, int kTokens, int kRowSides, int kTokenSides, int kParts, int kStages>
+struct Many8 {
+  static constexpr int waves = kRowSides * kTokenSides, rows = 32 * kRows * kRowSides, tokens = 32 * kTokens * kTokenSides;
+  static constexpr int w_bytes = rows * 64, step_bytes = w_bytes + tokens * 128;
+  static constexpr int scale_rows = rows + tokens, scales_at = kStages * step_bytes, part_bytes = scales_at + 2 * 16 * scale_rows;
+  static constexpr int group = kRows % 4 == 0 ? 4 : kRows % 3 == 0 ? 3 : kRows;   // tiles of 32 rows that go to y at once
+  static constexpr int pitch = 32 * group + 8;                                    // bf16, of a token's rows on their way
+  static constexpr int lds_bytes = kParts * part_bytes;
+  static_assert(32 * pitch * 2 * waves <= lds_bytes && rows * tokens * 4 * (kParts > 1) <= lds_bytes && lds_bytes <= 160 * 1024, "what a compute unit has");
+};
+
+// The tile that a workgroup takes.  Workgroups go to the eight XCDs in turn, and those of one get tiles that lie together: groups of four
+// tiles of tokens by all rows, the group's tokens first, so that what an XCD's compute units work on at a time is about eight by four
+// tiles, whose codes its L2 reads once.
+struct TilePlace {
+  int row, token;
+};
+__device__ __forceinline__ TilePlace tile_of_workgroup(int id, int row_tiles, int token_tiles) {
+  const int tiles = row_tiles * token_tiles, xcd = id & 7, each = tiles >> 3, more = tiles & 7;
+  const int tile = xcd * each + min(xcd, more) + (id >> 3);
+  const int group = tile / (4 * row_tiles), in_group = tile - group * 4 * row_tiles, wide = min(4, token_tiles - 4 * group);
+  return {in_group / wide, 4 * group + in_group % wide};
+}
+
+template <int kRows, int kTokens, int kRowSides, int kTokenSides, int kParts, int kStages, bool kQuantize>
+__global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * kTokenSides * kParts >= 16 ? 4 : 3) void mx8_many_kernel(const Product8Args p) {
+  using M = Many8<kRows, kTokens, kRowSides, kTokenSides, kParts, kStages>;
+  constexpr int kWaves = M::waves;
+  constexpr int kWAll = M::rows / 16, kXAll = M::tokens / 8;   // fetches of a step: 16 rows' 64 bytes or 8 tokens' 128
+  constexpr int kWFetches = (kWAll + kWaves - 1) / kWaves, kXFetches = (kXAll + kWaves - 1) / kWaves;
+  __shared__ u32x4 all_lds[M::lds_bytes / 16];
+  const int lane = threadIdx.x & 63, part = kParts == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * kWaves));
+  const int tid = threadIdx.x - part * 64 * kWaves, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5, in_tile = lane & 31, row_side = wave % kRowSides, token_side = wave / kRowSides;
+  u32x4 *const lds = all_lds + part * (M::part_bytes / 16);
+  const int row_tiles = (p.height + M::rows - 1) / M::rows;
+  const TilePlace place = tile_of_workgroup(blockIdx.x, row_tiles, (p.tokens + M::tokens - 1) / M::tokens);
+  const int row0 = place.row * M::rows, token0 = place.token * M::tokens;
+  const int blocks = blocks_of(p.width), steps = (blocks + 3) / 4;
+  // the part's steps: as many turns for each part; those behind the last step have scales of nothing
+  const int turns = (steps + kParts - 1) / kParts, first_step = part * turns;
+  const uint8_t *code_tile = p.codes + static_cast<int64_t>(row0) * blocks * kBlockBytes;
+  const uint8_t *x_tile = p.x_codes + static_cast<int64_t>(token0) * blocks * kBlock;
+  const int last_row = p.height - 1 - row0, last_token = p.tokens - 1 - token0;
+  const uint32_t lds_at = mx4::lds_address(lds);
+
+  // What this lane fetches of a step (fetches that are left over repeat the last): rows' four parts of 16 bytes, part i at
+  // i ^ (row / 4 % 4), and tokens' eight, part i at i ^ (token / 2 % 8).  From a step to the next only the base moves, but for the
+  // last, where blocks that are not there repeat the last one.
+  uint32_t w_at[kWFetches], x_at[kXFetches];
+  int x_part[kXFetches];
+  const int w_part = (lane & 3) ^ (lane >> 4);
+#pragma unroll
+  for (int i = 0; i < kWFetches; i++)
+    w_at[i] = (min(min(i * kWaves + wave, kWAll - 1) * 16 + (lane >> 2), last_row) * blocks + w_part) * kBlockBytes;
+#pragma unroll
+  for (int i = 0; i < kXFetches; i++) {
+    const int which = kXAll % kWaves ? min(i * kWaves + wave, kXAll - 1) : i * kWaves + wave;
+    x_part[i] = (lane & 7) ^ (4 * ((kWaves % 2 || kXAll % kWaves ? which : wave) & 1) + (lane >> 4));
+    x_at[i] = min(which * 8 + (lane >> 3), last_token) * blocks * kBlock + x_part[i] * 16;
+  }
+  auto fetch_step = [&](int side, int turn) {
+    const uint32_t to = lds_at + side * M::step_bytes;
+    const int step = min(first_step + turn, steps - 1), last = blocks - 1 - 4 * step;
+    const uint8_t *w_from = code_tile + step * 64, *x_from = x_tile + step * 128;
+#pragma unroll
+    for (int i = 0; i < kWFetches; i++)
+      mx4::fetch(w_from, w_at[i] - max(w_part - last, 0) * kBlockBytes, to + min(i * kWaves + wave, kWAll - 1) * 1024);
+#pragma unroll
+    for (int i = 0; i < kXFetches; i++)
+      mx4::fetch(x_from, x_at[i] - max((x_part[i] >> 1) - last, 0) * kBlock, to + M::w_bytes + min(i * kWaves + wave, kXAll - 1) * 1024);
+  };
+  // This thread's rows' or tokens' scales of the sixteen blocks of four turns, as two eights, each from its first block on or the row's
+  // last eight (the caller's rows have as many); what is left over repeats the last.
+  constexpr int kScaleRows = (M::scale_rows + 64 * kWaves - 1) / (64 * kWaves);
+  uint64_t scales[kScaleRows][2];
+  auto load_scales = [&](int turn) {
+    const int first = 4 * (first_step + turn);
+#pragma unroll
+    for (int j = 0; j < kScaleRows; j++) {
+      const int row = min(j * 64 * kWaves + tid, M::scale_rows - 1);
+      const uint8_t *from = row < M::rows ? p.scales + static_cast<int64_t>(min(row0 + row, p.height - 1)) * blocks
+                                          : p.x_scales + static_cast<int64_t>(min(token0 + row - M::rows, p.tokens - 1)) * blocks;
+#pragma unroll
+      for (int i = 0; i < 2; i++) __builtin_memcpy(&scales[j][i], from + min(first + 8 * i, blocks - 8), 8);
+    }
+  };
+  uint32_t *const scale_lds = reinterpret_cast<uint32_t *>(lds) + M::scales_at / 4;
+  auto put_scales = [&](int turn) {   // zeros behind the row's last; of four turns, each turn's rows back to back
+    const int first = 4 * (first_step + turn);
+#pragma unroll
+    for (int j = 0; j < kScaleRows; j++) {
+      uint32_t *to = scale_lds + (turn & 4) * M::scale_rows + min(j * 64 * kWaves + tid, M::scale_rows - 1);
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int behind = max(first + 8 * i + 8 - blocks, 0);
+        const uint64_t v = behind < 8 ? scales[j][i] >> 8 * behind : 0;
+        to[2 * i * M::scale_rows] = static_cast<uint32_t>(v);
+        to[(2 * i + 1) * M::scale_rows] = static_cast<uint32_t>(v >> 32);
+      }
+    }
+  };
+
+  f32x16 sum[kRows][kTokens];
+#pragma unroll
+  for (int r = 0; r < kRows; r++)
+#pragma unroll
+    for (int n = 0; n < kTokens; n++) sum[r][n] = f32x16{0};
+
+  const u32x4 *w_mine = lds + (row_side * kRows * 32 + in_tile) * 4, *x_mine = lds + M::w_bytes / 16 + (token_side * kTokens * 32 + in_tile) * 8;
+  int as[kRows], bs[kTokens];   // a step's scales of this half's blocks: bytes 0 and 2
+  auto multiply = [&](int side, auto which) {   // a step's first or second 64 values
+    constexpr int k = decltype(which)::value;
+    const u32x4 *w = w_mine + side * (M::step_bytes / 16), *x = x_mine + side * (M::step_bytes / 16);
+    u32x4 a[kRows];
+    i32x8 b[kTokens];
+#pragma unroll
+    for (int r = 0; r < kRows; r++) a[r] = w[r * 128 + ((2 * k + half) ^ (in_tile >> 2 & 3))];
+#pragma unroll
+    for (int n = 0; n < kTokens; n++)
+      b[n] = operand(x[n * 256 + ((4 * k + half) ^ (in_tile >> 1 & 7))], x[n * 256 + ((4 * k + 2 + half) ^ (in_tile >> 1 & 7))]);
+#pragma unroll
+    for (int r = 0; r < kRows; r++)
+#pragma unroll
+      for (int n = 0; n < kTokens; n++)
+        sum[r][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4::wide(a[r]), b[n], sum[r][n], 4, 0, 2 * k, as[r], 2 * k, bs[n]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // Turn t finds its codes there, asks for those of turn t + kStages - 1, whose place was read in the turn before, and multiplies.  The third of
+  // four turns puts the next four's scales where those of the four before were.
+  int side = 0, ahead = kStages - 1;
+  auto turn = [&](auto in_four, int t) {
+    mx4::meet<(kStages - 2) * (kWFetches + kXFetches)>();   // but for the codes that later turns asked for
+    if (decltype(in_four)::value == 2) {
+      put_scales(t + 2);
+      load_scales(t + 6);
+    }
+    fetch_step(ahead, t + kStages - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    const uint32_t *from = scale_lds + (t & 7) * M::scale_rows + in_tile;
+#pragma unroll
+    for (int r = 0; r < kRows; r++) as[r] = static_cast<int>(from[(row_side * kRows + r) * 32] >> (8 * half));
+#pragma unroll
+    for (int n = 0; n < kTokens; n++) bs[n] = static_cast<int>(from[M::rows + (token_side * kTokens + n) * 32] >> (8 * half));
+    multiply(side, std::integral_constant<int, 0>{});
+    multiply(side, std::integral_constant<int, 1>{});
+    side = side == kStages - 1 ? 0 : side + 1;
+    ahead = ahead == kStages - 1 ? 0 : ahead + 1;
+  };
+  load_scales(0);
+  put_scales(0);
+  load_scales(4);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; i++) fetch_step(i, i);
+  int t = 0;
+  for (;;) {
+    turn(std::integral_constant<int, 0>{}, t);
+    if (++t == turns) break;
+    turn(std::integral_constant<int, 1>{}, t);
+    if (++t == turns) break;
+    turn(std::integral_constant<int, 2>{}, t);
+    if (++t == turns) break;
+    turn(std::integral_constant<int, 3>{}, t);
+    if (++t == turns) break;
+  }
+  mx4::meet<0>();   // nothing is on its way into LDS any more, and nobody reads it
+  if constexpr (kParts > 1) {   // the parts' sums, added in their order
+    f32x4 *const place_of = reinterpret_cast<f32x4 *>(all_lds) + tid;
+    constexpr int kFours = 4 * kRows * kTokens;
+    for (int other = 1; other < kParts; other++) {
+      if (part == other) {
+#pragma unroll
+        for (int i = 0; i < kFours; i++) {
+          const f32x16 &v = sum[i / 4 / kTokens][i / 4 % kTokens];
+          place_of[i * 64 * kWaves] = f32x4{v[i % 4 * 4], v[i % 4 * 4 + 1], v[i % 4 * 4 + 2], v[i % 4 * 4 + 3]};
+        }
+      }
+      __syncthreads();
+      if (part == 0) {
+#pragma unroll
+        for (int i = 0; i < kFours; i++) {
+          const f32x4 v = place_of[i * 64 * kWaves];
+#pragma unroll
+          for (int k = 0; k < 4; k++) sum[i / 4 / kTokens][i / 4 % kTokens][i % 4 * 4 + k] += v[k];
+        }
+      }
+      __syncthreads();
+    }
+    if (part) return;
+  }
+
+  const int first_row = row0 + row_side * kRows * 32, first_token = token0 + token_side * kTokens * 32;
+  if (p.relu) {
+#pragma unroll
+    for (int r = 0; r < kRows; r++)
+#pragma unroll
+      for (int n = 0; n < kTokens; n++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) sum[r][n][i] = bent(sum[r][n][i], 1);
+  }
+  if constexpr (!kQuantize) {   // to y past LDS, a part of the wavefront's own, so that whole lines are written
+    uint16_t *const out = reinterpret_cast<uint16_t *>(all_lds) + wave * 32 * M::pitch;
+    constexpr int kPieces = 4 * M::group;   // of eight rows, of a token
+#pragma unroll
+    for (int n = 0; n < kTokens; n++)
+#pragma unroll
+      for (int g = 0; g < kRows; g += M::group) {
+#pragma unroll
+        for (int r = 0; r < M::group; r++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const f32x16 &v = sum[g + r][n];
+            const uint32_t two[2] = {mx4::two_bf16(v[4 * i], v[4 * i + 1]), mx4::two_bf16(v[4 * i + 2], v[4 * i + 3])};
+            __builtin_memcpy(__builtin_assume_aligned(out + in_tile * M::pitch + 32 * r + 8 * i + 4 * half, 8), two, 8);
+          }
+        sub1::wave_lds_fence();
+#pragma unroll
+        for (int i = 0; i < 32 * kPieces / 64; i++) {
+          const int piece = 64 * i + lane, token = first_token + 32 * n + piece / kPieces, row = first_row + 32 * g + piece % kPieces * 8;
+          if (token >= p.tokens) continue;
+          const uint16_t *from = out + piece / kPieces * M::pitch + piece % kPieces * 8;
+          uint16_t *to = p.y + token * p.ldy + row;
+          if (row + 8 <= p.height) {
+            u32x4 v;
+            __builtin_memcpy(&v, __builtin_assume_aligned(from, 16), 16);
+            __builtin_memcpy(to, &v, 16);
+          } else {
+            for (int k = 0; row + k < p.height; k++) to[k] = from[k];
+          }
+        }
+        sub1::wave_lds_fence();
+      }
+  } else {
+    // a token's 32 rows of a tile are a block, which lanes l and l + 32 hold: fours of rows in turn, which two swaps of half
+    // wavefronts bring to sixteen and sixteen in order
+    const int y_blocks = blocks_of(p.height);
+#pragma unroll
+    for (int n = 0; n < kTokens; n++) {
+      const int token = first_token + 32 * n + in_tile;
+#pragma unroll
+      for (int r = 0; r < kRows; r++) {
+        const int left = p.height - first_row - 32 * r;
+        uint32_t largest = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          if (8 * (i / 4) + 4 * half + i % 4 >= left) sum[r][n][i] = 0;
+          largest = max(largest, __float_as_uint(sum[r][n][i]) & 0x7fffffffu);
+        }
+        largest = max(largest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(largest), 32)));
+        const uint32_t byte = scale_byte(largest);
+        u32x2 c[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; k++) v[k] = sum[r][n][8 * i + k];
+          c[i] = pack8(v, byte);
+        }
+        const auto one = __builtin_amdgcn_permlane32_swap(c[0][0], c[1][0], false, false);
+        const auto two = __builtin_amdgcn_permlane32_swap(c[0][1], c[1][1], false, false);
+        if (left > 0 && token < p.tokens) {
+          const int64_t block = static_cast<int64_t>(token) * y_blocks + first_row / 32 + r;
+          *reinterpret_cast<u32x4 *>(p.y_codes + block * kBlock + 16 * half) = u32x4{one[0], one[1], two[0], two[1]};
+          if (half == 0) p.y_scales[block] = static_cast<uint8_t>(byte);
+        }
+      }
+    }
+  }
+}
+
+template <int kRows, int kTokens, int kRowSides, int kTokenSides, int kParts, int kStages>
+void launch_many(const Product8Args &p, hipStream_t s) {
+  using M = Many8<kRows, kTokens, kRowSides, kTokenSides, kParts, kStages>;
+  const unsigned tiles = static_cast<unsigned>((p.height + M::rows - 1) / M::rows * ((p.tokens + M::tokens - 1) / M::tokens));
+  if (p.y_codes)
+    mx8_many_kernel<kRows, kTokens, kRowSides, kTokenSides, kParts, kStages, true><<<tiles, 64 * M::waves * kParts, 0, s>>>(p);
   else
-    launch_few<2, 2>(p, s);
+    mx8_many_kernel<kRows, kTokens, kRowSides, kTokenSides, kParts, kStages, false><<<tiles, 64 * M::waves * kParts, 0, s>>>(p);
+}
+
+// Which kernel, for more tokens than one: that with the shortest estimate.  A form's tiles run `at_once` to a compute unit; a turn of its steps takes
+// `turn` where one tile or fewer is on each, and `busy` for every tile where there are more (it is then shared); what does not depend on the row's
+// length is `start` a launch and `more` a full round of the compute units.  In us, fitted to graphs of calls of 17 to 8192 tokens through 2080 x 6144,
+// 6144 x 2080, 1024 x 4096, 4096 x 1024, 3001 x 1023, 768 x 2500 and 1500 x 1500, to 6 to 14 % each; of those 126 the form with
+// the shortest estimate took 1.2 % longer than the best on average, 28 % at most.
+struct Form {
+  int rows, tokens, parts, at_once;   // few: parts are wavefronts, of 256 values a turn
+  float start, turn, busy, more;
+  void (*launch)(const Product8Args &, hipStream_t);
+};
+constexpr int kForms = 13, kFewForms = 3;
+const Form kForm[kForms] = {
+    {16, 16, 8, 3, 2.6f, 0.82f, 0.70f, 0.0f, launch_few<1, 1>},   // (not for a result in 8 bits: half a block)
+    {32, 16, 8, 2, 2.6f, 1.13f, 0.95f, 0.0f, launch_few<2, 1>},
+    {32, 32, 8, 1, 2.4f, 0.56f, 1.75f, 0.4f, launch_few<2, 2>},
+    {64, 32, 4, 1, 3.8f, 0.21f, 0.57f, 2.3f, launch_many<1, 1, 2, 1, 4, 4>},
+    {64, 64, 2, 2, 3.5f, 0.22f, 0.42f, 2.0f, launch_many<1, 1, 2, 2, 2, 3>},
+    {64, 64, 1, 3, 3.3f, 0.23f, 0.22f, 1.2f, launch_many<1, 1, 2, 2, 1, 4>},
+    {128, 64, 2, 1, 4.0f, 0.03f, 0.59f, 3.0f, launch_many<2, 1, 2, 2, 2, 3>},
+    {128, 64, 1, 2, 3.8f, 0.35f, 0.33f, 1.6f, launch_many<2, 1, 2, 2, 1, 3>},
+    {128, 128, 2, 1, 4.8f, 0.86f, 0.89f, 4.2f, launch_many<2, 2, 2, 2, 2, 2>},
+    {128, 128, 1, 2, 4.7f, 0.36f, 0.50f, 2.6f, launch_many<2, 2, 2, 2, 1, 3>},
+    {256, 128, 1, 2, 4.9f, 0.63f, 0.76f, 5.4f, launch_many<2, 2, 4, 2, 1, 2>},
+    {256, 256, 1, 1, 6.9f, 1.14f, 1.19f, 8.1f, launch_many<2, 2, 4, 4, 1, 2>},
+    {288, 256, 1, 1, 8.2f, 0.95f, 1.31f, 12.6f, launch_many<3, 2, 3, 4, 1, 2>},
+};
+constexpr int kUnits = 256;   // compute units
+
+int launch_product(const Product8Args &p, hipStream_t s) {
+  const int blocks = blocks_of(p.width);
+  if (p.tokens == 1) {
+    sub1::note_kernel("mx8_one_kernel");
+    const bool halves = mx4::halves_pay(p.width, p.height);
+    if (p.y_codes) return halves ? launch_one<32, true>(p, s) : launch_one<64, true>(p, s);
+    return halves ? launch_one<32, false>(p, s) : launch_one<64, false>(p, s);
+  }
+  int best = -1;
+  float shortest = 0;
+  for (int i = 0; i < kForms; i++) {
+    const Form &f = kForm[i];
+    const bool few = i < kFewForms;
+    if ((p.y_codes && f.rows < 32) || (!few && blocks < 8)) continue;   // (through LDS: whole eights of scales)
+    const int64_t tiles = static_cast<int64_t>((p.height + f.rows - 1) / f.rows) * ((p.tokens + f.tokens - 1) / f.tokens);
+    const int64_t rounds = tiles / (kUnits * f.at_once), left = (tiles - rounds * kUnits * f.at_once + kUnits - 1) / kUnits;
+    const int steps = few ? (blocks + 7) / 8 : (blocks + 3) / 4, turns = (steps + f.parts - 1) / f.parts;
+    const float time = f.start + rounds * (f.more + turns * fmaxf(f.turn, f.busy * f.at_once)) + (left ? turns * fmaxf(f.turn, f.busy * left) : 0.0f);
+    if (best < 0 || time < shortest) best = i, shortest = time;
+  }
+  sub1::note_kernel(best < kFewForms ? "mx8_few_kernel" : "mx8_many_kernel");
+  kForm[best].launch(p, s);
   HIP_TRY(hipGetLastError());
   return SUB1_OK;
 }
