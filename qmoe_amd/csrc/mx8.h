@@ -18,11 +18,54 @@ using mx4::u32x4;
 
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 
-// quad_perm of DPP: a lane's neighbour, and the lane two further
-constexpr int kDppSwap1 = 0xb1, kDppSwap2 = 0x4e;
+// DPP: a lane's neighbour and the lane two further (quad_perm), halves of a row of 16 and rows backwards
+constexpr int kDppSwap1 = 0xb1, kDppSwap2 = 0x4e, kDppHalfMirror = 0x141, kDppMirror = 0x140;
 template <int kCtrl>
 __device__ __forceinline__ uint32_t of_lane(uint32_t v) {
   return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, 0xf, 0xf, true));
+}
+
+// The op of v over kLanes lanes that lie together (16 or 64), in all of them.
+template <int kLanes, class Op>
+__device__ __forceinline__ uint32_t over_lanes(uint32_t v, Op op) {
+  v = op(v, of_lane<kDppSwap1>(v));
+  v = op(v, of_lane<kDppSwap2>(v));
+  v = op(v, of_lane<kDppHalfMirror>(v));
+  v = op(v, of_lane<kDppMirror>(v));
+  if constexpr (kLanes == 64) {
+    const auto rows = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op(rows[0], rows[1]);
+    const auto halves = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = op(halves[0], halves[1]);
+  }
+  return v;
+}
+
+__device__ __forceinline__ double double_of(uint32_t high, uint32_t low) {
+  return __longlong_as_double(static_cast<unsigned long long>(high) << 32 | low);
+}
+// Sums over kLanes lanes, in all of them, the same bits in each.
+template <int kLanes>
+__device__ __forceinline__ double sum_over(double v) {
+  auto add = [&](auto control) {
+    const unsigned long long u = __double_as_longlong(v);
+    v += double_of(of_lane<decltype(control)::value>(static_cast<uint32_t>(u >> 32)), of_lane<decltype(control)::value>(static_cast<uint32_t>(u)));
+  };
+  add(std::integral_constant<int, kDppSwap1>{});
+  add(std::integral_constant<int, kDppSwap2>{});
+  add(std::integral_constant<int, kDppHalfMirror>{});
+  add(std::integral_constant<int, kDppMirror>{});
+  if constexpr (kLanes == 64) {
+    unsigned long long u = __double_as_longlong(v);
+    auto high = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(u >> 32), static_cast<uint32_t>(u >> 32), false, false);
+    auto low = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(u), static_cast<uint32_t>(u), false, false);
+    v = double_of(high[0], low[0]) + double_of(high[1], low[1]);
+    u = __double_as_longlong(v);
+    high = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(u >> 32), static_cast<uint32_t>(u >> 32), false, false);
+    low = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(u), static_cast<uint32_t>(u), false, false);
+    v = double_of(high[0], low[0]) + double_of(high[1], low[1]);
+  }
+  return v;
 }
 
 __device__ __forceinline__ uint32_t largest_of(const float (&v)[8]) {

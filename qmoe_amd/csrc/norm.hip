@@ -37,15 +37,16 @@ __device__ __forceinline__ Factor factor_of(const NormArgs &a, double sum) {
 
 // A row's values stay in registers, kPer eights a thread: one read of x and r, one write of s and y.  The sum of squares is held
 // in 64 bits: no square of an fp32 value overflows there and the order of the sum does not count; the vector
-// units add and multiply 64 bits as fast as 32.  kWave: a wavefront a row, four rows a workgroup, nothing waits for another
-// wavefront; else a workgroup a row.
-template <class T, class R, bool kResidual, bool kWave, int kPer>
-__global__ __launch_bounds__(kWave ? 256 : 1024) void rms_norm_kernel(const NormArgs a) {
+// units add and multiply 64 bits as fast as 32.  kLanes: 16 or 64 lanes a row, where nothing waits for another wavefront; 0: a workgroup a row.
+template <class T, class R, bool kResidual, int kLanes, int kPer>
+__global__ __launch_bounds__(kLanes ? 256 : 1024) void rms_norm_kernel(const NormArgs a) {
   __shared__ double parts[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = kWave ? blockIdx.x * int64_t{4} + wave : blockIdx.x;
-  if (kWave && row >= a.rows) return;
-  const int me = kWave ? lane : static_cast<int>(threadIdx.x), lanes = kWave ? 64 : static_cast<int>(blockDim.x);
+  constexpr int kRows = kLanes ? 256 / kLanes : 1;
+  const int64_t mine = kLanes ? blockIdx.x * int64_t{kRows} + threadIdx.x / (kLanes ? kLanes : 1) : blockIdx.x;
+  if (kLanes != 0 && mine - lane / (kLanes ? kLanes : 1) >= a.rows) return;   // (a whole wavefront)
+  const int64_t row = kLanes == 16 && mine >= a.rows ? a.rows - 1 : mine;     // what is not there repeats the wavefront's last row
+  const int me = kLanes ? threadIdx.x % (kLanes ? kLanes : 1) : threadIdx.x, lanes = kLanes ? kLanes : static_cast<int>(blockDim.x);
   float v[kPer][8], w[kPer][8];
   {
     const uint8_t *from = a.x + row * a.x_bytes, *other = a.residual + row * a.residual_bytes;
@@ -92,12 +93,10 @@ __global__ __launch_bounds__(kWave ? 256 : 1024) void rms_norm_kernel(const Norm
   for (int i = 0; i < kPer; i++)
 #pragma unroll
     for (int k = 0; k < 8; k++) sum = fma(static_cast<double>(v[i][k]), static_cast<double>(v[i][k]), sum);
-  sum = mx4::wave_sum(sum);
-  if (kWave) {
-    const unsigned long long u = __double_as_longlong(sum);
-    sum = __longlong_as_double(static_cast<unsigned long long>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u >> 32), 63))) << 32 |
-                               static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u), 63)));
+  if constexpr (kLanes != 0) {
+    sum = sum_over<kLanes>(sum);
   } else {
+    sum = mx4::wave_sum(sum);
     if (lane == 63) parts[wave] = sum;
     __syncthreads();
     sum = 0;
@@ -174,26 +173,44 @@ __global__ __launch_bounds__(1024) void rms_norm_wide_kernel(const NormArgs a) {
   }
 }
 
+template <class T, class R, bool kResidual, int kLanes, int kPer>
+void launch_lanes(const NormArgs &a, hipStream_t s) {
+  constexpr int kRows = 256 / kLanes;
+  rms_norm_kernel<T, R, kResidual, kLanes, kPer><<<static_cast<unsigned>((a.rows + kRows - 1) / kRows), 256, 0, s>>>(a);
+}
+
+// Which form (us, in a graph).  Few rows: a workgroup each, an eight a thread as far as 1024 threads go (1000 x 2080, residual, to 8 bits 6.1, by a wavefront
+// each 7.2; 4000 14.2 and 15.3), and rows of fp32 that a wavefront's registers hold barely (4096 x 4096, residual 43 and 50).  Many: a
+// wavefront each (16384 x 2080 48 and 53; without residual 26 and 36).  Many narrow ones: a quarter of one (16384 x 100 5.8 and
+// 11, 16000 x 300 11.3 and 12.8; 1000 x 300 by a workgroup each 3.9, by quarters 4.7).
 template <class T, class R, bool kResidual>
 int launch_rows(const NormArgs &a, hipStream_t s) {
   const int eights = blocks_of(a.width) * 4;
-  if (eights <= 64 * 8 && a.rows > 512) {
+  const bool in_fp32 = sizeof(T) == 4 || (kResidual && sizeof(R) == 4);
+  if (eights <= 64 && a.rows > 2048) {
+    sub1::note_kernel("rms_norm_kernel, 16 lanes a row");
+    if (eights <= 16) launch_lanes<T, R, kResidual, 16, 1>(a, s);
+    else if (eights <= 32) launch_lanes<T, R, kResidual, 16, 2>(a, s);
+    else if (eights <= 48) launch_lanes<T, R, kResidual, 16, 3>(a, s);
+    else launch_lanes<T, R, kResidual, 16, 4>(a, s);
+  } else if (a.rows > 4096 && eights <= (in_fp32 ? 4 : 8) * 64) {
     sub1::note_kernel("rms_norm_kernel, a wavefront a row");
-    const unsigned grid = static_cast<unsigned>((a.rows + 3) / 4);
     const int per = (eights + 63) / 64;
-    if (per == 1) rms_norm_kernel<T, R, kResidual, true, 1><<<grid, 256, 0, s>>>(a);
-    else if (per == 2) rms_norm_kernel<T, R, kResidual, true, 2><<<grid, 256, 0, s>>>(a);
-    else if (per == 3) rms_norm_kernel<T, R, kResidual, true, 3><<<grid, 256, 0, s>>>(a);
-    else if (per == 4) rms_norm_kernel<T, R, kResidual, true, 4><<<grid, 256, 0, s>>>(a);
-    else if (per == 5) rms_norm_kernel<T, R, kResidual, true, 5><<<grid, 256, 0, s>>>(a);
-    else if (per == 6) rms_norm_kernel<T, R, kResidual, true, 6><<<grid, 256, 0, s>>>(a);
-    else rms_norm_kernel<T, R, kResidual, true, 8><<<grid, 256, 0, s>>>(a);
+    if (per == 1) launch_lanes<T, R, kResidual, 64, 1>(a, s);
+    else if (per == 2) launch_lanes<T, R, kResidual, 64, 2>(a, s);
+    else if (per == 3) launch_lanes<T, R, kResidual, 64, 3>(a, s);
+    else if (per == 4) launch_lanes<T, R, kResidual, 64, 4>(a, s);
+    else if constexpr (sizeof(T) == 2 && sizeof(R) == 2) {
+      if (per == 5) launch_lanes<T, R, kResidual, 64, 5>(a, s);
+      else if (per == 6) launch_lanes<T, R, kResidual, 64, 6>(a, s);
+      else launch_lanes<T, R, kResidual, 64, 8>(a, s);
+    }
   } else {
     sub1::note_kernel("rms_norm_kernel, a workgroup a row");
     const unsigned grid = static_cast<unsigned>(a.rows);
-    if (eights <= 1024) rms_norm_kernel<T, R, kResidual, false, 1><<<grid, (eights + 63) / 64 * 64, 0, s>>>(a);
-    else if (eights <= 2048) rms_norm_kernel<T, R, kResidual, false, 2><<<grid, 1024, 0, s>>>(a);
-    else if (eights <= 4096) rms_norm_kernel<T, R, kResidual, false, 4><<<grid, 1024, 0, s>>>(a);
+    if (eights <= 1024) rms_norm_kernel<T, R, kResidual, 0, 1><<<grid, (eights + 63) / 64 * 64, 0, s>>>(a);
+    else if (eights <= 2048) rms_norm_kernel<T, R, kResidual, 0, 2><<<grid, 1024, 0, s>>>(a);
+    else if (eights <= 4096) rms_norm_kernel<T, R, kResidual, 0, 4><<<grid, 1024, 0, s>>>(a);
     else rms_norm_wide_kernel<T, R, kResidual><<<grid, 1024, 0, s>>>(a);
   }
   HIP_TRY(hipGetLastError());

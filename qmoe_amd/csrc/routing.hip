@@ -21,7 +21,7 @@ struct RouteArgs {
   float *shares;
   void *index;
   int64_t row_bytes, tokens;
-  int experts, top_k, groups, top_groups, group_mark, sigmoid, normalize, wide_index;
+  int experts, top_k, groups, top_groups, group_mark, sigmoid, normalize, wide_index, group_bits;   // 2^group_bits: groups and more
   float scale;
 };
 
@@ -52,38 +52,37 @@ __device__ __forceinline__ double value_of(uint64_t rank) {
                    : __longlong_as_double(rank >> 63 ? rank & 0x7fffffffffffffffull : ~rank);
 }
 
-template <class Combine>
-__device__ __forceinline__ uint32_t wave_all(uint32_t v, Combine combine) {   // zeros from beyond the lanes do no harm
-  v = combine(v, static_cast<uint32_t>(sub1::dpp_or_zero<sub1::kDppRowShr1, 0xf>(static_cast<int>(v))));
-  v = combine(v, static_cast<uint32_t>(sub1::dpp_or_zero<sub1::kDppRowShr2, 0xf>(static_cast<int>(v))));
-  v = combine(v, static_cast<uint32_t>(sub1::dpp_or_zero<sub1::kDppRowShr4, 0xf>(static_cast<int>(v))));
-  v = combine(v, static_cast<uint32_t>(sub1::dpp_or_zero<sub1::kDppRowShr8, 0xf>(static_cast<int>(v))));
-  v = combine(v, static_cast<uint32_t>(sub1::dpp_or_zero<sub1::kDppBcast15, 0xa>(static_cast<int>(v))));
-  v = combine(v, static_cast<uint32_t>(sub1::dpp_or_zero<sub1::kDppBcast31, 0xc>(static_cast<int>(v))));
-  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
+template <int kLanes>
+__device__ __forceinline__ uint32_t largest_over(uint32_t v) {
+  return over_lanes<kLanes>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
-__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
-  return wave_all(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+template <int kLanes>
+__device__ __forceinline__ uint32_t smallest_over(uint32_t v) {
+  return over_lanes<kLanes>(v, [](uint32_t a, uint32_t b) { return min(a, b); });
 }
-__device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
-  const uint32_t high = wave_largest(static_cast<uint32_t>(v >> 32));
-  return static_cast<uint64_t>(high) << 32 | wave_largest(static_cast<uint32_t>(v >> 32) == high ? static_cast<uint32_t>(v) : 0u);
+template <int kLanes>
+__device__ __forceinline__ uint64_t largest_over(uint64_t v) {
+  const uint32_t high = largest_over<kLanes>(static_cast<uint32_t>(v >> 32));
+  return static_cast<uint64_t>(high) << 32 | largest_over<kLanes>(static_cast<uint32_t>(v >> 32) == high ? static_cast<uint32_t>(v) : 0u);
 }
-__device__ __forceinline__ double wave_total(double v) {
-  const uint64_t u = __double_as_longlong(mx4::wave_sum(v));
-  return __longlong_as_double(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u >> 32), 63))) << 32 |
-                              static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u), 63)));
-}
-
 struct Best {
   uint64_t rank;
   int at;   // -1: none
 };
 // The lanes' best, of equal ranks the lowest `at`.
 __device__ __forceinline__ Best wave_best(Best b) {
-  const uint64_t rank = wave_largest(b.at < 0 ? 0 : b.rank);
-  const uint32_t at = wave_largest(b.at >= 0 && b.rank == rank ? ~static_cast<uint32_t>(b.at) : 0u);
+  const uint64_t rank = largest_over<64>(b.at < 0 ? uint64_t{0} : b.rank);
+  const uint32_t at = largest_over<64>(b.at >= 0 && b.rank == rank ? ~static_cast<uint32_t>(b.at) : 0u);
   return {rank, at ? static_cast<int>(~at) : -1};
+}
+
+__device__ __forceinline__ void store_choice(const RouteArgs &a, int64_t token, int place, double share, int expert) {
+  const int64_t at = token * a.top_k + place;
+  a.shares[at] = static_cast<float>(share * a.scale);
+  if (a.wide_index)
+    static_cast<int64_t *>(a.index)[at] = expert;
+  else
+    static_cast<int32_t *>(a.index)[at] = expert;
 }
 
 // A wavefront's token, everything computed again in 64 bits wherever it is asked for: right for every case.
@@ -95,13 +94,13 @@ __device__ __forceinline__ void route_exactly(const RouteArgs &a, int64_t token)
   if (!a.sigmoid) {
     uint64_t largest = 0;
     for (int e = lane; e < a.experts; e += 64) largest = max(largest, rank_of(logit_at<T>(row, e)));
-    most = value_of(wave_largest(largest));
+    most = value_of(largest_over<64>(largest));
     if (most == -INFINITY) {
       most = 0;   // all of them masked: scores of zero
     } else {
       double sum = 0;
       for (int e = lane; e < a.experts; e += 64) sum += exp(logit_at<T>(row, e) - most);
-      under = wave_total(sum);
+      under = sum_over<64>(sum);
     }
   }
   auto score = [&](int e) {
@@ -160,29 +159,295 @@ __device__ __forceinline__ void route_exactly(const RouteArgs &a, int64_t token)
   const bool has = lane < a.top_k;
   double share = has ? score(mine) : 0.0;
   if (a.normalize) {
-    const double total = wave_total(share);
+    const double total = sum_over<64>(share);
     if (total != 0) share /= total;
   }
-  if (has) {
-    const int64_t at = token * a.top_k + lane;
-    a.shares[at] = static_cast<float>(share * a.scale);
-    if (a.wide_index)
-      static_cast<int64_t *>(a.index)[at] = mine;
-    else
-      static_cast<int32_t *>(a.index)[at] = mine;
-  }
+  if (has) store_choice(a, token, lane, share, mine);
 }
 
 template <class T>
-__global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
+__global__ __launch_bounds__(256) void route_exact_kernel(const RouteArgs a) {
   const int64_t token = blockIdx.x * int64_t{4} + (threadIdx.x >> 6);
   if (token < a.tokens) route_exactly<T>(a, token);
 }
 
+// ---------------------------------------------------------------- the quick form ---
+
+__device__ __forceinline__ uint32_t rank32(float v) {   // as rank_of; of numbers alone
+  const uint32_t bits = __float_as_uint(v + 0.0f);
+  return bits >> 31 ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float value32(uint32_t rank) {
+  return __uint_as_float(rank >> 31 ? rank & 0x7fffffffu : ~rank);
+}
+
+// kLanes lanes a token, kPer experts a lane.  Scores are computed in 32 bits, which places all experts but those next to each other; from
+// there are taken the top_k and on as long as the next may be one of them for all that is known, and of those alone the order is found in 64
+// bits.  What that leaves open (marks of groups too close to tell, more near the last than there are lanes) and what is no
+// number goes to the exact form.  A lane has experts of one group, as many together as 16 bytes
+// of logits hold, then those behind the group's other lanes', kPer in all.  An expert's key is its rank with j in the last bits, so that the largest key says which it is.
+template <class T, int kLanes, int kPer>
+__device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token) {
+  constexpr uint32_t kIndex = kPer - 1;
+  constexpr float kLog2e = 1.44269504f;
+  const int lane = threadIdx.x & (kLanes - 1), size = a.experts / a.groups, group_lanes = kLanes >> a.group_bits;
+  const int group = lane / group_lanes, sub = lane & (group_lanes - 1), base = group * size;
+  const bool in_group = group < a.groups;
+  const uint8_t *row = a.logits + token * a.row_bytes;
+  constexpr int kTogether = kPer < 16 / static_cast<int>(sizeof(T)) ? kPer : 16 / static_cast<int>(sizeof(T));
+  auto at_of = [&](int j) { return kTogether * (sub + group_lanes * (j / kTogether)) + j % kTogether; };   // in its group
+  float v[kPer], b[kPer];
+  const T *const logits = reinterpret_cast<const T *>(row) + base;
+#pragma unroll
+  for (int j = 0; j < kPer; j += kTogether) {
+    T some[kTogether] = {};
+    if (in_group && at_of(j) + kTogether <= size) {
+      __builtin_memcpy(some, logits + at_of(j), sizeof(some));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kTogether; i++)
+        if (in_group && at_of(j + i) < size) some[i] = logits[at_of(j + i)];
+    }
+#pragma unroll
+    for (int i = 0; i < kTogether; i++) v[j + i] = static_cast<float>(some[i]);
+  }
+  if (a.bias) {
+#pragma unroll
+    for (int j = 0; j < kPer; j += kTogether) {
+      float some[kTogether] = {};
+      if (in_group && at_of(j) + kTogether <= size) {
+        __builtin_memcpy(some, a.bias + base + at_of(j), sizeof(some));
+      } else {
+#pragma unroll
+        for (int i = 0; i < kTogether; i++)
+          if (in_group && at_of(j + i) < size) some[i] = a.bias[base + at_of(j + i)];
+      }
+#pragma unroll
+      for (int i = 0; i < kTogether; i++) b[j + i] = some[i];
+    }
+  }
+  bool odd = false;   // something that the exact form has to look at
+  float most = 0, largest_score = 1;
+  double under = 1;
+  const bool approximate = a.bias != nullptr;
+  auto there = [&](int j) { return in_group && at_of(j) < size; };
+  if (!a.sigmoid) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) m = there(j) ? fmaxf(m, v[j]) : m;
+    most = value32(largest_over<kLanes>(rank32(m)));
+    double sum = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; j++)
+      sum += there(j) ? static_cast<double>(__builtin_amdgcn_exp2f((v[j] - most) * kLog2e)) : 0.0;
+    under = sum_over<kLanes>(sum);
+    largest_score = static_cast<float>(1 / under);
+    odd |= !(fabsf(most) < INFINITY);
+  }
+  const float over = largest_score;
+  auto score32 = [&](float l) {
+    return a.sigmoid ? __builtin_amdgcn_rcpf(1 + __builtin_amdgcn_exp2f(-l * kLog2e)) : __builtin_amdgcn_exp2f((l - most) * kLog2e) * over;
+  };
+  // how far apart two sums of scores and biases near `c` may be taken for when they are not.  A sigmoid is off by less than 2^-22 (its
+  // argument's rounding, at most 1.5 |l| 2^-24 s (1 - s), the exponential's and the quotient's steps), a share by less than 2^-20 of the
+  // largest (|l - most| e^(l - most) is at most 0.37; a sum over 4096 is off by 2^-20 of itself); a mark has two of them, a sum's steps are 2^-24 c.
+  auto tolerance = [&](float c) { return (a.sigmoid ? 0x1p-20f : 0x1p-18f * largest_score) + 0x1p-21f * fabsf(c); };
+  auto exact_score = [&](float l) {
+    return a.sigmoid ? 1 / (1 + exp(-static_cast<double>(l))) : exp(static_cast<double>(l) - most) / under;
+  };
+  auto sum_exactly = [&] {
+    double sum = 0;
+    for (int j = 0; j < kPer; j++)
+      if (there(j)) sum += exp(static_cast<double>(logit_at<T>(row, base + at_of(j))) - most);
+    under = sum_over<kLanes>(sum);
+  };
+  float one = -INFINITY, two = -INFINITY;   // the lane's best of its group, for the group's mark
+  const bool by_marks = a.top_groups < a.groups, marks_of_scores = approximate || a.group_mark == 2;
+  uint32_t key[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; j++) {
+    float c = v[j];
+    if (approximate) {
+      c = score32(v[j]) + b[j];
+      odd |= there(j) && !(fabsf(c) < INFINITY);
+    }
+    odd |= there(j) && c != c;
+    key[j] = there(j) ? (rank32(c) & ~kIndex) | (kIndex - j) : 0;
+    if (by_marks) {
+      v[j] = there(j) ? (!approximate && marks_of_scores ? score32(v[j]) : c) : -INFINITY;
+      two = fmaxf(two, fminf(one, v[j]));
+      one = fmaxf(one, v[j]);
+    }
+  }
+  if (by_marks) {
+    for (int by = 1; by < group_lanes; by *= 2) {
+      const float other_one = __shfl_xor(one, by, kLanes), other_two = __shfl_xor(two, by, kLanes);
+      two = fmaxf(fmaxf(two, other_two), fminf(one, other_one));
+      one = fmaxf(one, other_one);
+    }
+    const bool of_two = a.group_mark == 2 && size > 1;
+    const float mark = of_two ? one + two : one;
+    odd |= in_group && marks_of_scores && !(fabsf(mark) < INFINITY);
+    const uint32_t rank = in_group ? rank32(mark) : 0;
+    bool taken = false;
+    uint32_t last = 0;
+    auto pick = [&](auto from) {   // the groups with the largest marks, of equal ones the lower; the last one's mark
+      auto most_of = largest_over<kLanes>(from);
+      taken = false;
+      for (int i = 0; i < a.top_groups; i++) {
+        most_of = largest_over<kLanes>(taken ? decltype(from)(0) : from);
+        taken |= static_cast<uint32_t>(group) == smallest_over<kLanes>(!taken && from == most_of ? static_cast<uint32_t>(group) : ~0u);
+      }
+      return most_of;
+    };
+    last = pick(rank);
+    if (marks_of_scores) {
+      const float kept = value32(last), next = value32(largest_over<kLanes>(taken ? 0 : rank));
+      if (__ballot(!odd && !(next < kept - tolerance(kept)))) {   // too close: marks in 64 bits, of the experts that may be in them
+        if (!a.sigmoid) sum_exactly();
+        const float least = of_two ? two : one;
+        const float from = least - tolerance(least);
+        uint64_t look = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) look |= static_cast<uint64_t>(there(j) && v[j] >= from) << j;
+        double exact_one = -INFINITY, exact_two = -INFINITY;
+        while (__ballot(look != 0)) {
+          if (look) {
+            const int e = base + at_of(__ffsll(static_cast<unsigned long long>(look)) - 1);
+            const double c = exact_score(logit_at<T>(row, e)) + (approximate ? static_cast<double>(a.bias[e]) : 0.0);
+            exact_two = fmax(exact_two, fmin(exact_one, c));
+            exact_one = fmax(exact_one, c);
+            look &= look - 1;
+          }
+        }
+        for (int by = 1; by < group_lanes; by *= 2) {
+          const double other_one = __shfl_xor(exact_one, by, kLanes), other_two = __shfl_xor(exact_two, by, kLanes);
+          exact_two = fmax(fmax(exact_two, other_two), fmin(exact_one, other_one));
+          exact_one = fmax(exact_one, other_one);
+        }
+        pick(in_group ? rank_of(of_two ? exact_one + exact_two : exact_one) : uint64_t{0});
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; j++) key[j] = taken ? key[j] : 0;
+  }
+
+  // lane i of the token has the i-th found; behind top_k as long as the next may belong before it
+  int mine = 0, found = 0;
+  uint32_t least = 0;
+  for (int i = 0; i < kLanes; i++) {
+    uint32_t best = key[0];
+#pragma unroll
+    for (int j = 1; j < kPer; j++) best = max(best, key[j]);
+    const uint32_t m = largest_over<kLanes>(best);
+    bool more = i < a.top_k;
+    if (i == a.top_k - 1) least = m & ~kIndex;
+    if (!more && m) {
+      const float kept = value32(least), next = value32(m & ~kIndex);
+      more = approximate ? !(next < kept - tolerance(kept) - kPer * 0x1p-22f * fabsf(kept)) : (m & ~kIndex) == least;
+    }
+    if (!__ballot(more)) break;
+    const int at = at_of(static_cast<int>(kIndex - (m & kIndex)));
+    const uint32_t e = smallest_over<kLanes>(best == m ? static_cast<uint32_t>(base + at) : ~0u);
+    const uint32_t gone = best == m && static_cast<uint32_t>(base + at) == e ? m : ~0u;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) key[j] = key[j] == gone ? 0 : key[j];
+    if (more) {
+      if (lane == i) mine = static_cast<int>(e);
+      found = i + 1;
+    }
+    odd |= i == kLanes - 1;
+  }
+
+  // in 64 bits: scores of those found, their order
+  const bool has = lane < found;
+  const float l = logit_at<T>(row, mine);
+  double score = exact_score(l);
+  int place = 0;
+  for (int again = 0; again < 2; again++) {
+    const double c = approximate ? score + a.bias[mine] : static_cast<double>(l);
+    // they are in order but where they were told apart by less than the keys hold
+    const double after = __shfl(c, lane + 1, kLanes);
+    const int index_after = __shfl(mine, lane + 1, kLanes);
+    bool close = lane + 1 < found && fabs(c - after) < 0x1p-20 * largest_score;   // (the sum under the scores is of those in 32 bits)
+    place = lane;
+    if (__ballot(lane + 1 < found && !(c > after || (c == after && mine < index_after)))) {
+      place = 0;
+      for (int i = 0; i < kLanes; i++) {
+        if (!__ballot(i < found)) break;
+        const double other = __shfl(c, i, kLanes);
+        const int at = __shfl(mine, i, kLanes);
+        if (i < found && i != lane) {
+          place += other > c || (other == c && at < mine);
+          close |= has && fabs(other - c) < 0x1p-20 * largest_score;
+        }
+      }
+    }
+    if (again || a.sigmoid || !approximate || !__ballot(close && !odd)) break;
+    sum_exactly();
+    score = exact_score(l);
+  }
+  const uint64_t odds = __ballot(odd) >> (threadIdx.x & (64 - kLanes));   // of this token's lanes, from bit 0 on
+  if (kLanes == 64 ? odds != 0 : (odds & 0xffff) != 0) return false;
+  const bool kept = has && place < a.top_k;
+  double share = kept ? score : 0.0;
+  if (a.normalize) {
+    const double total = sum_over<kLanes>(share);
+    if (total != 0) share /= total;
+  }
+  if (kept) store_choice(a, token, place, share, mine);
+  return true;
+}
+
+template <class T, int kLanes, int kPer>
+__global__ __launch_bounds__(256) void route_quick_kernel(const RouteArgs a) {
+  constexpr int kTokens = 64 / kLanes;   // of a wavefront
+  const int64_t first = (blockIdx.x * int64_t{4} + (threadIdx.x >> 6)) * kTokens;
+  if (first >= a.tokens) return;
+  const int64_t token = first + (threadIdx.x & 63) / kLanes;
+  // tokens that are not there repeat the last
+  const uint64_t done = __ballot(route_quickly<T, kLanes, kPer>(a, token < a.tokens ? token : a.tokens - 1));
+  if (done == ~uint64_t{0}) return;
+  for (int i = 0; i < kTokens && first + i < a.tokens; i++)
+    if (!(done >> (i * kLanes) & 1)) route_exactly<T>(a, first + i);
+}
+
+template <class T, int kLanes, int kPer>
+void launch_quick(const RouteArgs &a, hipStream_t s) {
+  constexpr int kTokens = 4 * 64 / kLanes;
+  route_quick_kernel<T, kLanes, kPer><<<static_cast<unsigned>((a.tokens + kTokens - 1) / kTokens), 256, 0, s>>>(a);
+}
+
 template <class T>
-int launch_route(const RouteArgs &a, hipStream_t s) {
-  sub1::note_kernel("route_kernel");
-  route_kernel<T><<<static_cast<unsigned>((a.tokens + 3) / 4), 256, 0, s>>>(a);
+int launch_route(RouteArgs a, hipStream_t s) {
+  a.group_bits = 0;
+  while (1 << a.group_bits < a.groups) a.group_bits++;
+  // experts a lane, with 16 or 64 lanes a token
+  auto per = [&](int lanes) {
+    const int of_group = lanes >> a.group_bits;
+    return of_group ? (a.experts / a.groups + of_group - 1) / of_group : 1 << 30;
+  };
+  const int per16 = per(16), per64 = per(64);
+  if (a.tokens >= 1024 && per16 <= 16 && a.top_k <= 12) {
+    sub1::note_kernel("route_quick_kernel, 16 lanes a token");
+    if (per16 <= 1) launch_quick<T, 16, 1>(a, s);
+    else if (per16 <= 2) launch_quick<T, 16, 2>(a, s);
+    else if (per16 <= 4) launch_quick<T, 16, 4>(a, s);
+    else if (per16 <= 8) launch_quick<T, 16, 8>(a, s);
+    else launch_quick<T, 16, 16>(a, s);
+  } else if (per64 <= 64 && a.top_k <= 56) {
+    sub1::note_kernel("route_quick_kernel, 64 lanes a token");
+    if (per64 <= 1) launch_quick<T, 64, 1>(a, s);
+    else if (per64 <= 2) launch_quick<T, 64, 2>(a, s);
+    else if (per64 <= 4) launch_quick<T, 64, 4>(a, s);
+    else if (per64 <= 8) launch_quick<T, 64, 8>(a, s);
+    else if (per64 <= 16) launch_quick<T, 64, 16>(a, s);
+    else if (per64 <= 32) launch_quick<T, 64, 32>(a, s);
+    else launch_quick<T, 64, 64>(a, s);
+  } else {
+    sub1::note_kernel("route_exact_kernel");
+    route_exact_kernel<T><<<static_cast<unsigned>((a.tokens + 3) / 4), 256, 0, s>>>(a);
+  }
   HIP_TRY(hipGetLastError());
   return SUB1_OK;
 }
@@ -251,7 +516,7 @@ extern "C" int sub1_route(const sub1_router *router, const void *logits, int typ
   if (misaligned(logits, kTypeBytes[type]) || misaligned(shares, 4) || misaligned(index, index_bytes) || misaligned(r.bias, 4))
     return fail(SUB1_ERR_ALIGN, "sub1_route: misaligned pointer");
   const RouteArgs a{static_cast<const uint8_t *>(logits), r.bias, shares, index, ldl * kTypeBytes[type], tokens, r.experts, r.top_k,
-                    r.groups, r.top_groups, r.group_mark, r.scores == SUB1_ROUTE_SIGMOID, r.normalize != 0, index_bytes == 8, r.scale};
+                    r.groups, r.top_groups, r.group_mark, r.scores == SUB1_ROUTE_SIGMOID, r.normalize != 0, index_bytes == 8, 0, r.scale};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (type == SUB1_MX4_BF16) return launch_route<__bf16>(a, s);
   if (type == SUB1_MX4_FP16) return launch_route<_Float16>(a, s);

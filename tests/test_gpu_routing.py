@@ -93,6 +93,66 @@ def test_scores_closer_than_fp32_can_tell(scores):
         check(logits[t:t + 1].cuda(), 2, scores, grouped.cuda(), 8, 2, 2)
 
 
+def check_many(logits, top_k, scores, bias, groups, top_groups, group_mark, normalize):
+    """Many tokens at once, numbers alone: the same by sorts over all of them."""
+    shares, index = routing.route(logits, top_k, scores, bias, groups, top_groups, group_mark, normalize)
+    l = logits.double()
+    s = torch.softmax(l, -1) if scores == 'softmax' else 1 / (1 + torch.exp(-l))
+    c = s if bias is None else s + bias.double()
+    key = l if bias is None else c
+    if top_groups < groups:
+        of = torch.sort((key if group_mark == 1 else c).view(len(l), groups, -1), -1, descending=True)[0][..., :group_mark].sum(-1)
+        best = torch.sort(of, dim=-1, descending=True, stable=True)[1][:, :top_groups]
+        kept = torch.zeros_like(of, dtype=torch.bool).scatter_(1, best, True).repeat_interleave(key.shape[1] // groups, 1)
+        key = torch.where(kept, key, -float('inf'))
+    at = torch.sort(key, dim=-1, descending=True, stable=True)[1][:, :top_k]
+    assert torch.equal(index, at)
+    want = s.gather(1, at)
+    if normalize:
+        want = want / want.sum(-1, keepdim=True)
+    assert bool(((shares - want).abs() <= (logits.shape[-1] + top_k + 16) * 2.0 ** -23 * want + 2.0 ** -126).all())
+
+
+@pytest.mark.parametrize('experts,top_k,groups,top_groups', CASES)
+@pytest.mark.parametrize('scores', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('biased', [False, True])
+def test_route_many_tokens(experts, top_k, groups, top_groups, scores, biased):
+    g = gen(experts + top_k + 1)
+    bias = 0.1 * torch.randn(experts, generator=g).cuda() if biased else None
+    for i, (name, tokens) in enumerate((('fp32', 3001), ('bf16', 1025), ('fp16', 1536))):
+        logits = part((2 * torch.randn((tokens, experts), generator=g) + torch.randn((1, experts), generator=g)).to(TYPES[name]), i % 2 == 1)
+        for group_mark in (1, 2):
+            check_many(logits, top_k, scores, bias, groups, top_groups, group_mark, i % 2 == 0)
+        # many equal ones, and many close ones
+        check_many((logits.float() / 2).round().to(TYPES[name]), top_k, scores, bias, groups, top_groups, 2, True)
+        check_many((1 + 1e-6 * logits.float()).to(TYPES[name]), top_k, scores, None if bias is None else 1e-6 * bias, groups, top_groups, 1, True)
+
+
+@pytest.mark.parametrize('scores', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('experts,groups,top_groups', [(60, 1, 1), (60, 6, 2), (256, 8, 4), (200, 1, 1)])
+def test_what_is_no_number_among_many_tokens(scores, experts, groups, top_groups):
+    """Rows with masks and NaN give in a large call what they give in a small one, and their neighbours too."""
+    inf, nan = float('inf'), float('nan')
+    g = gen(experts)
+    logits = torch.randn((2000, experts), generator=g)
+    logits[3] = -inf
+    logits[100, 2:] = -inf
+    logits[101, 5] = nan
+    logits[500] = nan
+    logits[501, 7] = inf
+    logits[900:904, ::3] = -inf
+    logits[1200, 3:] = torch.finfo(torch.float32).min
+    logits[1300] = 0.25
+    logits[1999, -1] = nan
+    rows = [0, 2, 3, 4, 99, 100, 101, 102, 500, 501, 502, 903, 1199, 1200, 1201, 1300, 1301, 1998, 1999]
+    for bias in (None, 0.1 * torch.randn(experts, generator=g).cuda()):
+        for group_mark in (1, 2):
+            many = routing.route(logits.cuda(), 6, scores, bias, groups, top_groups, group_mark, True)
+            few = check(logits[rows].cuda(), 6, scores, bias, groups, top_groups, group_mark, True)
+            assert torch.equal(many[1][rows], few[1])
+            assert torch.allclose(many[0][rows], few[0], rtol=1e-5, atol=1e-37, equal_nan=True)
+
+
 def test_shapes_of_routing():
     logits = torch.randn((3, 5, 40), generator=gen(3)).cuda()
     shares, index = routing.route(logits, 2)
