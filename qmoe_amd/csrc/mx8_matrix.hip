@@ -339,8 +339,9 @@ void launch_few(const Product8Args &p, hipStream_t s) {
 template <int kRows, int kTokens, int kRowSides, int kTokenSides, int kParts, int kStages>
 struct Many8 {
   static constexpr int waves = kRowSides * kTokenSides, rows = 32 * kRows * kRowSides, tokens = 32 * kTokens * kTokenSides;
+  static constexpr int chunk = waves >= 16 ? 8 : 4;   // steps whose scales are loaded at once (8192^3 438 us by eights, 455 by fours; with 12 waves no less)
   static constexpr int w_bytes = rows * 64, step_bytes = w_bytes + tokens * 128;
-  static constexpr int scale_rows = rows + tokens, scales_at = kStages * step_bytes, part_bytes = scales_at + 2 * 16 * scale_rows;
+  static constexpr int scale_rows = rows + tokens, scales_at = kStages * step_bytes, part_bytes = scales_at + 2 * 4 * chunk * scale_rows;
   static constexpr int group = kRows % 4 == 0 ? 4 : kRows % 3 == 0 ? 3 : kRows;   // tiles of 32 rows that go to y at once
   static constexpr int pitch = 32 * group + 8;                                    // bf16, of a token's rows on their way
   static constexpr int lds_bytes = kParts * part_bytes;
@@ -361,7 +362,7 @@ __device__ __forceinline__ TilePlace tile_of_workgroup(int id, int row_tiles, in
 }
 
 template <int kRows, int kTokens, int kRowSides, int kTokenSides, int kParts, int kStages, bool kQuantize>
-__global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * kTokenSides * kParts >= 16 ? 4 : 3) void mx8_many_kernel(const Product8Args p) {
+__global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * kTokenSides * kParts == 12 ? 3 : 4) void mx8_many_kernel(const Product8Args p) {
   using M = Many8<kRows, kTokens, kRowSides, kTokenSides, kParts, kStages>;
   constexpr int kWaves = M::waves;
   constexpr int kWAll = M::rows / 16, kXAll = M::tokens / 8;   // fetches of a step: 16 rows' 64 bytes or 8 tokens' 128
@@ -408,15 +409,15 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * 
     for (int i = 0; i < kXFetches; i++)
       mx4::fetch(x_from, x_at[i] - max((x_part[i] >> 1) - last, 0) * kBlock, to + M::w_bytes + min(i * kWaves + wave, kXAll - 1) * 1024);
   };
-  // This thread's rows' or tokens' scales of the sixteen blocks of four turns, as two eights, each from its first block on or the row's
-  // last eight (the caller's rows have as many); what is left over repeats the last.
-  constexpr int kScaleRows = (M::scale_rows + 64 * kWaves - 1) / (64 * kWaves);
-  uint64_t scales[kScaleRows][2];
+  // This thread's pieces of the scales of M::chunk turns, sixteen blocks of a row or token each, as two eights, each from its first
+  // block on or the row's last eight (the caller's rows have as many); what is left over repeats the last.
+  constexpr int kOfRow = M::chunk / 4, kAllPieces = M::scale_rows * kOfRow, kPieces = (kAllPieces + 64 * kWaves - 1) / (64 * kWaves);
+  uint64_t scales[kPieces][2];
+  auto piece_of = [&](int j) { return min(j * 64 * kWaves + tid, kAllPieces - 1); };
   auto load_scales = [&](int turn) {
-    const int first = 4 * (first_step + turn);
 #pragma unroll
-    for (int j = 0; j < kScaleRows; j++) {
-      const int row = min(j * 64 * kWaves + tid, M::scale_rows - 1);
+    for (int j = 0; j < kPieces; j++) {
+      const int piece = piece_of(j), row = piece / kOfRow, first = 4 * (first_step + turn) + 16 * (piece % kOfRow);
       const uint8_t *from = row < M::rows ? p.scales + static_cast<int64_t>(min(row0 + row, p.height - 1)) * blocks
                                           : p.x_scales + static_cast<int64_t>(min(token0 + row - M::rows, p.tokens - 1)) * blocks;
 #pragma unroll
@@ -424,11 +425,11 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * 
     }
   };
   uint32_t *const scale_lds = reinterpret_cast<uint32_t *>(lds) + M::scales_at / 4;
-  auto put_scales = [&](int turn) {   // zeros behind the row's last; of four turns, each turn's rows back to back
-    const int first = 4 * (first_step + turn);
+  auto put_scales = [&](int turn) {   // zeros behind the row's last; of each turn the rows back to back
 #pragma unroll
-    for (int j = 0; j < kScaleRows; j++) {
-      uint32_t *to = scale_lds + (turn & 4) * M::scale_rows + min(j * 64 * kWaves + tid, M::scale_rows - 1);
+    for (int j = 0; j < kPieces; j++) {
+      const int piece = piece_of(j), row = piece / kOfRow, first = 4 * (first_step + turn) + 16 * (piece % kOfRow);
+      uint32_t *to = scale_lds + ((turn & M::chunk) + 4 * (piece % kOfRow)) * M::scale_rows + row;
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const int behind = max(first + 8 * i + 8 - blocks, 0);
@@ -464,18 +465,18 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * 
         sum[r][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4::wide(a[r]), b[n], sum[r][n], 4, 0, 2 * k, as[r], 2 * k, bs[n]);
     __builtin_amdgcn_sched_barrier(0);
   };
-  // Turn t finds its codes there, asks for those of turn t + kStages - 1, whose place was read in the turn before, and multiplies.  The third of
-  // four turns puts the next four's scales where those of the four before were.
+  // Turn t finds its codes there, asks for those of turn t + kStages - 1, whose place was read in the turn before, and multiplies.  The last but one of a chunk of
+  // turns puts the next chunk's scales where those of the chunk before were.
   int side = 0, ahead = kStages - 1;
-  auto turn = [&](auto in_four, int t) {
+  auto turn = [&](auto in_chunk, int t) {
     mx4::meet<(kStages - 2) * (kWFetches + kXFetches)>();   // but for the codes that later turns asked for
-    if (decltype(in_four)::value == 2) {
+    if (decltype(in_chunk)::value == M::chunk - 2) {
       put_scales(t + 2);
-      load_scales(t + 6);
+      load_scales(t + 2 + M::chunk);
     }
     fetch_step(ahead, t + kStages - 1);
     __builtin_amdgcn_sched_barrier(0);
-    const uint32_t *from = scale_lds + (t & 7) * M::scale_rows + in_tile;
+    const uint32_t *from = scale_lds + (t & (2 * M::chunk - 1)) * M::scale_rows + in_tile;
 #pragma unroll
     for (int r = 0; r < kRows; r++) as[r] = static_cast<int>(from[(row_side * kRows + r) * 32] >> (8 * half));
 #pragma unroll
@@ -487,7 +488,7 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * 
   };
   load_scales(0);
   put_scales(0);
-  load_scales(4);
+  load_scales(M::chunk);
 #pragma unroll
   for (int i = 0; i < kStages - 1; i++) fetch_step(i, i);
   int t = 0;
@@ -500,6 +501,16 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * 
     if (++t == turns) break;
     turn(std::integral_constant<int, 3>{}, t);
     if (++t == turns) break;
+    if constexpr (M::chunk == 8) {
+      turn(std::integral_constant<int, 4>{}, t);
+      if (++t == turns) break;
+      turn(std::integral_constant<int, 5>{}, t);
+      if (++t == turns) break;
+      turn(std::integral_constant<int, 6>{}, t);
+      if (++t == turns) break;
+      turn(std::integral_constant<int, 7>{}, t);
+      if (++t == turns) break;
+    }
   }
   mx4::meet<0>();   // nothing is on its way into LDS any more, and nobody reads it
   if constexpr (kParts > 1) {   // the parts' sums, added in their order
@@ -639,7 +650,7 @@ const Form kForm[kForms] = {
     {128, 128, 2, 1, 4.8f, 0.86f, 0.89f, 4.2f, launch_many<2, 2, 2, 2, 2, 2>},
     {128, 128, 1, 2, 4.7f, 0.36f, 0.50f, 2.6f, launch_many<2, 2, 2, 2, 1, 3>},
     {256, 128, 1, 2, 4.9f, 0.63f, 0.76f, 5.4f, launch_many<2, 2, 4, 2, 1, 2>},
-    {256, 256, 1, 1, 6.9f, 1.14f, 1.19f, 8.1f, launch_many<2, 2, 4, 4, 1, 2>},
+    {256, 256, 1, 1, 6.9f, 1.11f, 1.15f, 8.1f, launch_many<2, 2, 4, 4, 1, 2>},
     {288, 256, 1, 1, 8.2f, 0.95f, 1.31f, 12.6f, launch_many<3, 2, 3, 4, 1, 2>},
 };
 constexpr int kUnits = 256;   // compute units
