@@ -725,6 +725,10 @@ int sub1_mx8_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t row
 int sub1_mx8_product(const uint8_t *codes, const uint8_t *scales, int height, int width, const uint8_t *x_codes,
                      const uint8_t *x_scales, int relu, void *y, int64_t ldy, uint8_t *y_codes, uint8_t *y_scales, int tokens,
                      void *stream);
+/* For tests: later sub1_mx8_product launches for more than one token take form `which` (1 .. SUB1_MX8_FORMS) instead of
+ * the one estimated fastest, where the arguments allow it; 0: by estimate. */
+#define SUB1_MX8_FORMS 13
+int sub1_test_mx8_form(int which);
 
 /*
  * Root-mean-square norm of the rows of x [rows, width], the residual's addition before it:

@@ -20,6 +20,7 @@ MX4_LAYER_TOKENS = 256            # SUB1_MX4_LAYER_TOKENS
 MX4_LAYER_TOP_K = 8               # SUB1_MX4_LAYER_TOP_K
 MX4_LAYER_EXPERTS = 4096          # SUB1_MX4_LAYER_EXPERTS
 
+MX8_FORMS = 13                    # SUB1_MX8_FORMS
 NORM_MAX_ROWS = 1 << 30           # SUB1_NORM_MAX_ROWS
 NORM_LEAST_EPS = 1e-30            # SUB1_NORM_LEAST_EPS
 ROUTE_MAX_EXPERTS = 4096          # SUB1_ROUTE_MAX_EXPERTS
@@ -161,6 +162,7 @@ PROTOTYPES = {
     'sub1_mx8_quantize': (_int, [_vp, _int, _i64, _i64, _int, _vp, _vp, _vp]),
     'sub1_mx8_dequantize': (_int, [_vp, _vp, _i64, _int, _vp, _int, _i64, _vp]),
     'sub1_mx8_product': (_int, [_vp, _vp, _int, _int, _vp, _vp, _int, _vp, _i64, _vp, _vp, _int, _vp]),
+    'sub1_test_mx8_form': (_int, [_int]),
     'sub1_rms_norm': (_int, [ctypes.POINTER(Norm), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp]),
     'sub1_route': (_int, [ctypes.POINTER(Router), _vp, _int, _i64, _i64, _vp, _vp, _int, _vp]),
     'sub1_combine': (_int, [_vp, _int, _vp, _vp, _i64, _int, _int, _vp, _vp]),

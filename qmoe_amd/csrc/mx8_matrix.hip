@@ -1,6 +1,7 @@
 // Activations in microscaled 8 bits: values to the format and back, and their products with matrices
 // in microscaled 4 bits.
 #include "mx8.h"
+#include <atomic>
 #include <cmath>
 
 using namespace mx8;
@@ -637,7 +638,9 @@ struct Form {
   float start, turn, busy, more;
   void (*launch)(const Product8Args &, hipStream_t);
 };
-constexpr int kForms = 13, kFewForms = 3;
+std::atomic<int> g_forced_form{0};   // sub1_test_mx8_form
+
+constexpr int kForms = SUB1_MX8_FORMS, kFewForms = 3;
 const Form kForm[kForms] = {
     {16, 16, 8, 3, 2.6f, 0.82f, 0.70f, 0.0f, launch_few<1, 1>},   // (not for a result in 8 bits: half a block)
     {32, 16, 8, 2, 2.6f, 1.13f, 0.95f, 0.0f, launch_few<2, 1>},
@@ -663,12 +666,17 @@ int launch_product(const Product8Args &p, hipStream_t s) {
     if (p.y_codes) return halves ? launch_one<32, true>(p, s) : launch_one<64, true>(p, s);
     return halves ? launch_one<32, false>(p, s) : launch_one<64, false>(p, s);
   }
+  const int forced = g_forced_form.load(std::memory_order_relaxed) - 1;
   int best = -1;
   float shortest = 0;
   for (int i = 0; i < kForms; i++) {
     const Form &f = kForm[i];
     const bool few = i < kFewForms;
     if ((p.y_codes && f.rows < 32) || (!few && blocks < 8)) continue;   // (through LDS: whole eights of scales)
+    if (i == forced) {
+      best = i;
+      break;
+    }
     const int64_t tiles = static_cast<int64_t>((p.height + f.rows - 1) / f.rows) * ((p.tokens + f.tokens - 1) / f.tokens);
     const int64_t rounds = tiles / (kUnits * f.at_once), left = (tiles - rounds * kUnits * f.at_once + kUnits - 1) / kUnits;
     const int steps = few ? (blocks + 7) / 8 : (blocks + 3) / 4, turns = (steps + f.parts - 1) / f.parts;
@@ -745,6 +753,12 @@ extern "C" int sub1_mx8_dequantize(const uint8_t *codes, const uint8_t *scales, 
     else
       mx8_dequantize_kernel<float><<<grid, 256, 0, s>>>(c, sc, n, width, to, row_bytes);
   });
+}
+
+extern "C" int sub1_test_mx8_form(int which) {
+  if (which < 0 || which > kForms) return fail(SUB1_ERR_SHAPE, "sub1_test_mx8_form: no form %d", which);
+  g_forced_form.store(which, std::memory_order_relaxed);
+  return SUB1_OK;
 }
 
 extern "C" int sub1_mx8_product(const uint8_t *codes, const uint8_t *scales, int height, int width, const uint8_t *x_codes,

@@ -35,6 +35,7 @@ def test_header_constants_match_binding():
     for name, value in (('ROUTE_MAX_EXPERTS', _lib.ROUTE_MAX_EXPERTS), ('ROUTE_MAX_TOP_K', _lib.ROUTE_MAX_TOP_K),
                         ('ROUTE_SOFTMAX', 0), ('ROUTE_SIGMOID', 1)):
         assert int(re.search(r'#define SUB1_%s (\d+)' % name, text).group(1)) == value
+    assert '#define SUB1_MX8_FORMS 13' in text and _lib.MX8_FORMS == 13
     assert '#define SUB1_NORM_MAX_ROWS (1 << 30)' in text and _lib.NORM_MAX_ROWS == 1 << 30
     assert '#define SUB1_ROUTE_MAX_TOKENS (1 << 24)' in text and _lib.ROUTE_MAX_TOKENS == 1 << 24
     assert '#define SUB1_NORM_LEAST_EPS 1e-30' in text and _lib.NORM_LEAST_EPS == 1e-30
@@ -67,6 +68,12 @@ def test_the_product_refuses(change, status):
     for at, value in change.items():
         args[at] = value
     assert _lib.load().sub1_mx8_product(*args) == status
+
+
+def test_forms_that_are_not_there():
+    for which in (-1, _lib.MX8_FORMS + 1):
+        assert _lib.load().sub1_test_mx8_form(which) == -2
+    assert _lib.load().sub1_test_mx8_form(0) == 0
 
 
 def test_the_norm_refuses():

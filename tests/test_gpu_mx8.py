@@ -146,6 +146,51 @@ def test_product_into_eight_bits(height, width, tokens):
         bo.check_quantized(y_codes[at].cpu().numpy(), y_scales[at].cpu().numpy(), np.maximum(exact, 0) if relu else exact, off)
 
 
+@pytest.fixture
+def form():
+    """Sets the form that products take, and back."""
+    yield lambda which: _lib.check(_lib.load().sub1_test_mx8_form(which))
+    _lib.check(_lib.load().sub1_test_mx8_form(0))
+
+
+@pytest.mark.parametrize('which', range(1, _lib.MX8_FORMS + 1))
+@pytest.mark.parametrize('height,width,tokens', [(300, 1000, 300), (33, 256, 2), (577, 2079, 515), (289, 225, 257), (96, 4500, 65), (2081, 640, 31),
+                                                 (64, 1152, 128), (1100, 3201, 1030)])
+def test_every_form(which, height, width, tokens, form):
+    """Odd tiles, rows of a step, of fewer steps than there are groups that share them, and many."""
+    codes, scales, w = matrix(height, width, height + width, spread=3)
+    x_codes, x_scales, x = activations(tokens, width, tokens + width)
+    exact, off = bo.product8_bound(x, w)
+    fine = some(tokens)
+    finely = bo.product8_bound_finely(x[fine], w)
+    form(which)
+    got = mx8.product(x_codes, x_scales, codes, scales, width)
+    within(got, *bo.to_bf16(exact, off))
+    within(got[fine], *bo.to_bf16(*finely))
+    y_codes, y_scales = mx8.product(x_codes, x_scales, codes, scales, width, True, True)
+    bo.check_quantized(y_codes.cpu().numpy(), y_scales.cpu().numpy(), np.maximum(exact, 0), off)
+    bo.check_quantized(y_codes[fine].cpu().numpy(), y_scales[fine].cpu().numpy(), np.maximum(finely[0], 0), finely[1])
+    x_scales[-1, -1], scales[height // 2, 0] = 255, 255       # no numbers in the last token and a row
+    got = host(mx8.product(x_codes, x_scales, codes, scales, width))
+    assert np.isnan(got[-1]).all() and np.isnan(got[:, height // 2]).all()
+    assert np.isfinite(np.delete(got[:-1], height // 2, 1)).all()
+
+
+@pytest.mark.parametrize('which', range(1, _lib.MX8_FORMS + 1))
+def test_sums_past_fp32(which, form):
+    """Scales whose products fp32 does not hold: infinite, of the sum's sign."""
+    codes, scales, w = matrix(70, 256, 5)
+    codes &= 0x77
+    codes |= 0x11                                             # no zeros, none negative
+    x_codes = torch.full((70, 256), 0x38, dtype=torch.uint8, device='cuda')
+    x_codes[1::2] |= 0x80
+    x_scales, scales = torch.full((70, 8), 254, dtype=torch.uint8, device='cuda'), torch.full_like(scales, 254)
+    form(which)
+    got = mx8.product(x_codes, x_scales, codes, scales, 256)
+    assert bool((got[0::2] == float('inf')).all()) and bool((got[1::2] == -float('inf')).all())
+    assert bool((mx8.product(x_codes[:1], x_scales[:1], codes, scales, 256) == float('inf')).all())
+
+
 @pytest.mark.parametrize('tokens', [1, 5, 16, 40, 130, 600])
 @pytest.mark.parametrize('quantize', [False, True])
 @pytest.mark.parametrize('relu', [False, True])
