@@ -174,8 +174,8 @@ __global__ __launch_bounds__(256) void route_exact_kernel(const RouteArgs a) {
 // ---------------------------------------------------------------- the quick form ---
 
 __device__ __forceinline__ uint32_t rank32(float v) {   // as rank_of; of numbers alone
-  const uint32_t bits = __float_as_uint(v + 0.0f);
-  return bits >> 31 ? ~bits : bits | 0x80000000u;
+  const int32_t bits = __float_as_int(v + 0.0f);
+  return static_cast<uint32_t>(bits ^ (bits >> 31 | static_cast<int32_t>(0x80000000)));
 }
 __device__ __forceinline__ float value32(uint32_t rank) {
   return __uint_as_float(rank >> 31 ? rank & 0x7fffffffu : ~rank);
@@ -230,17 +230,18 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
   float most = 0, largest_score = 1;
   double under = 1;
   const bool approximate = a.bias != nullptr;
-  auto there = [&](int j) { return in_group && at_of(j) < size; };
+  const int limit = in_group ? size : 0;
+  auto there = [&](int j) { return at_of(j) < limit; };
   if (!a.sigmoid) {
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kPer; j++) m = there(j) ? fmaxf(m, v[j]) : m;
     most = value32(largest_over<kLanes>(rank32(m)));
-    double sum = 0;
+    double sum[4] = {0, 0, 0, 0};   // (four chains: one of 64-bit sums takes its time)
 #pragma unroll
     for (int j = 0; j < kPer; j++)
-      sum += there(j) ? static_cast<double>(__builtin_amdgcn_exp2f((v[j] - most) * kLog2e)) : 0.0;
-    under = sum_over<kLanes>(sum);
+      sum[j % 4] += static_cast<double>(there(j) ? __builtin_amdgcn_exp2f((v[j] - most) * kLog2e) : 0.0f);
+    under = sum_over<kLanes>((sum[0] + sum[1]) + (sum[2] + sum[3]));
     largest_score = static_cast<float>(1 / under);
     odd |= !(fabsf(most) < INFINITY);
   }
@@ -427,14 +428,17 @@ int launch_route(RouteArgs a, hipStream_t s) {
     const int of_group = lanes >> a.group_bits;
     return of_group ? (a.experts / a.groups + of_group - 1) / of_group : 1 << 30;
   };
+  // A wavefront for four tokens where there are several for every SIMD, else for one (us in a graph: 8192 tokens' 8 of 256 in groups, a bias, 11 and 16; 8
+  // of 512, softmax, a bias 14.7 and 19; 4096 tokens' 2 of 128 4.4 and 5.2; 2048 tokens' 8 of 256 in groups 9.3 and 7.6, 1 of 128 4.0 and 3.8).
   const int per16 = per(16), per64 = per(64);
-  if (a.tokens >= 1024 && per16 <= 16 && a.top_k <= 12) {
+  if (a.tokens > 2500 && per16 <= 32 && a.top_k <= 12) {
     sub1::note_kernel("route_quick_kernel, 16 lanes a token");
     if (per16 <= 1) launch_quick<T, 16, 1>(a, s);
     else if (per16 <= 2) launch_quick<T, 16, 2>(a, s);
     else if (per16 <= 4) launch_quick<T, 16, 4>(a, s);
     else if (per16 <= 8) launch_quick<T, 16, 8>(a, s);
-    else launch_quick<T, 16, 16>(a, s);
+    else if (per16 <= 16) launch_quick<T, 16, 16>(a, s);
+    else launch_quick<T, 16, 32>(a, s);
   } else if (per64 <= 64 && a.top_k <= 56) {
     sub1::note_kernel("route_quick_kernel, 64 lanes a token");
     if (per64 <= 1) launch_quick<T, 64, 1>(a, s);
