@@ -411,7 +411,7 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * 
       mx4::fetch(x_from, x_at[i] - max((x_part[i] >> 1) - last, 0) * kBlock, to + M::w_bytes + min(i * kWaves + wave, kXAll - 1) * 1024);
   };
   // This thread's pieces of the scales of M::chunk turns, sixteen blocks of a row or token each, as two eights, each from its first
-  // block on or the row's last eight (the caller's rows have as many); what is left over repeats the last.
+  // block on or the row's last eight, of a row of fewer those at the top; what is left over repeats the last.
   constexpr int kOfRow = M::chunk / 4, kAllPieces = M::scale_rows * kOfRow, kPieces = (kAllPieces + 64 * kWaves - 1) / (64 * kWaves);
   uint64_t scales[kPieces][2];
   auto piece_of = [&](int j) { return min(j * 64 * kWaves + tid, kAllPieces - 1); };
@@ -421,8 +421,18 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * 
       const int piece = piece_of(j), row = piece / kOfRow, first = 4 * (first_step + turn) + 16 * (piece % kOfRow);
       const uint8_t *from = row < M::rows ? p.scales + static_cast<int64_t>(min(row0 + row, p.height - 1)) * blocks
                                           : p.x_scales + static_cast<int64_t>(min(token0 + row - M::rows, p.tokens - 1)) * blocks;
+      if (blocks >= 8) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) __builtin_memcpy(&scales[j][i], from + min(first + 8 * i, blocks - 8), 8);
+        for (int i = 0; i < 2; i++) __builtin_memcpy(&scales[j][i], from + min(first + 8 * i, blocks - 8), 8);
+      } else {
+        uint64_t all = 0;
+#pragma unroll
+        for (int b = 0; b < 7; b++) {
+          const uint64_t scale = from[min(b, blocks - 1)];
+          if (b < blocks) all = all >> 8 | scale << 56;
+        }
+        scales[j][0] = scales[j][1] = all;
+      }
     }
   };
   uint32_t *const scale_lds = reinterpret_cast<uint32_t *>(lds) + M::scales_at / 4;
@@ -672,7 +682,7 @@ int launch_product(const Product8Args &p, hipStream_t s) {
   for (int i = 0; i < kForms; i++) {
     const Form &f = kForm[i];
     const bool few = i < kFewForms;
-    if ((p.y_codes && f.rows < 32) || (!few && blocks < 8)) continue;   // (through LDS: whole eights of scales)
+    if (p.y_codes && f.rows < 32) continue;
     if (i == forced) {
       best = i;
       break;

@@ -177,6 +177,40 @@ def test_every_form(which, height, width, tokens, form):
 
 
 @pytest.mark.parametrize('which', range(1, _lib.MX8_FORMS + 1))
+@pytest.mark.parametrize('height,width,tokens', [(130, 1, 70), (33, 33, 2), (300, 96, 300), (70, 128, 31), (577, 129, 130), (289, 224, 257)])
+def test_every_form_on_rows_of_few_blocks(which, height, width, tokens, form):
+    """Fewer than eight: their scales are loaded one by one; some groups have no step at all."""
+    codes, scales, w = matrix(height, width, height + width, spread=3)
+    x_codes, x_scales, x = activations(tokens, width, tokens + width)
+    exact, off = bo.product8_bound_finely(x, w)
+    form(which)
+    within(mx8.product(x_codes, x_scales, codes, scales, width), *bo.to_bf16(exact, off))
+    y_codes, y_scales = mx8.product(x_codes, x_scales, codes, scales, width, True, True)
+    bo.check_quantized(y_codes.cpu().numpy(), y_scales.cpu().numpy(), np.maximum(exact, 0), off)
+    x_scales[-1, -1], scales[height // 2, -1] = 255, 255
+    got = host(mx8.product(x_codes, x_scales, codes, scales, width))
+    assert np.isnan(got[-1]).all() and np.isnan(got[:, height // 2]).all()
+    assert np.isfinite(np.delete(got[:-1], height // 2, 1)).all()
+
+
+@pytest.mark.parametrize('which', [0, 1, 2, 3, 4])
+def test_the_most_tokens(which, form):
+    """As many as a call takes, through a narrow matrix: the most tiles of tokens that a launch has."""
+    tokens, height, width = _lib.MX4_MAX_TOKENS, 33, 40
+    codes, scales, w = matrix(height, width, 1)
+    x_codes, x_scales, x = activations(tokens, width, 2)
+    form(which)
+    got = mx8.product(x_codes, x_scales, codes, scales, width)
+    at = [0, 15, 16, tokens // 2, tokens - 17, tokens - 16, tokens - 1]
+    within(got[at], *bo.to_bf16(*bo.product8_bound_finely(x[at], w)))
+    # two roundings of 2^-8 of a value each, and twice 5 eights' products cut off by 7 2^-14 of the eight's largest (0.0043 of it)
+    form(0)
+    for part in (slice(0, 3000), slice(tokens - 3000, tokens)):
+        again = mx8.product(x_codes[part].contiguous(), x_scales[part].contiguous(), codes, scales, width)
+        assert bool(((got[part].float() - again.float()).abs() <= 0.02 * again.float().abs().max()).all())
+
+
+@pytest.mark.parametrize('which', range(1, _lib.MX8_FORMS + 1))
 def test_sums_past_fp32(which, form):
     """Scales whose products fp32 does not hold: infinite, of the sum's sign."""
     codes, scales, w = matrix(70, 256, 5)
