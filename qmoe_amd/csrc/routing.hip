@@ -188,6 +188,8 @@ __device__ __forceinline__ float value32(uint32_t rank) {
 // of logits hold, then those behind the group's other lanes', kPer in all.  An expert's key is its rank with j in the last bits, so that the largest key says which it is.
 template <class T, int kLanes, int kPer>
 __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token) {
+  __shared__ uint16_t all_places[256];
+  uint16_t *const places = all_places + (threadIdx.x & ~(kLanes - 1));   // of this token
   constexpr uint32_t kIndex = kPer - 1;
   constexpr float kLog2e = 1.44269504f;
   const int lane = threadIdx.x & (kLanes - 1), size = a.experts / a.groups, group_lanes = kLanes >> a.group_bits;
@@ -333,14 +335,30 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
     for (int j = 0; j < kPer; j++) key[j] = taken ? key[j] : 0;
   }
 
-  // lane i of the token has the i-th found; behind top_k as long as the next may belong before it
-  int mine = 0, found = 0;
+  // The lane's largest keys, the largest first: a choice takes one off, and only a lane that has given all of them goes through its
+  // experts again.
+  constexpr int kTop = kPer < 3 ? kPer : 3;
+  uint32_t top[kTop];
+  auto look = [&](uint32_t below) {
+#pragma unroll
+    for (int i = 0; i < kTop; i++) top[i] = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+      uint32_t k = key[j] < below ? key[j] : 0;
+#pragma unroll
+      for (int i = 0; i < kTop; i++) {
+        const uint32_t less = min(top[i], k);
+        top[i] = max(top[i], k);
+        k = less;
+      }
+    }
+  };
+  look(~0u);
+  // places[i] is the i-th found; behind top_k as long as the next may belong before it
+  int found = 0, given = 0;
   uint32_t least = 0;
   for (int i = 0; i < kLanes; i++) {
-    uint32_t best = key[0];
-#pragma unroll
-    for (int j = 1; j < kPer; j++) best = max(best, key[j]);
-    const uint32_t m = largest_over<kLanes>(best);
+    const uint32_t best = top[0], m = largest_over<kLanes>(best);
     bool more = i < a.top_k;
     if (i == a.top_k - 1) least = m & ~kIndex;
     if (!more && m) {
@@ -348,20 +366,32 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
       more = approximate ? !(next < kept - tolerance(kept) - kPer * 0x1p-22f * fabsf(kept)) : (m & ~kIndex) == least;
     }
     if (!__ballot(more)) break;
-    const int at = at_of(static_cast<int>(kIndex - (m & kIndex)));
-    const uint32_t e = smallest_over<kLanes>(best == m ? static_cast<uint32_t>(base + at) : ~0u);
-    const uint32_t gone = best == m && static_cast<uint32_t>(base + at) == e ? m : ~0u;
-#pragma unroll
-    for (int j = 0; j < kPer; j++) key[j] = key[j] == gone ? 0 : key[j];
-    if (more) {
-      if (lane == i) mine = static_cast<int>(e);
-      found = i + 1;
+    const uint32_t e = static_cast<uint32_t>(base + at_of(static_cast<int>(kIndex - (best & kIndex))));
+    bool mine = best == m && m;
+    if (__popcll(__ballot(mine)) != 64 / kLanes) {   // of equal ones the lower
+      const uint32_t lowest = smallest_over<kLanes>(mine ? e : ~0u);
+      mine &= e == lowest;
     }
+    if (mine) {
+      if (more) places[i] = static_cast<uint16_t>(e);
+#pragma unroll
+      for (int k = 0; k < kTop; k++) top[k] = k + 1 < kTop ? top[k + 1] : 0;
+      given++;
+    }
+    if (kTop < kPer && __ballot(mine && given == kTop)) {
+      if (mine && given == kTop) {
+        look(m);
+        given = 0;
+      }
+    }
+    if (more) found = i + 1;
     odd |= i == kLanes - 1;
   }
+  sub1::wave_lds_fence();
 
   // in 64 bits: scores of those found, their order
   const bool has = lane < found;
+  const int mine = has ? min(static_cast<int>(places[lane]), a.experts - 1) : 0;   // (where there is something odd nothing may be found)
   const float l = logit_at<T>(row, mine);
   double score = exact_score(l);
   int place = 0;
