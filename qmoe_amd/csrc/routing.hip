@@ -367,7 +367,7 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
     }
     if (!__ballot(more)) break;
     const uint32_t e = static_cast<uint32_t>(base + at_of(static_cast<int>(kIndex - (best & kIndex))));
-    bool mine = best == m && m;
+    bool mine = best == m;   // (of a token that has none left all of them)
     if (__popcll(__ballot(mine)) != 64 / kLanes) {   // of equal ones the lower
       const uint32_t lowest = smallest_over<kLanes>(mine ? e : ~0u);
       mine &= e == lowest;

@@ -153,6 +153,21 @@ def test_what_is_no_number_among_many_tokens(scores, experts, groups, top_groups
             assert torch.allclose(many[0][rows], few[0], rtol=1e-5, atol=1e-37, equal_nan=True)
 
 
+@pytest.mark.parametrize('experts,top_k', [(12, 12), (12, 10), (24, 11), (9, 9)])
+def test_equal_ones_beside_rows_with_fewer_numbers(experts, top_k):
+    """Rows that share a wavefront: one has its last two equal where another has none left but what is no number."""
+    logits = torch.randn((2601, experts), generator=gen(experts))
+    logits[:, -2:] = -9.0
+    for i in range(2):
+        logits[i::4, :2].view(torch.int32)[:] = -1             # NaN with every bit set
+    for dtype in (torch.float32, torch.bfloat16):
+        l = logits.to(dtype)
+        assert bool(l.isnan().any())
+        _, index = routing.route(l.cuda(), top_k, 'sigmoid')
+        _, want = bo.route(host(l), top_k, 'sigmoid', None, 1, 1, 1, False, 1.0)
+        assert np.array_equal(index.cpu().numpy(), want)
+
+
 def test_shapes_of_routing():
     logits = torch.randn((3, 5, 40), generator=gen(3)).cuda()
     shares, index = routing.route(logits, 2)
