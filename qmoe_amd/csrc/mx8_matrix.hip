@@ -21,7 +21,8 @@ namespace {
 
 // ------------------------------------------------------- to the format and back ---
 
-// Four lanes a block, eight values a lane.
+// Four lanes a block, eight values a lane: 16 bytes of bf16 a load, 8 of codes a store.  Bound by HBM: 16384 x 2080 in
+// bf16 to the format 21 us (4.9 TB/s, as a copy), back 17 (codes that were just written are partly still on the chip).
 template <class T>
 __global__ __launch_bounds__(256) void mx8_quantize_kernel(const uint8_t *__restrict__ x, int64_t row_bytes, uint32_t rows,
                                                            int width, uint8_t *__restrict__ codes,
@@ -55,6 +56,18 @@ __global__ __launch_bounds__(256) void mx8_dequantize_kernel(const uint8_t *__re
 }
 
 // ------------------------------------------------------------------- products ---
+//
+// y[t, r] = sum over k of W[r, k] x[t, k]: a block's 32 products times both blocks' powers of two.  One token goes
+// through the vector units; from two on the scaled MFMAs take both sides' codes as they lie, at the rate of 8 bits (of
+// a tile in registers 3.7 PFLOP/s, and 4.6 of zeros: power).  They add the products of eight neighbours as whole
+// numbers of 2^-14 times the power of two in the largest of them, cut off toward zero below, and those sums in fp32; a
+// product has six bits at most, so that nothing is lost of those from 2^-8 of the largest on.  That is less than a
+// rounding of a result to bf16; of a result in 8 bits a few codes in ten thousand are a step off those that sums in 64
+// bits would get.  (Products in bf16, which have no such step, run at half the rate and ask for both sides to be
+// expanded.)
+//
+// The compiler may move an MFMA into a branch that alone uses its result, where lanes outside hold no operands: all
+// lanes use these sums.
 
 struct Product8Args {
   const uint8_t *codes, *scales, *x_codes, *x_scales;
@@ -72,9 +85,11 @@ __device__ __forceinline__ i32x8 operand(u32x4 a, u32x4 b) {
                static_cast<int>(b[0]), static_cast<int>(b[1]), static_cast<int>(b[2]), static_cast<int>(b[3])};
 }
 
-// One token: kLanes lanes, a wavefront or half of one, take a whole row, a block a lane at a time, as mx4_one_kernel does; the token waits in
-// LDS as bf16 (exact: an e4m3 has four bits), its scales beside it.  A block's 32 products are added without scales, then brought to the power of two of
-// both, so that no value leaves a type's range on the way.  For a result in 8 bits a workgroup has the 32 rows of a block.
+// One token: kLanes lanes, a wavefront or half of one, take a whole row, a block a lane at a time, as mx4_one_kernel
+// does; the token waits in LDS as bf16 (exact: an e4m3 has four bits), its scales beside it.  A block's 32 products are
+// added without scales, then brought to the power of two of both, so that no value leaves a type's range on the way.
+// For a result in 8 bits a workgroup has the 32 rows of a block.  Reads 17 bytes for 32 products, so HBM would bound it
+// (2080 x 6144: 6.8 MB, 1.4 us); it takes 3.8 us, 2.2 of them an empty launch's, the rest two trips to memory.
 constexpr int kOneWaves = mx4::kOneWaves;
 __host__ __device__ constexpr int one_token_bytes(int width) { return mx4::one_lds_bytes(width); }
 __host__ __device__ constexpr int one_lds_bytes(int width) { return one_token_bytes(width) + (blocks_of(width) + 15) / 16 * 16; }
@@ -170,10 +185,12 @@ int launch_one(const Product8Args &p, hipStream_t s) {
   return SUB1_OK;
 }
 
-// Few tokens: eight wavefronts a workgroup take eight blocks of its rows and tokens in turn; whole lines are read and the
-// blocks handed round through LDS, a part of the wavefront's own, the next ones on their way meanwhile.
+// Few tokens: eight wavefronts a workgroup take eight blocks of its rows and tokens in turn; whole lines are read and
+// the blocks handed round through LDS, a part of the wavefront's own, the next ones on their way meanwhile.
 // v_mfma_scale_f32_16x16x128_f8f6f4 takes lane l's block l / 16 of row l % 16 as it is; of token l % 16 it takes in
-// lane l the 16 values from 16 (l / 16) on and the 16 from 64 + 16 (l / 16) on, but its scale for block l / 16.
+// lane l the 16 values from 16 (l / 16) on and the 16 from 64 + 16 (l / 16) on, but its scale for block l / 16.  Bound
+// by trips to memory, one a turn of the eight wavefronts (16 tokens through 2080 x 6144, three turns: 4.8 us in a
+// graph; its bytes take 1.4); more tokens cost the tokens' own reads, which every workgroup of rows repeats (64: 7.6).
 template <int kRows, int kTokens>
 __global__ __launch_bounds__(64 * kFewWaves) void mx8_few_kernel(const Product8Args p) {
   constexpr int kStage = kRows * 128 + kTokens * 256;   // of 16 bytes: 16 rows of 128, 16 tokens of 256
@@ -330,13 +347,19 @@ void launch_few(const Product8Args &p, hipStream_t s) {
   mx8_few_kernel<kRows, kTokens><<<grid, 64 * kFewWaves, 0, s>>>(p);
 }
 
-// Many tokens: kRowSides by kTokenSides wavefronts, each with 32 kRows rows of the matrix and 32 kTokens tokens, 128 values
-// of a row a step.  Codes of both sides go straight into LDS, kStages steps of them; nothing but a wavefront's operands and sums is in
-// registers, so that three or four wavefronts a SIMD fit, one's reads of LDS under the others' products.  kParts groups of such wavefronts share a
-// tile's steps, where tiles alone would leave compute units idle.  v_mfma_scale_f32_32x32x64_f8f6f4 takes lane l's
-// block l / 32 of row l % 32 as it is, of token l % 32 the 16 values from 16 (l / 32) on and the 16 from 32 + 16 (l / 32) on, and each
-// side's scale for block l / 32 as one byte of a register.  Scales come through registers, sixteen (four steps') of a row or token a
-// thread, and LDS: loaded by each wavefront for itself they were two of three requests to L2, which bound the launch.
+// Many tokens: kRowSides by kTokenSides wavefronts, each with 32 kRows rows of the matrix and 32 kTokens tokens, 128
+// values of a row a step.  Codes of both sides go straight into LDS, kStages steps of them; nothing but a wavefront's
+// operands and sums is in registers, so that three or four wavefronts a SIMD fit, one's reads of LDS under the others'
+// products.  kParts groups of such wavefronts share a tile's steps, where tiles alone would leave compute units idle.
+// v_mfma_scale_f32_32x32x64_f8f6f4 takes lane l's block l / 32 of row l % 32 as it is, of token l % 32 the 16 values
+// from 16 (l / 32) on and the 16 from 32 + 16 (l / 32) on, and each side's scale for block l / 32 as one byte of a
+// register.  Scales come through registers, sixteen (four steps') of a row or token a thread, and LDS: loaded by each
+// wavefront for itself they were two of three requests to L2, which bound the launch. 8192 tokens through 2080 x 6144
+// take 89 us (2.3 PFLOP/s), through 8192 x 8192 420 (2.6); matrix cores are busy for 58 % of the launch at clocks that
+// power holds at 2.0 GHz.  Without the fetches of codes it took 22 % less, without scales 11, without y's stores 9; 256
+// x 256 with operands read ahead by 8 wavefronts 97 where 16 wavefronts without took 84 (2048 rows), three stages as
+// two; two steps a turn, fetches after the first products, a higher priority for wavefronts in their products: within 2
+// %.
 template <int kRows, int kTokens, int kRowSides, int kTokenSides, int kParts, int kStages>
 struct Many8 {
   static constexpr int waves = kRowSides * kTokenSides, rows = 32 * kRows * kRowSides, tokens = 32 * kTokens * kTokenSides;
@@ -349,9 +372,9 @@ struct Many8 {
   static_assert(32 * pitch * 2 * waves <= lds_bytes && rows * tokens * 4 * (kParts > 1) <= lds_bytes && lds_bytes <= 160 * 1024, "what a compute unit has");
 };
 
-// The tile that a workgroup takes.  Workgroups go to the eight XCDs in turn, and those of one get tiles that lie together: groups of four
-// tiles of tokens by all rows, the group's tokens first, so that what an XCD's compute units work on at a time is about eight by four
-// tiles, whose codes its L2 reads once.
+// The tile that a workgroup takes.  Workgroups go to the eight XCDs in turn, and those of one get tiles that lie
+// together: groups of four tiles of tokens by all rows, the group's tokens first, so that what an XCD's compute units
+// work on at a time is about eight by four tiles, whose codes its L2 reads once.
 struct TilePlace {
   int row, token;
 };
@@ -476,8 +499,9 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * 
         sum[r][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4::wide(a[r]), b[n], sum[r][n], 4, 0, 2 * k, as[r], 2 * k, bs[n]);
     __builtin_amdgcn_sched_barrier(0);
   };
-  // Turn t finds its codes there, asks for those of turn t + kStages - 1, whose place was read in the turn before, and multiplies.  The last but one of a chunk of
-  // turns puts the next chunk's scales where those of the chunk before were.
+  // Turn t finds its codes there, asks for those of turn t + kStages - 1, whose place was read in the turn before, and
+  // multiplies.  The last but one of a chunk of turns puts the next chunk's scales where those of the chunk before
+  // were.
   int side = 0, ahead = kStages - 1;
   auto turn = [&](auto in_chunk, int t) {
     mx4::meet<(kStages - 2) * (kWFetches + kXFetches)>();   // but for the codes that later turns asked for
@@ -638,11 +662,13 @@ void launch_many(const Product8Args &p, hipStream_t s) {
     mx8_many_kernel<kRows, kTokens, kRowSides, kTokenSides, kParts, kStages, false><<<tiles, 64 * M::waves * kParts, 0, s>>>(p);
 }
 
-// Which kernel, for more tokens than one: that with the shortest estimate.  A form's tiles run `at_once` to a compute unit; a turn of its steps takes
-// `turn` where one tile or fewer is on each, and `busy` for every tile where there are more (it is then shared); what does not depend on the row's
-// length is `start` a launch and `more` a full round of the compute units.  In us, fitted to graphs of calls of 17 to 8192 tokens through 2080 x 6144,
-// 6144 x 2080, 1024 x 4096, 4096 x 1024, 3001 x 1023, 768 x 2500 and 1500 x 1500, to 6 to 14 % each; of those 126 the form with
-// the shortest estimate took 1.2 % longer than the best on average, 28 % at most.
+// Which kernel, for more tokens than one: that with the shortest estimate.  A form's tiles run `at_once` to a compute
+// unit; a turn of its steps takes `turn` where one tile or fewer is on each, and `busy` for every tile where there are
+// more (it is then shared); what does not depend on the row's length is `start` a launch and `more` a full round of the
+// compute units.  In us, fitted to graphs of calls of 17 to 8192 tokens through 2080 x 6144, 6144 x 2080, 1024 x 4096,
+// 4096 x 1024, 3001 x 1023, 768 x 2500 and 1500 x 1500, to 6 to 14 % each; of those 126 the form with the shortest
+// estimate took 1.2 % longer than the best on average, 28 % at most; of 42 through rows of 1 to 8 blocks 4 %, 29 at
+// most.
 struct Form {
   int rows, tokens, parts, at_once;   // few: parts are wavefronts, of 256 values a turn
   float start, turn, busy, more;

@@ -35,9 +35,12 @@ __device__ __forceinline__ Factor factor_of(const NormArgs &a, double sum) {
   return {large ? 0x1p-64f : 1.0f, static_cast<float>(large ? factor * 0x1p64 : factor)};
 }
 
-// A row's values stay in registers, kPer eights a thread: one read of x and r, one write of s and y.  The sum of squares is held
-// in 64 bits: no square of an fp32 value overflows there and the order of the sum does not count; the vector
-// units add and multiply 64 bits as fast as 32.  kLanes: 16 or 64 lanes a row, where nothing waits for another wavefront; 0: a workgroup a row.
+// A row's values stay in registers, kPer eights a thread: one read of x and r, one write of s and y.  The sum of
+// squares is held in 64 bits: no square of an fp32 value overflows there and the order of the sum does not count; the
+// vector units add and multiply 64 bits as fast as 32.  kLanes: 16 or 64 lanes a row, where nothing waits for another
+// wavefront; 0: a workgroup a row. Bound by HBM: 16384 x 2080 in bf16 with a residual, to 8 bits, 48 us in a graph, 5.0
+// TB/s (a copy: 4.95 to 5.4); 16384 x 1023 in fp16, whose rows do not lie on 16 bytes, 3.7 TB/s.  Loads and stores that
+// pass the caches by measured alike.
 template <class T, class R, bool kResidual, int kLanes, int kPer>
 __global__ __launch_bounds__(kLanes ? 256 : 1024) void rms_norm_kernel(const NormArgs a) {
   __shared__ double parts[16];
@@ -179,10 +182,11 @@ void launch_lanes(const NormArgs &a, hipStream_t s) {
   rms_norm_kernel<T, R, kResidual, kLanes, kPer><<<static_cast<unsigned>((a.rows + kRows - 1) / kRows), 256, 0, s>>>(a);
 }
 
-// Which form (us, in a graph).  Few rows: a workgroup each, an eight a thread as far as 1024 threads go (1000 x 2080, residual, to 8 bits 6.1, by a wavefront
-// each 7.2; 4000 14.2 and 15.3), and rows of fp32 that a wavefront's registers hold barely (4096 x 4096, residual 43 and 50).  Many: a
-// wavefront each (16384 x 2080 48 and 53; without residual 26 and 36).  Many narrow ones: a quarter of one (16384 x 100 5.8 and
-// 11, 16000 x 300 11.3 and 12.8; 1000 x 300 by a workgroup each 3.9, by quarters 4.7).
+// Which form (us, in a graph).  Few rows: a workgroup each, an eight a thread as far as 1024 threads go (1000 x 2080,
+// residual, to 8 bits 6.1, by a wavefront each 7.2; 4000 14.2 and 15.3), and rows of fp32 that a wavefront's registers
+// hold barely (4096 x 4096, residual 43 and 50).  Many: a wavefront each (16384 x 2080 48 and 53; without residual 26
+// and 36).  Many narrow ones: a quarter of one (16384 x 100 5.8 and 11, 16000 x 300 11.3 and 12.8; 1000 x 300 by a
+// workgroup each 3.9, by quarters 4.7).
 template <class T, class R, bool kResidual>
 int launch_rows(const NormArgs &a, hipStream_t s) {
   const int eights = blocks_of(a.width) * 4;

@@ -77,7 +77,8 @@ def dequantize(codes, scales, width, dtype=torch.bfloat16):
 
 
 def product(x_codes, x_scales, codes, scales, width, relu=False, quantize=False):
-    """bf16 [.., H] = x W^T with x [.., W] in 8 bits and W [H, W] in 4 (mx4.quantize); fp32 sums.  `relu`: what is below
+    """bf16 [.., H] = x W^T with x [.., W] in 8 bits and W [H, W] in 4 (mx4.quantize); fp32 sums (of eight neighbouring
+    products each, of which the matrix cores cut off what is below 2^-14 of the largest).  `relu`: what is below
     zero becomes zero; `quantize`: the result in 8 bits, (codes [.., 32 * blocks of H], scales), rounded once."""
     got = _quick('mx8_product', _entry('sub1_mx8_product'), x_codes, x_scales, codes, scales, width, relu, quantize)
     if got is not None:
