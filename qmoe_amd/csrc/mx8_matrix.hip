@@ -369,7 +369,7 @@ struct Many8 {
   static constexpr int group = kRows % 4 == 0 ? 4 : kRows % 3 == 0 ? 3 : kRows;   // tiles of 32 rows that go to y at once
   static constexpr int pitch = 32 * group + 8;                                    // bf16, of a token's rows on their way
   static constexpr int lds_bytes = kParts * part_bytes;
-  static_assert(32 * pitch * 2 * waves <= lds_bytes && rows * tokens * 4 * (kParts > 1) <= lds_bytes && lds_bytes <= 160 * 1024, "what a compute unit has");
+  static_assert(32 * pitch * 2 * waves <= lds_bytes && rows * tokens * 4 * (kParts - 1) <= lds_bytes && lds_bytes <= 160 * 1024, "what a compute unit has");
 };
 
 // The tile that a workgroup takes.  Workgroups go to the eight XCDs in turn, and those of one get tiles that lie
@@ -426,51 +426,77 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * 
     const uint32_t to = lds_at + side * M::step_bytes;
     const int step = min(first_step + turn, steps - 1), last = blocks - 1 - 4 * step;
     const uint8_t *w_from = code_tile + step * 64, *x_from = x_tile + step * 128;
+    auto fetch_all = [&](auto whole) {
 #pragma unroll
-    for (int i = 0; i < kWFetches; i++)
-      mx4::fetch(w_from, w_at[i] - max(w_part - last, 0) * kBlockBytes, to + min(i * kWaves + wave, kWAll - 1) * 1024);
+      for (int i = 0; i < kWFetches; i++)
+        mx4::fetch(w_from, decltype(whole)::value ? w_at[i] : w_at[i] - max(w_part - last, 0) * kBlockBytes, to + min(i * kWaves + wave, kWAll - 1) * 1024);
 #pragma unroll
-    for (int i = 0; i < kXFetches; i++)
-      mx4::fetch(x_from, x_at[i] - max((x_part[i] >> 1) - last, 0) * kBlock, to + M::w_bytes + min(i * kWaves + wave, kXAll - 1) * 1024);
+      for (int i = 0; i < kXFetches; i++)
+        mx4::fetch(x_from, decltype(whole)::value ? x_at[i] : x_at[i] - max((x_part[i] >> 1) - last, 0) * kBlock,
+                   to + M::w_bytes + min(i * kWaves + wave, kXAll - 1) * 1024);
+    };
+    if (last >= 3)
+      fetch_all(std::true_type());
+    else
+      fetch_all(std::false_type());
   };
-  // This thread's pieces of the scales of M::chunk turns, sixteen blocks of a row or token each, as two eights, each from its first
-  // block on or the row's last eight, of a row of fewer those at the top; what is left over repeats the last.
+  // This thread's pieces of the scales of M::chunk turns, sixteen blocks of a row or token each, as two eights, each from
+  // its first block on or the row's last eight, of a row of fewer those at the top; what is left over repeats the last.
   constexpr int kOfRow = M::chunk / 4, kAllPieces = M::scale_rows * kOfRow, kPieces = (kAllPieces + 64 * kWaves - 1) / (64 * kWaves);
-  uint64_t scales[kPieces][2];
-  auto piece_of = [&](int j) { return min(j * 64 * kWaves + tid, kAllPieces - 1); };
+  u32x4 scales[kPieces];
+  const uint8_t *scale_row[kPieces];
+  uint32_t *const scale_lds = reinterpret_cast<uint32_t *>(lds) + M::scales_at / 4;
+  uint32_t *scale_to[kPieces];
+#pragma unroll
+  for (int j = 0; j < kPieces; j++) {
+    const int piece = min(j * 64 * kWaves + tid, kAllPieces - 1), row = piece / kOfRow;
+    scale_row[j] = row < M::rows ? p.scales + static_cast<int64_t>(min(row0 + row, p.height - 1)) * blocks
+                                 : p.x_scales + static_cast<int64_t>(min(token0 + row - M::rows, p.tokens - 1)) * blocks;
+    scale_to[j] = scale_lds + 4 * (piece % kOfRow) * M::scale_rows + row;
+  }
+  auto first_of = [&](int j, int turn) { return 4 * (first_step + turn) + 16 * (kOfRow == 1 ? 0 : min(j * 64 * kWaves + tid, kAllPieces - 1) % kOfRow); };
+  auto whole_chunk = [&](int turn) { return 4 * (first_step + turn) + 16 * kOfRow <= blocks; };
   auto load_scales = [&](int turn) {
+    if (whole_chunk(turn)) {
 #pragma unroll
-    for (int j = 0; j < kPieces; j++) {
-      const int piece = piece_of(j), row = piece / kOfRow, first = 4 * (first_step + turn) + 16 * (piece % kOfRow);
-      const uint8_t *from = row < M::rows ? p.scales + static_cast<int64_t>(min(row0 + row, p.height - 1)) * blocks
-                                          : p.x_scales + static_cast<int64_t>(min(token0 + row - M::rows, p.tokens - 1)) * blocks;
-      if (blocks >= 8) {
+      for (int j = 0; j < kPieces; j++) __builtin_memcpy(&scales[j], scale_row[j] + first_of(j, turn), 16);
+    } else if (blocks >= 8) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) __builtin_memcpy(&scales[j][i], from + min(first + 8 * i, blocks - 8), 8);
-      } else {
+      for (int j = 0; j < kPieces; j++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          u32x2 eight;
+          __builtin_memcpy(&eight, scale_row[j] + min(first_of(j, turn) + 8 * i, blocks - 8), 8);
+          scales[j][2 * i] = eight[0], scales[j][2 * i + 1] = eight[1];
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPieces; j++) {
         uint64_t all = 0;
 #pragma unroll
         for (int b = 0; b < 7; b++) {
-          const uint64_t scale = from[min(b, blocks - 1)];
+          const uint64_t scale = scale_row[j][min(b, blocks - 1)];
           if (b < blocks) all = all >> 8 | scale << 56;
         }
-        scales[j][0] = scales[j][1] = all;
+        scales[j][0] = scales[j][2] = static_cast<uint32_t>(all), scales[j][1] = scales[j][3] = static_cast<uint32_t>(all >> 32);
       }
     }
   };
-  uint32_t *const scale_lds = reinterpret_cast<uint32_t *>(lds) + M::scales_at / 4;
   auto put_scales = [&](int turn) {   // zeros behind the row's last; of each turn the rows back to back
+    const bool whole = whole_chunk(turn);
 #pragma unroll
     for (int j = 0; j < kPieces; j++) {
-      const int piece = piece_of(j), row = piece / kOfRow, first = 4 * (first_step + turn) + 16 * (piece % kOfRow);
-      uint32_t *to = scale_lds + ((turn & M::chunk) + 4 * (piece % kOfRow)) * M::scale_rows + row;
+      uint32_t *to = scale_to[j] + (turn & M::chunk) * M::scale_rows;
+      if (!whole) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const int behind = max(first + 8 * i + 8 - blocks, 0);
-        const uint64_t v = behind < 8 ? scales[j][i] >> 8 * behind : 0;
-        to[2 * i * M::scale_rows] = static_cast<uint32_t>(v);
-        to[(2 * i + 1) * M::scale_rows] = static_cast<uint32_t>(v >> 32);
+        for (int i = 0; i < 2; i++) {
+          const int behind = max(first_of(j, turn) + 8 * i + 8 - blocks, 0);
+          const uint64_t v = behind < 8 ? (static_cast<uint64_t>(scales[j][2 * i + 1]) << 32 | scales[j][2 * i]) >> 8 * behind : 0;
+          scales[j][2 * i] = static_cast<uint32_t>(v), scales[j][2 * i + 1] = static_cast<uint32_t>(v >> 32);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < 4; i++) to[i * M::scale_rows] = scales[j][i];
     }
   };
 
@@ -504,11 +530,11 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * 
   // were.
   int side = 0, ahead = kStages - 1;
   auto turn = [&](auto in_chunk, int t) {
-    mx4::meet<(kStages - 2) * (kWFetches + kXFetches)>();   // but for the codes that later turns asked for
-    if (decltype(in_chunk)::value == M::chunk - 2) {
-      put_scales(t + 2);
-      load_scales(t + 2 + M::chunk);
-    }
+    if (decltype(in_chunk)::value == 0 && t == 0)
+      mx4::meet<63>();   // (waited for already)
+    else
+      mx4::meet<(kStages - 2) * (kWFetches + kXFetches)>();   // but for the codes that later turns asked for
+    if (decltype(in_chunk)::value == M::chunk - 2) put_scales(t + 2);
     fetch_step(ahead, t + kStages - 1);
     __builtin_amdgcn_sched_barrier(0);
     const uint32_t *from = scale_lds + (t & (2 * M::chunk - 1)) * M::scale_rows + in_tile;
@@ -517,15 +543,18 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * 
 #pragma unroll
     for (int n = 0; n < kTokens; n++) bs[n] = static_cast<int>(from[M::rows + (token_side * kTokens + n) * 32] >> (8 * half));
     multiply(side, std::integral_constant<int, 0>{});
+    if (decltype(in_chunk)::value == M::chunk - 2) load_scales(t + 2 + M::chunk);
     multiply(side, std::integral_constant<int, 1>{});
     side = side == kStages - 1 ? 0 : side + 1;
     ahead = ahead == kStages - 1 ? 0 : ahead + 1;
   };
-  load_scales(0);
+  load_scales(0);   // (with the first codes: one trip to memory)
+  fetch_step(0, 0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   put_scales(0);
   load_scales(M::chunk);
 #pragma unroll
-  for (int i = 0; i < kStages - 1; i++) fetch_step(i, i);
+  for (int i = 1; i < kStages - 1; i++) fetch_step(i, i);
   int t = 0;
   for (;;) {
     turn(std::integral_constant<int, 0>{}, t);
@@ -551,25 +580,25 @@ __global__ __launch_bounds__(64 * kRowSides * kTokenSides * kParts, kRowSides * 
   if constexpr (kParts > 1) {   // the parts' sums, added in their order
     f32x4 *const place_of = reinterpret_cast<f32x4 *>(all_lds) + tid;
     constexpr int kFours = 4 * kRows * kTokens;
-    for (int other = 1; other < kParts; other++) {
-      if (part == other) {
+    if (part) {
 #pragma unroll
-        for (int i = 0; i < kFours; i++) {
-          const f32x16 &v = sum[i / 4 / kTokens][i / 4 % kTokens];
-          place_of[i * 64 * kWaves] = f32x4{v[i % 4 * 4], v[i % 4 * 4 + 1], v[i % 4 * 4 + 2], v[i % 4 * 4 + 3]};
-        }
+      for (int i = 0; i < kFours; i++) {
+        const f32x16 &v = sum[i / 4 / kTokens][i / 4 % kTokens];
+        place_of[((part - 1) * kFours + i) * 64 * kWaves] = f32x4{v[i % 4 * 4], v[i % 4 * 4 + 1], v[i % 4 * 4 + 2], v[i % 4 * 4 + 3]};
       }
-      __syncthreads();
-      if (part == 0) {
+    }
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int other = 0; other < kParts - 1; other++)
 #pragma unroll
         for (int i = 0; i < kFours; i++) {
-          const f32x4 v = place_of[i * 64 * kWaves];
+          const f32x4 v = place_of[(other * kFours + i) * 64 * kWaves];
 #pragma unroll
           for (int k = 0; k < 4; k++) sum[i / 4 / kTokens][i / 4 % kTokens][i % 4 * 4 + k] += v[k];
         }
-      }
-      __syncthreads();
     }
+    __syncthreads();   // (y goes past the same memory)
     if (part) return;
   }
 
