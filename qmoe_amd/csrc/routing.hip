@@ -344,21 +344,18 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
   // experts again.
   constexpr int kTop = kPer < 3 ? kPer : 3;
   uint32_t top[kTop];
-  auto look = [&](uint32_t below) {
+  auto look = [&](auto all, uint32_t below) {   // of all keys, or those below
 #pragma unroll
     for (int i = 0; i < kTop; i++) top[i] = 0;
 #pragma unroll
     for (int j = 0; j < kPer; j++) {
-      uint32_t k = key[j] < below ? key[j] : 0;
+      const uint32_t k = decltype(all)::value || key[j] < below ? key[j] : 0;
 #pragma unroll
-      for (int i = 0; i < kTop; i++) {
-        const uint32_t less = min(top[i], k);
-        top[i] = max(top[i], k);
-        k = less;
-      }
+      for (int i = kTop - 1; i > 0; i--) top[i] = max(min(top[i - 1], top[i]), min(max(top[i - 1], top[i]), k));   // the one in the middle
+      top[0] = max(top[0], k);
     }
   };
-  look(~0u);
+  look(std::true_type(), 0);
   // places[i] is the i-th found; behind top_k as long as the next may belong before it
   int found = 0, given = 0;
   uint32_t least = 0;
@@ -385,7 +382,7 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
     }
     if (kTop < kPer && __ballot(mine && given == kTop)) {
       if (mine && given == kTop) {
-        look(m);
+        look(std::false_type(), m);
         given = 0;
       }
     }
