@@ -190,7 +190,7 @@ __device__ __forceinline__ float value32(uint32_t rank) {
 // last than there are lanes) and what is no number goes to the exact form.  A lane has experts of one group, as many
 // together as 16 bytes of logits hold, then those behind the group's other lanes', kPer in all.  An expert's key is its
 // rank with j in the last bits, so that the largest key says which it is.
-template <class T, int kLanes, int kPer>
+template <class T, int kLanes, int kPer, bool kSigmoid, bool kBias>
 __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token) {
   __shared__ uint16_t all_places[256];
   uint16_t *const places = all_places + (threadIdx.x & ~(kLanes - 1));   // of this token
@@ -217,7 +217,7 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
 #pragma unroll
     for (int i = 0; i < kTogether; i++) v[j + i] = static_cast<float>(some[i]);
   }
-  if (a.bias) {
+  if constexpr (kBias) {
 #pragma unroll
     for (int j = 0; j < kPer; j += kTogether) {
       float some[kTogether] = {};
@@ -235,10 +235,10 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
   bool odd = false;   // something that the exact form has to look at
   float most = 0, largest_score = 1;
   double under = 1;
-  const bool approximate = a.bias != nullptr;
+  constexpr bool approximate = kBias;
   const int limit = in_group ? size : 0;
   auto there = [&](int j) { return at_of(j) < limit; };
-  if (!a.sigmoid) {
+  if (!kSigmoid) {
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kPer; j++) m = there(j) ? fmaxf(m, v[j]) : m;
@@ -253,18 +253,19 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
   }
   const float over = largest_score;
   auto score32 = [&](float l) {
-    return a.sigmoid ? __builtin_amdgcn_rcpf(1 + __builtin_amdgcn_exp2f(-l * kLog2e)) : __builtin_amdgcn_exp2f((l - most) * kLog2e) * over;
+    return kSigmoid ? __builtin_amdgcn_rcpf(1 + __builtin_amdgcn_exp2f(-l * kLog2e)) : __builtin_amdgcn_exp2f((l - most) * kLog2e) * over;
   };
   // How far apart two sums of scores and biases near `c` may be taken for when they are not.  A sigmoid is off by less
   // than 2^-22 (its argument's rounding, at most 1.5 |l| 2^-24 s (1 - s), the exponential's and the quotient's steps),
   // a share by less than 2^-20 of the largest (|l - most| e^(l - most) is at most 0.37; a sum over 4096 is off by 2^-20
   // of itself); a mark has two of them, a sum's steps are 2^-24 c.
-  auto tolerance = [&](float c) { return (a.sigmoid ? 0x1p-20f : 0x1p-18f * largest_score) + 0x1p-21f * fabsf(c); };
+  auto tolerance = [&](float c) { return (kSigmoid ? 0x1p-20f : 0x1p-18f * largest_score) + 0x1p-21f * fabsf(c); };
   auto exact_score = [&](float l) {
-    return a.sigmoid ? 1 / (1 + exp(-static_cast<double>(l))) : exp(static_cast<double>(l) - most) / under;
+    return kSigmoid ? 1 / (1 + exp(-static_cast<double>(l))) : exp(static_cast<double>(l) - most) / under;
   };
   auto sum_exactly = [&] {
     double sum = 0;
+#pragma unroll 1   // (seldom, and long)
     for (int j = 0; j < kPer; j++)
       if (there(j)) sum += exp(static_cast<double>(logit_at<T>(row, base + at_of(j))) - most);
     under = sum_over<kLanes>(sum);
@@ -274,20 +275,21 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
   uint32_t key[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; j++) {
-    float c = v[j];
-    if (approximate) {
-      c = score32(v[j]) + b[j];
-      odd |= there(j) && !(fabsf(c) < INFINITY);
-    }
-    odd |= there(j) && c != c;
-    key[j] = there(j) ? (rank32(c) & ~kIndex) | (kIndex - j) : 0;
-    if (by_marks) {
-      v[j] = there(j) ? (!approximate && marks_of_scores ? score32(v[j]) : c) : -INFINITY;
-      two = fmaxf(two, fminf(one, v[j]));
-      one = fmaxf(one, v[j]);
-    }
+    if (approximate) v[j] = score32(v[j]) + b[j];
+    odd |= there(j) && (approximate ? !(fabsf(v[j]) < INFINITY) : v[j] != v[j]);
+    key[j] = there(j) ? (rank32(v[j]) & ~kIndex) | (kIndex - j) : 0;
   }
   if (by_marks) {
+    if (!approximate && marks_of_scores) {
+#pragma unroll
+      for (int j = 0; j < kPer; j++) v[j] = score32(v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+      const float c = there(j) ? v[j] : -INFINITY;
+      two = fmaxf(two, fminf(one, c));
+      one = fmaxf(one, c);
+    }
     for (int by = 1; by < group_lanes; by *= 2) {
       const float other_one = __shfl_xor(one, by, kLanes), other_two = __shfl_xor(two, by, kLanes);
       two = fmaxf(fmaxf(two, other_two), fminf(one, other_one));
@@ -312,7 +314,7 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
     if (marks_of_scores) {
       const float kept = value32(last), next = value32(largest_over<kLanes>(taken ? 0 : rank));
       if (__ballot(!odd && !(next < kept - tolerance(kept)))) {   // too close: marks in 64 bits, of the experts that may be in them
-        if (!a.sigmoid) sum_exactly();
+        if (!kSigmoid) sum_exactly();
         const float least = of_two ? two : one;
         const float from = least - tolerance(least);
         uint64_t look = 0;
@@ -359,6 +361,7 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
   // places[i] is the i-th found; behind top_k as long as the next may belong before it
   int found = 0, given = 0;
   uint32_t least = 0;
+#pragma unroll 1
   for (int i = 0; i < kLanes; i++) {
     const uint32_t best = top[0], m = largest_over<kLanes>(best);
     bool more = i < a.top_k;
@@ -416,7 +419,7 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
         }
       }
     }
-    if (again || a.sigmoid || !approximate || !__ballot(close && !odd)) break;
+    if (again || kSigmoid || !approximate || !__ballot(close && !odd)) break;
     sum_exactly();
     score = exact_score(l);
   }
@@ -432,14 +435,14 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
   return true;
 }
 
-template <class T, int kLanes, int kPer>
+template <class T, int kLanes, int kPer, bool kSigmoid, bool kBias>
 __global__ __launch_bounds__(256) void route_quick_kernel(const RouteArgs a) {
   constexpr int kTokens = 64 / kLanes;   // of a wavefront
   const int64_t first = (blockIdx.x * int64_t{4} + (threadIdx.x >> 6)) * kTokens;
   if (first >= a.tokens) return;
   const int64_t token = first + (threadIdx.x & 63) / kLanes;
   // tokens that are not there repeat the last
-  const uint64_t done = __ballot(route_quickly<T, kLanes, kPer>(a, token < a.tokens ? token : a.tokens - 1));
+  const uint64_t done = __ballot(route_quickly<T, kLanes, kPer, kSigmoid, kBias>(a, token < a.tokens ? token : a.tokens - 1));
   if (done == ~uint64_t{0}) return;
   for (int i = 0; i < kTokens && first + i < a.tokens; i++)
     if (!(done >> (i * kLanes) & 1)) route_exactly<T>(a, first + i);
@@ -448,7 +451,14 @@ __global__ __launch_bounds__(256) void route_quick_kernel(const RouteArgs a) {
 template <class T, int kLanes, int kPer>
 void launch_quick(const RouteArgs &a, hipStream_t s) {
   constexpr int kTokens = 4 * 64 / kLanes;
-  route_quick_kernel<T, kLanes, kPer><<<static_cast<unsigned>((a.tokens + kTokens - 1) / kTokens), 256, 0, s>>>(a);
+  const unsigned grid = static_cast<unsigned>((a.tokens + kTokens - 1) / kTokens);
+  if (a.sigmoid) {
+    if (a.bias) route_quick_kernel<T, kLanes, kPer, true, true><<<grid, 256, 0, s>>>(a);
+    else route_quick_kernel<T, kLanes, kPer, true, false><<<grid, 256, 0, s>>>(a);
+  } else {
+    if (a.bias) route_quick_kernel<T, kLanes, kPer, false, true><<<grid, 256, 0, s>>>(a);
+    else route_quick_kernel<T, kLanes, kPer, false, false><<<grid, 256, 0, s>>>(a);
+  }
 }
 
 template <class T>
