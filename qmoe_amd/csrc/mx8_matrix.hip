@@ -354,12 +354,13 @@ void launch_few(const Product8Args &p, hipStream_t s) {
 // v_mfma_scale_f32_32x32x64_f8f6f4 takes lane l's block l / 32 of row l % 32 as it is, of token l % 32 the 16 values
 // from 16 (l / 32) on and the 16 from 32 + 16 (l / 32) on, and each side's scale for block l / 32 as one byte of a
 // register.  Scales come through registers, sixteen (four steps') of a row or token a thread, and LDS: loaded by each
-// wavefront for itself they were two of three requests to L2, which bound the launch. 8192 tokens through 2080 x 6144
-// take 89 us (2.3 PFLOP/s), through 8192 x 8192 420 (2.6); matrix cores are busy for 58 % of the launch at clocks that
-// power holds at 2.0 GHz.  Without the fetches of codes it took 22 % less, without scales 11, without y's stores 9; 256
-// x 256 with operands read ahead by 8 wavefronts 97 where 16 wavefronts without took 84 (2048 rows), three stages as
-// two; two steps a turn, fetches after the first products, a higher priority for wavefronts in their products: within 2
-// %.
+// wavefront for itself they were two of three requests to L2, which bound the launch.  8192 tokens through 2080 x 6144
+// take 90 us a call (2.3 PFLOP/s), through 8192 x 8192 410 to 420 in a graph (2.6); of zeros 70 and 300: power is the
+// bound, matrix cores are busy for three quarters of the loop's cycles at 1.7 to 2.0 GHz. Without the fetches of codes
+// it took 22 % less, without scales 11, without y's stores 9; 256 x 256 by 8 wavefronts as by 16 within 2 %, three
+// stages as two; two steps a turn, fetches after the first products, a higher priority for wavefronts in their
+// products: within 2 %. Smaller calls are bound by what a compute unit moves from L2 into LDS: 28 to 30 bytes a cycle,
+// of 35 that loads alone reach (568 tokens through 2080 x 6144: 153 tiles of 768 KB, 19.8 us).
 template <int kRows, int kTokens, int kRowSides, int kTokenSides, int kParts, int kStages>
 struct Many8 {
   static constexpr int waves = kRowSides * kTokenSides, rows = 32 * kRows * kRowSides, tokens = 32 * kTokens * kTokenSides;
