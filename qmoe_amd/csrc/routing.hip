@@ -249,6 +249,7 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
     for (int j = 0; j < kPer; j++)
       sum[j % 4] += static_cast<double>(there(j) ? __builtin_amdgcn_exp2f((v[j] - most) * kLog2e) : 0.0f);
     under = sum_over<kLanes>((sum[0] + sum[1]) + (sum[2] + sum[3]));
+    if (most == -INFINITY) most = 0, under = 1;   // all of them masked: scores of zero
     largest_score = static_cast<float>(1 / under);
     odd |= !(fabsf(most) < INFINITY);
   }
@@ -269,7 +270,8 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
 #pragma unroll 1   // (seldom, and long)
     for (int j = 0; j < kPer; j++)
       if (there(j)) sum += exp(static_cast<double>(logit_at<T>(row, base + at_of(j))) - most);
-    under = sum_over<kLanes>(sum);
+    sum = sum_over<kLanes>(sum);
+    under = sum == 0 ? 1 : sum;
   };
   float one = -INFINITY, two = -INFINITY;   // the lane's best of its group, for the group's mark
   const bool by_marks = a.top_groups < a.groups, marks_of_scores = approximate || a.group_mark == 2;
@@ -359,22 +361,46 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
     }
   };
   look(std::true_type(), 0);
-  // places[i] is the i-th found; behind top_k as long as the next may belong before it
-  int found = 0, given = 0;
-  uint32_t least = 0;
-#pragma unroll 1
-  for (int i = 0; i < kLanes; i++) {
-    const uint32_t best = top[0], m = largest_over<kLanes>(best);
-    bool more = i < a.top_k;
-    if (i == a.top_k - 1) least = m & ~kIndex;
-    if (!more && m) {
-      const float kept = value32(least), next = value32(m & ~kIndex);
-      more = approximate ? !(next < kept - tolerance(kept) - kPer * 0x1p-22f * fabsf(kept)) : (m & ~kIndex) == least;
+  auto slack = [&](float c) { return tolerance(c) + kPer * 0x1p-22f * fabsf(c); };   // with what the keys leave out
+  // Whether those of a rank are equal, not only near each other: of equal logits and biases, and all others clear of them.
+  auto equal_ones = [&](uint32_t rank) {
+    uint64_t left = 0;
+    uint32_t below = 0, above = ~0u;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+      const uint32_t k = key[j] & ~kIndex;
+      left |= static_cast<uint64_t>(k == rank) << j;
+      if (approximate) {
+        below = max(below, k < rank ? k : 0u);
+        above = min(above, k > rank ? k : ~0u);
+      }
     }
-    if (!__ballot(more)) break;
-    const uint32_t e = static_cast<uint32_t>(base + at_of(static_cast<int>(kIndex - (best & kIndex))));
-    bool mine = best == m;   // (of a token that has none left all of them)
-    if (__popcll(__ballot(mine)) != 64 / kLanes) {   // of equal ones the lower
+    uint32_t most_l = 0, least_l = ~0u, most_b = 0, least_b = ~0u;
+    while (__ballot(left != 0)) {
+      if (left) {
+        const int e = base + at_of(__ffsll(static_cast<unsigned long long>(left)) - 1);
+        const uint32_t l = rank32(logit_at<T>(row, e)), c = approximate ? rank32(a.bias[e]) : 0;
+        most_l = max(most_l, l), least_l = min(least_l, l);
+        most_b = max(most_b, c), least_b = min(least_b, c);
+        left &= left - 1;
+      }
+    }
+    bool equal = largest_over<kLanes>(most_l) == smallest_over<kLanes>(least_l);
+    if (approximate) {
+      const float kept = value32(rank), far = slack(kept);
+      below = largest_over<kLanes>(below), above = smallest_over<kLanes>(above);
+      equal &= (below == 0 || value32(below) < kept - far) && (above == ~0u || value32(above) > kept + far);
+      most_b = largest_over<kLanes>(most_b), least_b = smallest_over<kLanes>(least_b);
+      equal &= most_b == least_b;
+    }
+    return equal;
+  };
+  // places[i] is the i-th found, of a rank the lower first; behind top_k as long as the next may belong before it
+  int given = 0;
+  auto take = [&](int i, uint32_t m, bool more) {
+    const uint32_t best = top[0], e = static_cast<uint32_t>(base + at_of(static_cast<int>(kIndex - (best & kIndex))));
+    bool mine = (best ^ m) <= kIndex;   // (of a token that has none left all of them)
+    if (__popcll(__ballot(mine)) != 64 / kLanes) {
       const uint32_t lowest = smallest_over<kLanes>(mine ? e : ~0u);
       mine &= e == lowest;
     }
@@ -386,12 +412,33 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
     }
     if (kTop < kPer && __ballot(mine && given == kTop)) {
       if (mine && given == kTop) {
-        look(std::false_type(), m);
+        look(std::false_type(), best);
         given = 0;
       }
     }
-    if (more) found = i + 1;
-    odd |= i == kLanes - 1;
+  };
+  uint32_t m = 0;
+#pragma unroll 1
+  for (int i = 0; i < a.top_k; i++) {
+    m = largest_over<kLanes>(top[0]);
+    take(i, m, true);
+  }
+  int found = a.top_k;
+  const uint32_t least = m & ~kIndex;
+  const float near = value32(least) - slack(value32(least));
+  auto may_belong = [&] { return m != 0 && (approximate ? !(value32(m & ~kIndex) < near) : (m & ~kIndex) == least); };
+  m = largest_over<kLanes>(top[0]);
+  if (__ballot(may_belong())) {
+    const bool settled = equal_ones(least);
+#pragma unroll 1
+    for (int i = a.top_k; i < kLanes; i++) {
+      const bool more = !settled && may_belong();
+      if (!__ballot(more)) break;
+      take(i, m, more);
+      if (more) found = i + 1;
+      odd |= i == kLanes - 1;
+      m = largest_over<kLanes>(top[0]);
+    }
   }
   sub1::wave_lds_fence();
 

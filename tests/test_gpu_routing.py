@@ -168,6 +168,33 @@ def test_equal_ones_beside_rows_with_fewer_numbers(experts, top_k):
         assert np.array_equal(index.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize('scores', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('experts,top_k,groups,top_groups', [(40, 3, 1, 1), (128, 1, 1, 1), (256, 8, 8, 4), (512, 12, 1, 1), (500, 7, 4, 2), (2048, 2, 1, 1), (4096, 20, 1, 1)])
+@pytest.mark.parametrize('tokens', [70, 2604])
+def test_many_equal_ones(tokens, experts, top_k, groups, top_groups, scores):
+    """Rows of padding (all equal), coarse logits, such that differ in their last bits alone: equal ones by the lower index,
+    others as they are, with no bias, one of zeros and one of few values."""
+    g = gen(experts + tokens)
+    logits = torch.randn((tokens, experts), generator=g)
+    logits[::2] = 0
+    logits[1::8] = (2 * logits[1::8]).round() / 2
+    logits[3::8] = 1 + torch.randint(0, 3, logits[3::8].shape, generator=g) * 2.0 ** -23
+    logits[5::16, experts // 3:] = -2.5
+    logits = logits.cuda()
+    for bias in (None, torch.zeros(experts).cuda(), torch.randint(0, 2, (experts,), generator=g).float().cuda() / 4):
+        for group_mark in (1, 2):
+            check_many(logits, top_k, scores, bias, groups, top_groups, group_mark, True)
+    some = logits[:40].clone()
+    some[7:, ::3] = -float('inf')                             # masked in part, and whole
+    some[20:30] = -float('inf')
+    some[31, 1:] = -float('inf')
+    for bias in (None, torch.zeros(experts).cuda()):
+        want = check(some, top_k, scores, bias, groups, top_groups, 2, True)
+        got = routing.route(some.repeat(-(-tokens // 40), 1), top_k, scores, bias, groups, top_groups, 2, True)
+        assert torch.equal(got[1], want[1].repeat(-(-tokens // 40), 1))
+        assert torch.allclose(got[0], want[0].repeat(-(-tokens // 40), 1), rtol=1e-5, atol=0)
+
+
 def test_shapes_of_routing():
     logits = torch.randn((3, 5, 40), generator=gen(3)).cuda()
     shares, index = routing.route(logits, 2)
