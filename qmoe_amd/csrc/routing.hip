@@ -182,15 +182,16 @@ __device__ __forceinline__ float value32(uint32_t rank) {
 }
 
 // kLanes lanes a token, kPer experts a lane; one read of the logits.  Bound by instructions and their latency, not by
-// memory: 8192 tokens' 8 of 256 in groups, with a bias, 8.6 us a call (9.2 MB would take 2), of which the choice of
-// groups takes 1.4, the eight choices 2.2, the bias and its scores 0.9, the rest a launch, the logits' trip and a look
-// at the chosen ones'; one token's kernel 2.1.  A kernel for each kind of scores, with and without a bias: 9.7 in a
+// memory: 8192 tokens' 8 of 256 in groups, with a bias, 8.0 us a call (9.2 MB would take 2), of which the choice of
+// groups takes 1.9, the eight choices 1.4, the bias and its scores 1.6, the rest a launch, the logits' trip and a look
+// at the chosen ones'; one token's kernel 2.0.  A kernel for each kind of scores, with and without a bias: 9.7 in a
 // graph, 11.6 where both were asked for at run time.  Scores are computed in 32 bits, which places all experts but
 // those next to each other; from there are taken the top_k and on as long as the next may be one of them for all that
-// is known, and of those alone the order is found in 64 bits.  What that leaves open (marks of groups too close to
-// tell, more near the last than there are lanes) and what is no number goes to the exact form.  A lane has experts of
-// one group, as many together as 16 bytes of logits hold, then those behind the group's other lanes', kPer in all.  An
-// expert's key is its rank with j in the last bits, so that the largest key says which it is.
+// is known, and of those alone the order is found in 64 bits; where they are equal to the last bit (padding, coarse
+// logits) the lower indexes are the answer, and no more are looked at.  What that leaves open (marks of groups too
+// close to tell, more near the last than there are lanes) and what is no number goes to the exact form.  A lane has
+// experts of one group, as many together as 16 bytes of logits hold, then those behind the group's other lanes', kPer
+// in all.  An expert's key is its rank with j in the last bits, so that the largest key says which it is.
 template <class T, int kLanes, int kPer, bool kSigmoid, bool kBias>
 __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token) {
   __shared__ uint16_t all_places[256];
@@ -519,10 +520,10 @@ int launch_route(RouteArgs a, hipStream_t s) {
     return of_group ? (a.experts / a.groups + of_group - 1) / of_group : 1 << 30;
   };
   // A wavefront for four tokens where there are several for every SIMD, else for one (us in a graph: 8192 tokens' 8 of
-  // 256 in groups, a bias, 9.6 and 13.7; 8 of 512, softmax, a bias 11.1 and 13.4; 4096 tokens' 2 of 128 4.1 and 4.5; 2048
-  // tokens' 8 of 256 in groups 7.2 and 7.0, 8 of 512 7.9 and 6.3, 1 of 128 3.8 and 3.7).
+  // 256 in groups, a bias, 9.1 and 12.3; 8 of 512, softmax 8.9 and 10.8; 1 of 128 4.1 and 5.6; 3000 tokens 7.3 and 7.4,
+  // 7.2 and 6.2, 3.7 and 4.0; 4096 tokens' 8 of 512 7.5 both; 2048 tokens' 7.1 and 6.0, 7.2 and 5.4, 3.7 and 3.6).
   const int per16 = per(16), per64 = per(64);
-  if (a.tokens > 2500 && per16 <= 32 && a.top_k <= 12) {
+  if (a.tokens > (per16 <= 16 ? 2500 : 4096) && per16 <= 32 && a.top_k <= 12) {
     sub1::note_kernel("route_quick_kernel, 16 lanes a token");
     if (per16 <= 1) launch_quick<T, 16, 1>(a, s);
     else if (per16 <= 2) launch_quick<T, 16, 2>(a, s);
