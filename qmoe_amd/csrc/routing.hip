@@ -188,10 +188,11 @@ __device__ __forceinline__ float value32(uint32_t rank) {
 // graph, 11.6 where both were asked for at run time.  Scores are computed in 32 bits, which places all experts but
 // those next to each other; from there are taken the top_k and on as long as the next may be one of them for all that
 // is known, and of those alone the order is found in 64 bits; where they are equal to the last bit (padding, coarse
-// logits) the lower indexes are the answer, and no more are looked at.  What that leaves open (marks of groups too
-// close to tell, more near the last than there are lanes) and what is no number goes to the exact form.  A lane has
-// experts of one group, as many together as 16 bytes of logits hold, then those behind the group's other lanes', kPer
-// in all.  An expert's key is its rank with j in the last bits, so that the largest key says which it is.
+// logits) the lower indexes are the answer, and no more are looked at.  Groups' marks too close to tell are computed
+// again in 64 bits, of the experts that may be in them. What is still open (more near the last than there are lanes)
+// and what is no number goes to the exact form.  A lane has experts of one group, as many together as 16 bytes of
+// logits hold, then those behind the group's other lanes', kPer in all.  An expert's key is its rank with j in the last
+// bits, so that the largest key says which it is.
 template <class T, int kLanes, int kPer, bool kSigmoid, bool kBias>
 __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token) {
   __shared__ uint16_t all_places[256];
@@ -346,8 +347,8 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
     for (int j = 0; j < kPer; j++) key[j] = taken ? key[j] : 0;
   }
 
-  // The lane's largest keys, the largest first: a choice takes one off, and only a lane that has given all of them goes through its
-  // experts again.
+  // The lane's largest keys, the largest first: a choice takes one off, and only a lane that has given all of them goes
+  // through its experts again.
   constexpr int kTop = kPer < 3 ? kPer : 3;
   uint32_t top[kTop];
   auto look = [&](auto all, uint32_t below) {   // of all keys, or those below
