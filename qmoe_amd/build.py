@@ -1,9 +1,11 @@
 """Compiles libsub1_hip.so for gfx950 with hipcc (cross-compiles without a GPU), and
 the Python extension that takes tensors apart for it with g++."""
+import concurrent.futures
 import os
 import re
 import subprocess
 import sysconfig
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -21,9 +23,7 @@ SOURCES = [os.path.join(HERE, 'csrc', 'sub1_kernels.hip'),
            os.path.join(HERE, 'csrc', 'sub1_tables.cpp')]
 
 HIPCC_FLAGS = [
-    '-O3', '--offload-arch=gfx950', '-fPIC', '-shared', '-std=c++17',
-    # the sources side by side: 95 s in place of 200
-    '-parallel-jobs=8',
+    '-O3', '--offload-arch=gfx950', '-fPIC', '-std=c++17',
     # keep the compiler from forming packed fp32 instructions
     '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
     # registers and scratch memory per kernel, read back below
@@ -32,17 +32,30 @@ HIPCC_FLAGS = [
 ]
 
 
+JOBS = 8      # compilers at a time: 95 s in place of 200
+
+
 def kernels_with_scratch(compiler_output):
-    """{kernel: bytes of scratch memory per lane} for the kernels that spill
-    registers, from the compiler's resource-usage remarks."""
-    found, name = {}, None
+    """{kernel: bytes of scratch memory per lane} for the kernels that spill registers, from the
+    compiler's resource-usage remarks on one source.  Raises RuntimeError where these are not a
+    name and a size in turn (lines cut into each other, one of them lost)."""
+    found, name, names, sizes = {}, None, 0, 0
     for line in compiler_output.splitlines():
-        m = re.search(r'remark: Function Name: (\S+)', line)
+        m = re.search(r'remark: Function Name: (\S+) \[-Rpass', line)
         if m:
-            name = m.group(1)
-        m = re.search(r'remark:\s+ScratchSize \[bytes/lane\]: (\d+)', line)
-        if m and name and int(m.group(1)):
-            found[name] = int(m.group(1))
+            if name:
+                raise RuntimeError('no scratch size of kernel %s in the compiler\'s remarks' % name)
+            name, names = m.group(1), names + 1
+        m = re.search(r'remark:\s+ScratchSize \[bytes/lane\]: (\d+) \[-Rpass', line)
+        if m:
+            if not name:
+                raise RuntimeError('a scratch size of no kernel in the compiler\'s remarks')
+            if int(m.group(1)):
+                found[name] = int(m.group(1))
+            name, sizes = None, sizes + 1
+    if not names == sizes == compiler_output.count('Function Name') == compiler_output.count('ScratchSize'):
+        raise RuntimeError('the compiler\'s remarks cannot be read: %d names and %d scratch sizes of %d and %d' % (
+            names, sizes, compiler_output.count('Function Name'), compiler_output.count('ScratchSize')))
     return found
 
 
@@ -84,17 +97,29 @@ def build_library(verbose=False):
     established; the code was restructured to fit)."""
     build_tensor_args()
     hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
-    cmd = [hipcc] + HIPCC_FLAGS + SOURCES + ['-o', LIB_PATH]
-    res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if res.returncode != 0:
-        raise RuntimeError('hipcc failed:\n' + res.stdout)
-    spilling = {k: v for k, v in kernels_with_scratch(res.stdout).items()
-                if v > SPILLS_ACCEPTED.get(k, 0)}
-    if spilling:
-        os.remove(LIB_PATH)
-        raise RuntimeError('kernels that spill registers to scratch memory: %s' % spilling)
+
+    def run(cmd):
+        res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        if res.returncode != 0:
+            raise RuntimeError('hipcc failed:\n' + res.stdout)
+        return res.stdout
+
+    # A compiler each, whose output is read by itself: several that write to one pipe cut each other's lines.
+    with tempfile.TemporaryDirectory() as objects, concurrent.futures.ThreadPoolExecutor(JOBS) as jobs:
+        into = [os.path.join(objects, os.path.basename(source) + '.o') for source in SOURCES]
+        outputs = list(jobs.map(lambda source, o: run([hipcc] + HIPCC_FLAGS + ['-c', source, '-o', o]), SOURCES, into))
+        spilling = {}
+        for source, output in zip(SOURCES, outputs):
+            if source.endswith('.hip') and 'Function Name' not in output:
+                raise RuntimeError('the compiler says nothing about the kernels of ' + source)
+            spilling.update((k, v) for k, v in kernels_with_scratch(output).items() if v > SPILLS_ACCEPTED.get(k, 0))
+        if spilling:
+            if os.path.exists(LIB_PATH):      # what is there is of other sources
+                os.remove(LIB_PATH)
+            raise RuntimeError('kernels that spill registers to scratch memory: %s' % spilling)
+        run([hipcc, '--offload-arch=gfx950', '-fPIC', '-shared'] + into + ['-o', LIB_PATH])
     if verbose:
-        print('\n'.join(l for l in res.stdout.splitlines() if 'kernel-resource-usage' not in l
+        print('\n'.join(l for l in ''.join(outputs).splitlines() if 'kernel-resource-usage' not in l
                         and not l.lstrip().startswith(('|', '^')) and '__global__' not in l))
     return LIB_PATH
 
