@@ -262,7 +262,7 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
   // How far apart two sums of scores and biases near `c` may be taken for when they are not.  A sigmoid is off by less
   // than 2^-22 (its argument's rounding, at most 1.5 |l| 2^-24 s (1 - s), the exponential's and the quotient's steps),
   // a share by less than 2^-20 of the largest (|l - most| e^(l - most) is at most 0.37; a sum over 4096 is off by 2^-20
-  // of itself); a mark has two of them, a sum's steps are 2^-24 c.
+  // of itself); a sum's steps are 2^-24 c.
   auto tolerance = [&](float c) { return (kSigmoid ? 0x1p-20f : 0x1p-18f * largest_score) + 0x1p-21f * fabsf(c); };
   auto exact_score = [&](float l) {
     return kSigmoid ? 1 / (1 + exp(-static_cast<double>(l))) : exp(static_cast<double>(l) - most) / under;
@@ -305,20 +305,21 @@ __device__ __forceinline__ bool route_quickly(const RouteArgs &a, int64_t token)
     odd |= in_group && marks_of_scores && !(fabsf(mark) < INFINITY);
     const uint32_t rank = in_group ? rank32(mark) : 0;
     bool taken = false;
-    uint32_t last = 0;
-    auto pick = [&](auto from) {   // the groups with the largest marks, of equal ones the lower; the last one's mark
-      auto most_of = largest_over<kLanes>(from);
+    auto pick = [&](auto from) {   // the groups with the largest marks, of equal ones the lower
       taken = false;
       for (int i = 0; i < a.top_groups; i++) {
-        most_of = largest_over<kLanes>(taken ? decltype(from)(0) : from);
+        const auto most_of = largest_over<kLanes>(taken ? decltype(from)(0) : from);
         taken |= static_cast<uint32_t>(group) == smallest_over<kLanes>(!taken && from == most_of ? static_cast<uint32_t>(group) : ~0u);
       }
-      return most_of;
     };
-    last = pick(rank);
+    pick(rank);
     if (marks_of_scores) {
-      const float kept = value32(last), next = value32(largest_over<kLanes>(taken ? 0 : rank));
-      if (__ballot(!odd && !(next < kept - tolerance(kept)))) {   // too close: marks in 64 bits, of the experts that may be in them
+      // A mark is off by what its addends are, which may be larger than it (two scores' errors, two sums' roundings, that
+      // of their own sum and one of what follows here): no group taken may be below one not taken.
+      const float off = 0.5f * tolerance(0) + 0x1p-22f * (of_two ? fabsf(one) + fabsf(two) : fabsf(one));
+      const uint32_t kept = smallest_over<kLanes>(taken && in_group ? rank32(mark - off) : ~0u);
+      const uint32_t next = largest_over<kLanes>(!taken && in_group ? rank32(mark + off) : 0);
+      if (__ballot(!odd && !(next < kept))) {   // too close: marks in 64 bits, of the experts that may be in them
         if (!kSigmoid) sum_exactly();
         const float least = of_two ? two : one;
         const float from = least - tolerance(least);
