@@ -131,7 +131,7 @@ class RoutedMLP(nn.Module):
 
     classifier  a module that gives logits [.., E] in bf16, fp16 or fp32 for hidden states [.., d_model]
     experts     sub1.Sub1Experts, E of them
-    The other arguments as in route; `bias` becomes a buffer."""
+    The other arguments as in route; `bias` becomes a buffer, which stays fp32 whatever type the module is brought to."""
 
     def __init__(self, classifier, experts, top_k=2, scores='softmax', bias=None, groups=1, top_groups=None, group_mark=1,
                  normalize=True, scale=1.0):
@@ -147,6 +147,13 @@ class RoutedMLP(nn.Module):
         self.scores, self.normalize, self.scale = scores, bool(normalize), float(scale)
         self.classifier, self.experts = classifier, experts
         self.register_buffer('bias', None if bias is None else bias.detach())
+
+    def _apply(self, fn, *args, **kwargs):
+        bias = self.bias
+        super()._apply(fn, *args, **kwargs)
+        if bias is not None and self.bias.dtype != torch.float32:
+            self.bias = bias.to(self.bias.device)       # moved, with the values that it had
+        return self
 
     def forward(self, hidden, residual=None):
         """hidden bf16 [.., d_model] -> (bf16 like it, residual added where there is one, shares [.., k], index [.., k])"""
