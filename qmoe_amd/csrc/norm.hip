@@ -199,9 +199,8 @@ int launch_rows(const NormArgs &a, hipStream_t s) {
     else launch_lanes<T, R, kResidual, 16, 4>(a, s);
   } else if (a.rows > 4096 && eights <= (in_fp32 ? 4 : 8) * 64) {
     sub1::note_kernel("rms_norm_kernel, a wavefront a row");
-    const int per = (eights + 63) / 64;
-    if (per == 1) launch_lanes<T, R, kResidual, 64, 1>(a, s);
-    else if (per == 2) launch_lanes<T, R, kResidual, 64, 2>(a, s);
+    const int per = (eights + 63) / 64;   // (narrower rows took quarters)
+    if (per == 2) launch_lanes<T, R, kResidual, 64, 2>(a, s);
     else if (per == 3) launch_lanes<T, R, kResidual, 64, 3>(a, s);
     else if (per == 4) launch_lanes<T, R, kResidual, 64, 4>(a, s);
     else if constexpr (sizeof(T) == 2 && sizeof(R) == 2) {
@@ -210,7 +209,7 @@ int launch_rows(const NormArgs &a, hipStream_t s) {
       else launch_lanes<T, R, kResidual, 64, 8>(a, s);
     }
   } else {
-    sub1::note_kernel("rms_norm_kernel, a workgroup a row");
+    sub1::note_kernel(eights <= 4096 ? "rms_norm_kernel, a workgroup a row" : "rms_norm_wide_kernel, a workgroup a row");
     const unsigned grid = static_cast<unsigned>(a.rows);
     if (eights <= 1024) rms_norm_kernel<T, R, kResidual, 0, 1><<<grid, (eights + 63) / 64 * 64, 0, s>>>(a);
     else if (eights <= 2048) rms_norm_kernel<T, R, kResidual, 0, 2><<<grid, 1024, 0, s>>>(a);
