@@ -737,7 +737,7 @@ int sub1_test_mx8_form(int which);
  * Root-mean-square norm of the rows of x [rows, width], the residual's addition before it:
  *   s = x + residual, rounded to the residual's type, to `total` (residual and total both NULL: s = x)
  *   y = s / sqrt(mean(s^2) + eps) * weight
- * y in x's type, or, with y NULL, in 8 bits as above to codes and scales.  Sums in 64 bits, one rounding of y.
+ * y in x's type, or, with y NULL, in 8 bits as above to codes and scales.  Sums in 64 bits, the factor and its products in fp32, then y rounded.
  * Types SUB1_MX4_BF16, _FP16 or _FP32; residual (and total) and weight each in x's or in _FP32.  Strides in elements.
  * y may be x and total the residual, of the same strides; otherwise results overlap nothing.  eps is at least
  * SUB1_NORM_LEAST_EPS.

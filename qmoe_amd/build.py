@@ -32,7 +32,7 @@ HIPCC_FLAGS = [
 ]
 
 
-JOBS = 8      # compilers at a time: 95 s in place of 200
+JOBS = 8      # compilers at a time: 95 to 110 s in place of 200
 
 
 def kernels_with_scratch(compiler_output):

@@ -90,7 +90,8 @@ __device__ __forceinline__ i32x8 operand(u32x4 a, u32x4 b) {
 // does; the token waits in LDS as bf16 (exact: an e4m3 has four bits), its scales beside it.  A block's 32 products are
 // added without scales, then brought to the power of two of both, so that no value leaves a type's range on the way.
 // For a result in 8 bits a workgroup has the 32 rows of a block.  Reads 17 bytes for 32 products, so HBM would bound it
-// (2080 x 6144: 6.8 MB, 1.4 us); it takes 3.8 us, 2.2 of them an empty launch's, the rest two trips to memory.
+// (2080 x 6144: 6.8 MB, 1.4 us); it takes 3.8 us, 2.2 of them an empty launch's, the rest two trips to memory.  Into 8 bits
+// 6.0 us in a graph for 4.3, 65 workgroups in place of 260; 6144 x 2080 4.9 for 4.2.
 constexpr int kOneWaves = mx4::kOneWaves;
 __host__ __device__ constexpr int one_token_bytes(int width) { return mx4::one_lds_bytes(width); }
 __host__ __device__ constexpr int one_lds_bytes(int width) { return one_token_bytes(width) + (blocks_of(width) + 15) / 16 * 16; }
@@ -356,8 +357,11 @@ void launch_few(const Product8Args &p, hipStream_t s) {
 // from 16 (l / 32) on and the 16 from 32 + 16 (l / 32) on, and each side's scale for block l / 32 as one byte of a
 // register.  Scales come through registers, sixteen (four steps') of a row or token a thread, and LDS: loaded by each
 // wavefront for itself they were two of three requests to L2, which bound the launch.  8192 tokens through 2080 x 6144
-// take 90 us a call (2.3 PFLOP/s), through 8192 x 8192 410 to 420 in a graph (2.6); of zeros 70 and 300: power is the
-// bound, matrix cores are busy for three quarters of the loop's cycles at 1.7 to 2.0 GHz. Without the fetches of codes
+// take 90 us a call (2.3 PFLOP/s), through 8192 x 8192 410 to 420 in a graph (2.6); of zeros, whose clock is higher, 70 and
+// 300.  By the row's length 10 us of the 87 to 90 are a launch, the start and y; the turns run at 84 % of the MFMAs' rate
+// from registers, of zeros as of random values, rows that are not there in the last tile among what they multiply (2304
+// rows take as long as 2080). Into 8 bits 85 to 92 us.  A part asks for kStages - 1 steps behind its last, which nobody
+// reads.  Without the fetches of codes
 // it took 22 % less, without scales 11, without y's stores 9; 256 x 256 by 8 wavefronts as by 16 within 2 %, three
 // stages as two; two steps a turn, fetches after the first products, a higher priority for wavefronts in their
 // products: within 2 %. Smaller calls are bound by what a compute unit moves from L2 into LDS: 28 to 30 bytes a cycle,

