@@ -5,8 +5,8 @@ import torch
 
 from oracle import block_oracle as bo
 from oracle import mx4_oracle as mo
-from qmoe_amd import _lib, mx8
-from test_gpu_mx4 import host
+from qmoe_amd import _lib, mx4, mx8
+from test_gpu_mx4 import host, matrix, within
 
 # One row and one token of 17 values that a search came upon: 64.2836 by 64 bits, 64.2497 by the matrix cores, 64.0 in bf16.
 X = [-0.34375, -128, -0.03515625, -0.1875, -0.5625, -0.234375, 0.109375, 0.203125, 0.025390625, -0.078125, 0.25, -0.171875, 0.0068359375,
@@ -94,3 +94,21 @@ def test_sums_of_a_block_to_the_bit(which, form):
     got = mx8.product(*given(np.repeat(x, 2, 0), w, np.repeat(xs, 2, 0), ws), 17)
     assert (host(got) == 64.0).all()
     assert mx8.product(*given(x, w, xs, ws), 17).item() == 64.5          # one token: nothing is cut off
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('tokens,height,width', [(1, 70, 500), (2, 5, 32), (61, 300, 1000), (333, 515, 2080), (1500, 200, 333)])
+def test_sums_in_fp32_of_the_same_activations(tokens, height, width):
+    """As bf16, which holds them exactly, through the same matrix: no more off than fp32 sums are."""
+    rng = np.random.default_rng(tokens)
+    nb = mo.blocks_of(width)
+    x = rng.integers(0, 256, (tokens, 32 * nb)).astype(np.uint8)
+    x[(x & 127) == 127] -= 1
+    x[:, width:] = 0
+    xs = rng.integers(117, 122, (tokens, nb)).astype(np.uint8)
+    value = bo.dequantize8(x, xs, width)
+    codes, scales, w = matrix(height, width, 9, spread=2)
+    back = mx8.dequantize(torch.from_numpy(x).cuda(), torch.from_numpy(xs).cuda(), width)
+    assert np.array_equal(host(back), value)
+    exact, off = value @ w.T, (width + 2) * 2.0 ** -23 * (np.abs(value) @ np.abs(w).T)
+    within(mx4.product(back, codes, scales), *bo.to_bf16(exact, off))
